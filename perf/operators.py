@@ -24,8 +24,7 @@ own = False
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PACKAGE = os.path.join(ROOT, "pallas-mosaic-gpu_b200")
 DEVICE = "cuda"
-E4M3_MAX = 448.0
-MIN_EXPONENT, MAX_EXPONENT = -64, 119
+MIN_EXPONENT, MAX_EXPONENT = -64, 120
 
 
 def _library():
