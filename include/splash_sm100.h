@@ -67,8 +67,9 @@ typedef struct SplashParams {
    * NULL when partial blocks are computed from `mask_desc`.  (The reference streams
    * int8 blocks, splash_attention_mgpu/mask_info.py:113-120.) */
   const int8_t* partial_blocks;
-  /* [mask_heads, 4] int32 {lo, hi, chunk, 0}: a key is visible iff
-   * lo <= kv_pos - q_pos <= hi and (chunk == 0 or q_pos/chunk == kv_pos/chunk).
+  /* [mask_heads, 4] int32 {lo, hi, chunk, sinks}: a key is visible iff
+   * (lo <= kv_pos - q_pos or kv_pos < sinks) and kv_pos - q_pos <= hi and
+   * (chunk == 0 or q_pos/chunk == kv_pos/chunk).  With a chunk, sinks is 0.
    * NULL when partial blocks are dense or when there are no partial blocks. */
   const int32_t* mask_desc;
   /* ---- results ------------------------------------------------------------ */
@@ -183,6 +184,63 @@ int64_t splash_bwd_fused_workspace_bytes(const SplashParams* p);
  * whose GPU work overlaps (different streams, no ordering between them) race on it --
  * serialise them. */
 int splash_bwd_fused_static(const SplashParams* p, void* stream);
+
+/* ---- Rotary positions ---------------------------------------------------- */
+
+/* Pair i of every row of q and k turns by positions[axis[i]] * f_i:
+ *   (a, b) -> (a cos - b sin, b cos + a sin), q also times q_scale;  inverse: the transpose, as the
+ * backward pass wants it.  No counterpart in the reference, whose callers rotate with JAX operations. */
+typedef struct SplashRotaryParams {
+  const void* q;           /* [batch, q_heads, len, head_dim] bf16/f16, strides below           */
+  const void* k;           /* [batch, k_heads, len, head_dim] or NULL                           */
+  void* q_out;             /* contiguous, like q                                                */
+  void* k_out;             /* contiguous, like k                                                */
+  const void* positions;   /* int32, or int64 with pos_is_64; any whole number                  */
+  const uint64_t* turns;   /* [pairs] f_i / (2 pi), modulo 1, in units of 2^-64                 */
+  const int32_t* axis;     /* [pairs] axis of each pair                                         */
+  int64_t q_stride[3];     /* elements from one batch row / head / position to the next         */
+  int64_t k_stride[3];
+  int64_t pos_stride[3];   /* batch row / axis / position                                       */
+  int32_t batch, q_heads, k_heads, len, head_dim;
+  int32_t pairs;           /* rotated pairs; numbers 2 * pairs .. head_dim - 1 of a row are kept */
+  int32_t dtype;           /* SPLASH_DTYPE_*                                                    */
+  int32_t adjacent;        /* pairs are (2i, 2i + 1) instead of (i, i + pairs)                  */
+  int32_t inverse, pos_is_64;
+  float q_scale;
+} SplashRotaryParams;
+
+int splash_rotary(const SplashRotaryParams* p, void* stream);
+
+/* ---- Paged cache of keys and values --------------------------------------- */
+
+/* Token t of sequence b lies in page page_table[b, t / page_size], row t % page_size; a page id outside
+ * [0, num_pages) and a token behind the table stand for no page: nothing is written there, zeros are read.
+ * 8-bit caches hold e4m3 codes and one exponent e per (token, head): x = code * 2^e, e the smallest whole
+ * number in [-64, 120] with max|x| <= 448 * 2^e; rows with an infinity or NaN have e = -128 and read as NaN.
+ * No counterpart in the reference. */
+typedef struct SplashCacheParams {
+  void* k_cache;              /* [num_pages, kv_heads, page_size, head_dim], 16-bit or e4m3, 16-byte aligned */
+  void* v_cache;
+  int8_t* k_exponent;         /* [num_pages, kv_heads, page_size]; NULL for 16-bit caches       */
+  int8_t* v_exponent;
+  const int32_t* page_table;  /* [batch, table_width], rows table_stride apart                  */
+  const int32_t* lengths;     /* write: [batch] index of each sequence's first new token; read: tokens to read */
+  const int32_t* counts;      /* write: [batch] new tokens of each sequence, or NULL: len       */
+  const void* k;              /* write: [batch, kv_heads, len, head_dim], strides below, 16-byte aligned rows */
+  const void* v;
+  void* k_out;                /* read: [batch, kv_heads, len, head_dim] contiguous; zeros from lengths[b] on */
+  void* v_out;
+  int64_t k_stride[3];        /* elements from one batch row / head / token to the next         */
+  int64_t v_stride[3];
+  int64_t table_stride;
+  int32_t batch, kv_heads, len, head_dim;
+  int32_t num_pages, page_size, table_width;
+  int32_t dtype;              /* of k, v, k_out and v_out                                       */
+  int32_t quantized;
+} SplashCacheParams;
+
+int splash_cache_write(const SplashCacheParams* p, void* stream);
+int splash_cache_read(const SplashCacheParams* p, void* stream);
 
 /* Copies the 4-int status word to the host after synchronising `stream`; returns
  * SPLASH_OK, SPLASH_DEVICE_TIMEOUT or SPLASH_CUDA_ERROR. `host_out` may be NULL. */

@@ -68,10 +68,10 @@ def emulate_forward(info, q, k, v, segment_ids=None, *, mask_value,
           if info.partial_mask_blocks is not None:
             vis &= info.partial_mask_blocks[info.mask_block[mh, qi, s]].astype(bool)
           else:
-            lo, hi, chunk, _ = info.mask_descriptors[mh]
+            lo, hi, chunk, sinks = info.mask_descriptors[mh]
             qp = np.arange(qi * bq, (qi + 1) * bq)[:, None]
             kp = np.arange(j * bkv, (j + 1) * bkv)[None, :]
-            vis &= (kp - qp >= lo) & (kp - qp <= hi)
+            vis &= ((kp - qp >= lo) | (kp < sinks)) & (kp - qp <= hi)
             if chunk:
               vis &= (qp // chunk) == (kp // chunk)
         else:

@@ -441,6 +441,7 @@ splash_bwd_col_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
             band_lo = max(band_lo, kv_pos - (start + chunk - 1));
             band_hi = min(band_hi, kv_pos - start);
           }
+          if (kv_pos < a.mask_desc[cur_mh * 4 + 3]) band_lo = -(1 << 30);  // a sink is seen from any distance
         }
         if (!warp_wait(SPLASH_CBAR(full, slot), phase, ctx, kBSiteEwFull, t)) { alive = false; break; }
         const int buf = t & 1;

@@ -274,7 +274,9 @@ splash_bwd_row_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       }
     } else {
       int band_lo = -(1 << 30), band_hi = (1 << 30);
+      int sinks = 0;  // keys below this position are seen from behind the window too
       if (a.mask_desc) {
+        sinks = a.mask_desc[mh * 4 + 3];
         band_lo = a.mask_desc[mh * 4 + 0];
         band_hi = a.mask_desc[mh * 4 + 1];
         const int chunk = a.mask_desc[mh * 4 + 2];
@@ -314,10 +316,11 @@ splash_bwd_row_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           uint32_t vis = row_on ? 0xffffffffu : 0u;
           if (partial && !a.has_dense) {
             const int d0 = kv0 + c * 32 - q_pos;
+            const int sink_cols = sinks - (kv0 + c * 32);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const int d = d0 + i;
-              if (d < band_lo || d > band_hi) vis &= ~(1u << i);
+              if ((d < band_lo && i >= sink_cols) || d > band_hi) vis &= ~(1u << i);
             }
           }
           if (partial && a.has_dense) {

@@ -648,6 +648,7 @@ splash_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             band_lo = max(band_lo, kv_pos - (start + chunk - 1));
             band_hi = min(band_hi, kv_pos - start);
           }
+          if (kv_pos < a.mask_desc[cur_mh * 4 + 3]) band_lo = -(1 << 30);  // a sink is seen from any distance
         }
         const int q0 = qblk * 128 + col0;  // sequence position of this thread's first column
         // Visibility of this thread's 64 columns (bit i of word c: column c * 32 + i).

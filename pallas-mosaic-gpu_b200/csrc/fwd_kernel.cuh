@@ -507,7 +507,9 @@ splash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     } else {
       // Per-row band in units of (kv_pos - q_pos); a chunk restriction folds in.
       int band_lo = -(1 << 30), band_hi = (1 << 30);
+      int sinks = 0;  // keys below this position are seen from behind the window too
       if (a.mask_desc) {
+        sinks = a.mask_desc[mh * 4 + 3];
         band_lo = a.mask_desc[mh * 4 + 0];
         band_hi = a.mask_desc[mh * 4 + 1];
         const int chunk = a.mask_desc[mh * 4 + 2];
@@ -578,10 +580,20 @@ splash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const bool partial = kind_now == SPLASH_BLOCK_PARTIAL;
         if (partial && !has_dense) {
           const int d0 = j_now * BKV - q_pos;
+          const int sink_cols = sinks - j_now * BKV;  // columns of this block that are sinks
+          if (sink_cols <= 0) {
 #pragma unroll
-          for (int i = 0; i < BKV; ++i) {
-            const int d = d0 + i;
-            if (d < band_lo || d > band_hi) sv[i] = -INFINITY;
+            for (int i = 0; i < BKV; ++i) {
+              const int d = d0 + i;
+              if (d < band_lo || d > band_hi) sv[i] = -INFINITY;
+            }
+          } else {
+            // Apart from the blocks without sinks, whose two comparisons per element it would make three.
+#pragma unroll
+            for (int i = 0; i < BKV; ++i) {
+              const int d = d0 + i;
+              if ((d < band_lo && i >= sink_cols) || d > band_hi) sv[i] = -INFINITY;
+            }
           }
         }
         if (partial && has_dense) {

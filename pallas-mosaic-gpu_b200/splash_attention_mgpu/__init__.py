@@ -4,7 +4,9 @@ Same import surface as the reference package (`splash_attention_mgpu/__init__.py
 """
 
 from .config import DEFAULT_MASK_VALUE, BlockSizes, SegmentIds
+from .kv_cache import KVCache, make_kv_cache
 from .mask_info import GpuMaskInfo, process_mask
+from .rotary import RotaryEmbedding, make_rotary
 from .splash_attention import (
     SplashAttentionKernel,
     attention_reference,
@@ -24,7 +26,7 @@ from .splash_attention_mask import (
 
 __all__ = [
     "BlockSizes", "CausalMask", "ChunkedCausalMask", "DEFAULT_MASK_VALUE",
-    "FullMask", "GpuMaskInfo", "LocalMask", "Mask", "MultiHeadMask",
-    "NumpyMask", "SegmentIds", "SplashAttentionKernel", "attention_reference",
-    "check_device_status", "make_splash_mha", "make_splash_mqa", "process_mask",
+    "FullMask", "GpuMaskInfo", "KVCache", "LocalMask", "Mask", "MultiHeadMask",
+    "NumpyMask", "RotaryEmbedding", "SegmentIds", "SplashAttentionKernel", "attention_reference",
+    "check_device_status", "make_kv_cache", "make_rotary", "make_splash_mha", "make_splash_mqa", "process_mask",
 ]

@@ -45,6 +45,9 @@ EXPORTED_SYMBOLS = (
     "splash_status_string",
     "splash_last_error",
     "splash_selftest_umma",
+    "splash_rotary",
+    "splash_cache_write",
+    "splash_cache_read",
 )
 
 
@@ -71,6 +74,33 @@ class SplashParams(Structure):
       ("num_stages", c_int32), ("sub_block", c_int32),
       ("mask_value", c_float), ("soft_cap", c_float),
       ("seg_ranges", c_void_p),
+  ]
+
+
+class SplashRotaryParams(Structure):
+  """Mirror of `struct SplashRotaryParams`."""
+
+  _fields_ = [
+      ("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p), ("positions", c_void_p),
+      ("turns", c_void_p), ("axis", c_void_p),
+      ("q_stride", c_int64 * 3), ("k_stride", c_int64 * 3), ("pos_stride", c_int64 * 3),
+      ("batch", c_int32), ("q_heads", c_int32), ("k_heads", c_int32), ("len", c_int32), ("head_dim", c_int32),
+      ("pairs", c_int32), ("dtype", c_int32), ("adjacent", c_int32), ("inverse", c_int32), ("pos_is_64", c_int32),
+      ("q_scale", c_float),
+  ]
+
+
+class SplashCacheParams(Structure):
+  """Mirror of `struct SplashCacheParams`."""
+
+  _fields_ = [
+      ("k_cache", c_void_p), ("v_cache", c_void_p), ("k_exponent", c_void_p), ("v_exponent", c_void_p),
+      ("page_table", c_void_p), ("lengths", c_void_p), ("counts", c_void_p),
+      ("k", c_void_p), ("v", c_void_p), ("k_out", c_void_p), ("v_out", c_void_p),
+      ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3), ("table_stride", c_int64),
+      ("batch", c_int32), ("kv_heads", c_int32), ("len", c_int32), ("head_dim", c_int32),
+      ("num_pages", c_int32), ("page_size", c_int32), ("table_width", c_int32),
+      ("dtype", c_int32), ("quantized", c_int32),
   ]
 
 
@@ -123,6 +153,11 @@ def load():
                                        c_int32, c_int32, c_int32, c_int32,
                                        c_void_p, c_void_p]
   lib.splash_selftest_umma.restype = c_int
+  for name, params in (("splash_rotary", SplashRotaryParams), ("splash_cache_write", SplashCacheParams),
+                       ("splash_cache_read", SplashCacheParams)):
+    fn = getattr(lib, name)
+    fn.argtypes = [POINTER(params), c_void_p]
+    fn.restype = c_int
   _lib = lib
   return lib
 

@@ -10,7 +10,7 @@ the reference takes it from a third-party library.
 Differences from the reference, all additive:
   * classification of computable masks is analytic (O(blocks), never O(S^2));
   * compaction is vectorised numpy instead of a Python double loop;
-  * `mask_descriptors` carries a per-head band descriptor `(lo, hi, chunk)` that
+  * `mask_descriptors` carries a per-head band descriptor `(lo, hi, chunk, sinks)` that
     the CUDA kernels evaluate in registers, so a MultiHeadMask made only of
     computable masks needs no dense blocks;
   * identical dense partial blocks are stored once.
@@ -56,7 +56,7 @@ class GpuMaskInfo:
   dkv_block_kind: np.ndarray  # i32[mask_heads, kv_blocks, max_dkv_steps]
   dkv_mask_block: np.ndarray | None
   partial_mask_blocks_t: np.ndarray | None  # int8[n, block_kv, block_q]
-  # i32[mask_heads, 4]: (lo, hi, chunk, 0) band descriptor per mask head; None
+  # i32[mask_heads, 4]: (lo, hi, chunk, sinks) band descriptor per mask head; None
   # when partial blocks are stored densely.
   mask_descriptors: np.ndarray | None = None
 
@@ -78,8 +78,8 @@ def _classify_band(mask, block_q: int, block_kv: int) -> np.ndarray:
   c0 = (np.arange(kv_len // block_kv, dtype=np.int64) * block_kv)[None, :]
   r1, c1 = r0 + block_q - 1, c0 + block_kv - 1
   dmin, dmax = c0 - r1, c1 - r0  # range of kv - q inside the block
-  all_vis = (dmin >= lo) & (dmax <= hi)
-  any_vis = (dmax >= lo) & (dmin <= hi)
+  all_vis = ((dmin >= lo) | (c1 < mask.num_sinks)) & (dmax <= hi)
+  any_vis = ((dmax >= lo) | (c0 < mask.num_sinks)) & (dmin <= hi)
   if chunk:
     same = ((r0 // chunk == r1 // chunk) & (c0 // chunk == c1 // chunk)
             & (r0 // chunk == c0 // chunk))
@@ -216,7 +216,7 @@ def process_mask(
   mask_function = mask_descriptors = None
   if computable:
     mask_function = _make_mask_function(heads)
-    mask_descriptors = np.array([list(h.band()) + [0] for h in heads], np.int32)
+    mask_descriptors = np.array([list(h.band()) + [h.num_sinks] for h in heads], np.int32)
   elif (block_mask == PARTIAL).any():
     partial_mask_blocks, mask_next = _extract_partial_blocks(
         heads, block_mask, block_q, block_kv)

@@ -8,7 +8,7 @@ the contract the reference's call sites rely on
 `tools/fuzz.py:61-76`):
 
   FullMask((q, kv)); CausalMask((q, kv), offset=0);
-  LocalMask((q, kv), (left, right), offset); ChunkedCausalMask((q, kv), chunk_size=c);
+  LocalMask((q, kv), (left, right), offset, num_sinks=0); ChunkedCausalMask((q, kv), chunk_size=c);
   NumpyMask(bool[q, kv]); MultiHeadMask([mask, ...])
 
   mask.shape       -> (q_len, kv_len)  ((heads, q_len, kv_len) for MultiHeadMask)
@@ -17,12 +17,14 @@ the contract the reference's call sites rely on
 Element semantics (q = query position, kv = key position):
 
   causal          q + offset >= kv
-  local           q + offset - left <= kv <= q + offset + right   (None = unbounded)
+  local           q + offset - left <= kv <= q + offset + right   (None = unbounded);
+                  with num_sinks also kv < num_sinks, as far as kv <= q + offset + right
   chunked causal  q >= kv  and  q // chunk == kv // chunk
   full            always visible
 
 Every computable mask reduces to one *band descriptor* `(lo, hi, chunk)`:
-visible iff `lo <= kv - q <= hi` and (`chunk == 0` or same chunk).  The CUDA
+visible iff `lo <= kv - q <= hi` and (`chunk == 0` or same chunk), and a number of
+sinks, positions below which `lo` does not count.  The CUDA
 kernels evaluate that descriptor in registers for partial blocks, which is how
 a per-head mix of computable masks stays free of dense mask blocks.
 """
@@ -85,6 +87,8 @@ class Mask:
 class _ComputableMask(Mask):
   """A mask defined by a band descriptor; never materialised as a whole."""
 
+  num_sinks = 0  # keys below this position are visible however far behind they lie
+
   def __init__(self, shape: tuple[int, int]):
     if len(shape) != 2:
       raise ValueError(f"mask shape must be (q_len, kv_len), got {shape}")
@@ -101,6 +105,8 @@ class _ComputableMask(Mask):
     kv_ids = np.asarray(kv_ids)
     diff = kv_ids - q_ids
     vis = (diff >= lo) & (diff <= hi)
+    if self.num_sinks:
+      vis = vis | ((kv_ids < self.num_sinks) & (diff <= hi))
     if chunk:
       vis = vis & ((q_ids // chunk) == (kv_ids // chunk))
     return vis
@@ -118,13 +124,14 @@ class _ComputableMask(Mask):
 
   def __eq__(self, other):
     return (type(self) is type(other) and self.shape == other.shape
-            and self.band() == other.band())
+            and self.band() == other.band() and self.num_sinks == other.num_sinks)
 
   def __hash__(self):
-    return hash((type(self).__name__, self.shape, self.band()))
+    return hash((type(self).__name__, self.shape, self.band(), self.num_sinks))
 
   def __repr__(self):
-    return f"{type(self).__name__}(shape={self.shape}, band={self.band()})"
+    sinks = f", num_sinks={self.num_sinks}" if self.num_sinks else ""
+    return f"{type(self).__name__}(shape={self.shape}, band={self.band()}{sinks})"
 
 
 class FullMask(_ComputableMask):
@@ -146,14 +153,21 @@ class CausalMask(_ComputableMask):
 
 
 class LocalMask(_ComputableMask):
-  """Sliding window: q + offset - left <= kv <= q + offset + right."""
+  """Sliding window: q + offset - left <= kv <= q + offset + right.
+
+  The first `num_sinks` keys stay visible behind the window, up to its right edge.  They are positions of the kv
+  sequence: segment ids still keep them from queries of another segment.
+  """
 
   def __init__(self, shape, window_size: tuple[int | None, int | None],
-               offset: int = 0):
+               offset: int = 0, num_sinks: int = 0):
     super().__init__(shape)
     left, right = window_size
     self.window_size = (left, right)
     self.offset = int(offset)
+    if num_sinks < 0:
+      raise ValueError(f"num_sinks must not be negative, got {num_sinks}")
+    self.num_sinks = min(int(num_sinks), self.shape[1])
 
   def band(self):
     left, right = self.window_size
