@@ -242,6 +242,44 @@ typedef struct SplashCacheParams {
 int splash_cache_write(const SplashCacheParams* p, void* stream);
 int splash_cache_read(const SplashCacheParams* p, void* stream);
 
+/* ---- Attention over the paged cache ---------------------------------------- */
+
+/* New tokens of every sequence against the keys in the cache, their own among them.  lengths[b] tokens of
+ * sequence b are in the cache, the last counts[b] (NULL: n; at most lengths[b]) of them new: row i of q[b] is
+ * new token i, with before[b] = lengths[b] - counts[b] tokens in front of it; rows from counts[b] on are padding
+ * and give zeros and lse = mask_value, as do rows that see no key.
+ *   run  (parents NULL): token i has position before + i and sees the keys at positions 0 .. before + i;
+ *   tree: token i follows token parents[b, i] < i of its sequence, or (any other number) the last one in front;
+ *     it has the position behind that one's and sees the keys in front, its ancestors and itself.
+ * window_left >= 0 leaves of those the ones at positions >= its own - window_left, and < num_sinks.
+ * Keys without a page (see SplashCacheParams) are seen by nobody.  No counterpart in the reference. */
+typedef struct SplashCachedParams {
+  const void* q;              /* [batch, heads, n, head_dim] bf16/f16, pre-scaled, contiguous, 16-byte aligned */
+  const void* k_cache;        /* as in SplashCacheParams                                        */
+  const void* v_cache;
+  const int8_t* k_exponent;   /* 16-byte aligned; NULL for 16-bit caches                        */
+  const int8_t* v_exponent;
+  const int32_t* page_table;  /* [batch, table_width], rows table_stride apart                  */
+  const int32_t* lengths;     /* [batch]                                                        */
+  const int32_t* counts;      /* [batch] or NULL                                                */
+  const int32_t* parents;     /* [batch, n], rows parents_stride apart (0: one tree), or NULL; n <= 128 */
+  void* out;                  /* [batch, heads, n, head_dim], 16-byte aligned                   */
+  float* lse_out;             /* [batch, heads, n] natural log, or NULL                         */
+  int32_t* status;            /* 4 x int32, see above                                           */
+  int64_t table_stride, parents_stride;
+  int32_t batch, heads, kv_heads, n, head_dim;
+  int32_t num_pages, page_size, table_width;
+  int32_t dtype;              /* of q and out, and of a 16-bit cache                            */
+  int32_t quantized;
+  int32_t window_left;        /* < 0: no window                                                 */
+  int32_t num_sinks;
+  float mask_value, soft_cap;
+} SplashCachedParams;
+
+/* Bytes of workspace (16-byte aligned, contents of no interest before or after) of a call; 0 for a call that is refused. */
+int64_t splash_cached_workspace_bytes(const SplashCachedParams* p);
+int splash_cached_fwd(const SplashCachedParams* p, void* workspace, int64_t bytes, void* stream);
+
 /* Copies the 4-int status word to the host after synchronising `stream`; returns
  * SPLASH_OK, SPLASH_DEVICE_TIMEOUT or SPLASH_CUDA_ERROR. `host_out` may be NULL. */
 int splash_read_status(const int32_t* status, int32_t* host_out, void* stream);

@@ -1,0 +1,957 @@
+// Attention of a few new tokens per sequence over a paged cache: one token, a run of tokens, or a tree of drafted ones.
+//
+// Mathematics.  A unit of work is (sequence, row tile, kv head): up to R rows -- the new tokens of the heads that share
+// the kv head -- against the keys its rows can see, in tiles of 128 keys:  S = Q K^T, online softmax, O += P V.
+//
+// What bounds it: HBM.  2 * 128 * head_dim numbers a tile are read once for all rows, and up to 128 rows of products
+// over them cost the tensor core less time than their transfer.  So everything is arranged to keep a ring of loads full:
+//   * The tiles of all units stand in one line that is cut into equal shares, one per CTA (one CTA per SM), whatever the
+//     lengths of the sequences are.  A unit that several CTAs share leaves partial results (unnormalised O, maximum and
+//     sum per row, f32) for cached_finish_kernel, which adds them in the order of the keys: the same bits every time.
+//   * One producer warp walks the line ahead of the others, across units: page ids a tile ahead, one TMA box per page.
+//   * Rows are few, so the 128 rows of an MMA are used otherwise: Q is laid into shared memory 128 / R times, and each
+//     copy's warps take the exponentials of their own part of the tile's keys (P is zero elsewhere); the copies' results
+//     are added like partial ones.  A softmax warp of a one-token call thus works on 32 of 128 keys.
+//   * Two warpgroups take the tiles in turn, each with maxima, sums and O columns of its own, so that one's softmax runs
+//     under the other's products.
+//
+// 8-bit caches are not widened on the way: e4m3 keys and values are operands of the MMA as they lie in the cache, and
+// the 16-bit Q and the probabilities are split into e4m3 terms instead, which are few:
+//   * q * 2^-eq = q1 + q2 (+ q3 for f16), each term what the ones before leave; S sums their products.  bf16 has 8 bits,
+//     a term 4: nothing is lost but below 2^-19 of the row's largest number.
+//   * 2^ek of a key scales its column of S; 2^ev of a value scales its column of P, and the running maximum is one of
+//     s + ev, so that the scaled probabilities stay within 2^8.
+//   * P = p1 + p2 / 16 with p1, p2 e4m3: about 8 bits, as a bf16 P has.  Half of the copies of the rows carry p1, half p2.
+#pragma once
+
+#include <stddef.h>
+
+#include "../../include/splash_sm100.h"
+#include "ptx.cuh"
+
+namespace splash {
+
+constexpr int kCachedThreads = 384;
+constexpr int kCachedTile = 128;        // keys per tile
+constexpr int kCachedMaxSlots = 12;
+constexpr int kCachedAuxSlots = 16;     // exponents of a tile; more than tiles can be on their way (see the producer)
+constexpr int kCachedMaxTree = 128;     // nodes of a drafted tree
+constexpr float kCachedLog2e = 1.4426950408889634f;
+constexpr float kCachedLn2 = 0.6931471805599453f;
+
+struct CachedArgs {
+  const void* q;
+  const int8_t* k_exponent;
+  const int8_t* v_exponent;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  const int32_t* counts;
+  const int32_t* parents;
+  void* out;
+  float* lse_out;
+  int32_t* status;
+  int32_t* starts;    // [batch * row_tiles + 1] first tile of each (sequence, row tile) in the line, and its length
+  float* part_o;      // [2 * CTAs, R, D]
+  float2* part_ml;    // [2 * CTAs, R]: maximum (powers of 2) and sum
+  int64_t table_stride, parents_stride;
+  int32_t batch, heads, kv_heads, n, rows, row_tiles, row_cap;  // rows = heads / kv_heads * n
+  int32_t num_pages, page_size, table_width;
+  int32_t window, sinks;  // window < 0: none
+  float mask_value, soft_cap;
+};
+
+// What the rows of one (sequence, row tile) can see, the same for every kv head.
+struct CachedGeom {
+  int count, before;   // new tokens; tokens in front of them
+  int i0, i1;          // new tokens among the rows of the tile: [i0, i1)
+  int lo, hi, sink_hi; // keys that some row sees lie in [lo, hi) or [0, sink_hi)
+  int first, sink_tiles, tiles;  // first tile of the window, tiles of sinks in front of it, all tiles
+};
+
+__device__ __forceinline__ CachedGeom cached_geom(const CachedArgs& a, int entry) {
+  CachedGeom g;
+  const int b = entry / a.row_tiles, rt = entry - b * a.row_tiles;
+  const int capacity = a.table_width * a.page_size;  // (checked on the host to fit)
+  const int len = min(max(a.lengths[b], 0), capacity);
+  g.count = min(a.counts ? min(max(a.counts[b], 0), a.n) : a.n, len);
+  g.before = len - g.count;
+  const int r0 = rt * a.row_cap, r1 = min(a.rows, r0 + a.row_cap);
+  g.i0 = 0;
+  g.i1 = g.count;
+  if (r1 - r0 < a.n && r0 % a.n <= (r1 - 1) % a.n) {  // rows of one head
+    g.i0 = r0 % a.n;
+    g.i1 = min(g.count, (r1 - 1) % a.n + 1);
+  }
+  g.hi = g.before + g.i1;
+  const bool tree = a.parents != nullptr;
+  g.lo = a.window < 0 ? 0 : max(0, g.before + (tree ? 0 : g.i0) - a.window);
+  g.sink_hi = a.window < 0 ? 0 : min(a.sinks, g.lo);
+  g.first = g.lo / kCachedTile;
+  g.sink_tiles = min((g.sink_hi + kCachedTile - 1) / kCachedTile, g.first);
+  g.tiles = g.i0 < g.i1 ? g.sink_tiles + (g.hi + kCachedTile - 1) / kCachedTile - g.first : 0;
+  return g;
+}
+
+// First tile of CTA c's share of a line of `total` tiles cut for `ctas` CTAs.
+__host__ __device__ __forceinline__ int cached_share(int c, int total, int ctas) {
+  return static_cast<int>(static_cast<long long>(c) * total / ctas);
+}
+
+// A CTA's way along its share: one segment (a unit or the part of it that falls into the share) after the other.
+struct CachedCursor {
+  int entry, head, tile, left;  // of the next segment; tiles left in the share
+  CachedGeom g;
+  int seg_tile, seg_n, seg_entry, seg_head;  // the current segment
+  bool whole;                                // it is all of its unit
+
+  __device__ __forceinline__ void start(const CachedArgs& a, int e, int h, int t, int n) {
+    entry = e; head = h; tile = t; left = n;
+    if (left > 0) g = cached_geom(a, entry);
+  }
+  __device__ __forceinline__ bool next(const CachedArgs& a) {
+    if (left <= 0) return false;
+    if (head == a.kv_heads) {
+      head = 0;
+      const int entries = a.batch * a.row_tiles;
+      do {
+        if (++entry >= entries) return false;
+        g = cached_geom(a, entry);
+      } while (g.tiles == 0);
+    }
+    seg_entry = entry;
+    seg_head = head;
+    seg_tile = tile;
+    seg_n = min(g.tiles - tile, left);
+    whole = tile == 0 && seg_n == g.tiles;
+    left -= seg_n;
+    tile = 0;
+    ++head;
+    return true;
+  }
+  // First key of the segment's i-th tile.
+  __device__ __forceinline__ int key0(int i) const {
+    const int t = seg_tile + i;
+    return (t < g.sink_tiles ? t : g.first + t - g.sink_tiles) * kCachedTile;
+  }
+};
+
+enum CachedSite : int {
+  kCSiteLoadEmpty = 301, kCSiteLoadQ, kCSiteMmaQ, kCSiteMmaFull, kCSiteMmaP, kCSiteMmaO, kCSiteSmxS, kCSiteSmxV,
+  kCSiteSmxSync, kCSiteSmxDone, kCSiteConvQ, kCSiteSmxAux,
+};
+
+template <int D, bool BF16, bool QUANT, int KG>
+struct CachedLayout {
+  static constexpr int kCopies = QUANT ? 2 * KG : KG;      // copies of the rows among the 128 of an MMA
+  static constexpr int kRows = 128 / kCopies;              // R
+  static constexpr int kKeys = kCachedTile / KG;           // keys whose probabilities a row's thread computes
+  static constexpr int kItem = QUANT ? 1 : 2;
+  static constexpr int kRowBytes = D * kItem;              // of a key
+  static constexpr int kBoxBytes = kRowBytes < 128 ? kRowBytes : 128;  // swizzle span = inner extent of a TMA box
+  static constexpr int kBoxes = kRowBytes / kBoxBytes;
+  static constexpr int kBoxElems = kBoxBytes / kItem;
+  static constexpr int kSlotBytes = kCachedTile * kRowBytes;
+  static constexpr int kTerms = QUANT ? (BF16 ? 2 : 3) : 1;
+  static constexpr int kQTerm = 128 * kRowBytes;
+  static constexpr int kQBytes = kTerms * kQTerm;
+  static constexpr int kStageStride = 36;                  // words per row of the staging area (32 used)
+  static constexpr int kStageBytes = 256 * kStageStride * 4;
+  // Behind the staging area: maxima and sums, barriers, then (8 bit) exponents, scales, row scales, and the tree.
+  static constexpr int kMlBytes = 256 * 8;
+  static constexpr int kBarBytes = 512;
+  static constexpr int kAuxBytes = QUANT ? kCachedAuxSlots * 2 * kCachedTile : 0;
+  static constexpr int kScaleBytes = QUANT ? 8 * kKeys * 12 : 0;  // per warp: three numbers for each of its keys
+  static constexpr int kQScaleBytes = QUANT ? 2 * 128 * 4 : 0;
+  static constexpr int kTreeBytes = kCachedMaxTree * 4 + 128 * 8 * 4;
+  static constexpr int kFixed = 1024 + kQBytes + kStageBytes + kMlBytes + kBarBytes + kAuxBytes + kScaleBytes + kQScaleBytes + kTreeBytes;
+  static constexpr int kSlotsFit = (227 * 1024 - kFixed) / kSlotBytes;
+  static constexpr int kSlots = kSlotsFit < kCachedMaxSlots ? kSlotsFit : kCachedMaxSlots;
+  static_assert(kSlots >= 4, "two tiles have to fit");
+  static constexpr int kSmem = kFixed + kSlots * kSlotBytes;
+  static constexpr int kOCol = 256;  // S of the two warpgroups | O of the two
+  // Registers of the warpgroups: 384 * 168 at launch = 256 * 208 + 128 * 88 = 256 * 184 + 128 * 136.
+  static constexpr int kSoftmaxRegs = kKeys == 128 ? 208 : 184;
+  static constexpr int kLoadRegs = kKeys == 128 ? 88 : 136;
+};
+
+struct CachedBarriers {
+  uint64_t full[kCachedMaxSlots], empty[kCachedMaxSlots];
+  uint64_t s_ready[2], p_ready[2];
+  uint64_t q_full, q_free, o_done, o_free, sync;
+  uint32_t tmem_base, abort_flag, dead;
+  int32_t first_entry, first_head, first_tile, num_tiles;
+};
+static_assert(sizeof(CachedBarriers) <= 512, "");
+
+// ---- 8-bit operands -------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t two) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ float exponent_scale(int e) {  // -128 marks a row that was not finite
+  return e == -128 ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+// Warp-collective forms as in ptx.cuh, for 8-bit operands (kind::f8f6f4, e4m3 by e4m3).
+__device__ __forceinline__ void umma8_ss2_w(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      ".reg .b64 da, db;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n\t"
+      "}\n"
+      ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma8_ts2_w(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      ".reg .b64 db;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], db, %4, p;\n\t"
+      "}\n"
+      ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Upper half of a shared-memory descriptor of tiles with 128- or 64-byte rows, swizzled over their rows.
+template <int BOX_BYTES>
+__host__ __device__ constexpr uint32_t cached_desc_hi() {
+  return (((8u * BOX_BYTES) >> 4) & 0x3fff) | (1u << 14) | ((BOX_BYTES == 128 ? 2u : 4u) << 29);
+}
+// Byte offset of 16-byte chunk `chunk` of row `row` in such a tile.
+template <int BOX_BYTES>
+__device__ __forceinline__ uint32_t cached_swz(uint32_t row, uint32_t chunk) {
+  if constexpr (BOX_BYTES == 128) return row * 128u + ((chunk ^ (row & 7u)) << 4);
+  else return row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4);
+}
+
+__device__ __forceinline__ int lds_s8(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared.s8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Bits [from, to) of a word.
+__device__ __forceinline__ uint32_t bit_run(int from, int to) {
+  from = max(from, 0);
+  to = min(to, 32);
+  return from < to ? (0xffffffffu >> (32 - to)) & (0xffffffffu << from) : 0u;
+}
+
+#define SPLASH_KBAR(field, idx) \
+  (bars_u32 + static_cast<uint32_t>(offsetof(CachedBarriers, field)) + 8u * static_cast<uint32_t>(idx))
+#define SPLASH_KWORD(field) (bars_u32 + static_cast<uint32_t>(offsetof(CachedBarriers, field)))
+
+template <int D, bool BF16, bool QUANT, int KG>
+__global__ void __launch_bounds__(kCachedThreads, 1)
+cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+              const __grid_constant__ CUtensorMap tm_v, const CachedArgs a) {
+  using L = CachedLayout<D, BF16, QUANT, KG>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t q_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t ring_u32 = q_u32 + L::kQBytes;
+  const uint32_t stage_u32 = ring_u32 + L::kSlots * L::kSlotBytes;
+  const uint32_t ml_u32 = stage_u32 + L::kStageBytes;
+  const uint32_t bars_u32 = ml_u32 + L::kMlBytes;
+  const uint32_t aux_u32 = bars_u32 + L::kBarBytes;
+  const uint32_t scale_u32 = aux_u32 + L::kAuxBytes;
+  const uint32_t qscale_u32 = scale_u32 + L::kScaleBytes;
+  const uint32_t parents_u32 = qscale_u32 + L::kQScaleBytes;
+  const uint32_t above_u32 = parents_u32 + kCachedMaxTree * 4;  // [128 rows][8 words]: 0, four words of bits, 0
+
+  const int warp = uniform_warp_index();
+  const int lane = threadIdx.x & 31;
+  const WaitCtx ctx{SPLASH_KWORD(abort_flag)};
+
+  // ---- set-up: barriers, tensor memory, this CTA's share of the line ------------------------------------------------
+  if (warp == 8) {
+    constexpr uint32_t kNumBarriers = offsetof(CachedBarriers, tmem_base) / 8;
+    for (uint32_t i = lane; i < kNumBarriers; i += 32) {
+      const uint32_t off = 8u * i;
+      uint32_t count = 1;
+      if (off >= offsetof(CachedBarriers, p_ready) && off < offsetof(CachedBarriers, q_full)) count = 128;
+      if (off == offsetof(CachedBarriers, q_full)) count = QUANT ? 32 : 1;
+      if (off == offsetof(CachedBarriers, o_free) || off == offsetof(CachedBarriers, sync)) count = 256;
+      mbar_init(bars_u32 + off, count);
+    }
+    if (lane == 0) {
+      sts32(SPLASH_KWORD(abort_flag), 0);
+      sts32(SPLASH_KWORD(dead), a.status[0] != 0);
+      prefetch_tensormap(&tm_k);
+      prefetch_tensormap(&tm_v);
+      if (!QUANT) prefetch_tensormap(&tm_q);
+    }
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  } else if (warp == 9) {
+    tmem_alloc(SPLASH_KWORD(tmem_base), 512);
+    tmem_relinquish();
+  } else if (warp == 0) {
+    const int entries = a.batch * a.row_tiles;
+    int total = 0;
+    for (int e0 = 0; e0 < entries; e0 += 32) {
+      const int mine = e0 + lane < entries ? cached_geom(a, e0 + lane).tiles * a.kv_heads : 0;
+      if (blockIdx.x == 0) {
+        int before = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+          const int x = __shfl_up_sync(0xffffffffu, before, d);
+          if (lane >= d) before += x;
+        }
+        if (e0 + lane < entries) a.starts[e0 + lane] = total + before - mine;
+      }
+      total += __reduce_add_sync(0xffffffffu, mine);
+    }
+    if (blockIdx.x == 0 && lane == 0) a.starts[entries] = total;
+    const int ctas = min(static_cast<int>(gridDim.x), total);  // a tile at least to each that takes part
+    const int c = blockIdx.x;
+    const int begin = c < ctas ? cached_share(c, total, ctas) : 0, end = c < ctas ? cached_share(c + 1, total, ctas) : 0;
+    if (begin < end) {
+      int passed = 0;
+      for (int e0 = 0; e0 < entries; e0 += 32) {
+        const int mine = e0 + lane < entries ? cached_geom(a, e0 + lane).tiles * a.kv_heads : 0;
+        const int sum = __reduce_add_sync(0xffffffffu, mine);
+        if (begin < passed + sum) {
+          int upto = mine;
+#pragma unroll
+          for (int d = 1; d < 32; d *= 2) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += x;
+          }
+          const int from = passed + upto - mine;
+          if (begin >= from && begin < from + mine) {
+            const int tiles = mine / a.kv_heads;
+            sts32(SPLASH_KWORD(first_entry), e0 + lane);
+            sts32(SPLASH_KWORD(first_head), (begin - from) / tiles);
+            sts32(SPLASH_KWORD(first_tile), (begin - from) % tiles);
+          }
+          break;
+        }
+        passed += sum;
+      }
+    }
+    if (lane == 0) sts32(SPLASH_KWORD(num_tiles), end - begin);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = lds32(SPLASH_KWORD(tmem_base));
+  if (lds32(SPLASH_KWORD(dead))) {
+    if (warp == 9) {
+      __syncwarp();
+      tmem_dealloc(tmem, 512);
+    }
+    return;
+  }
+  CachedCursor cur;
+  cur.start(a, lds32(SPLASH_KWORD(first_entry)), lds32(SPLASH_KWORD(first_head)), lds32(SPLASH_KWORD(first_tile)),
+            lds32(SPLASH_KWORD(num_tiles)));
+
+  if (warp >= 8) {
+    setmaxnreg_dec<L::kLoadRegs>();
+    if (warp == 8) {
+      // ------------------------------------------ loads --------------------------------------------------------------
+      // Order of the tiles in the ring, for T tiles of a segment: K0 K1 V0 K2 V1 ... K(T-1) V(T-2) V(T-1), which is the
+      // order in which the MMA warp uses them.  A lane has one page of a tile.
+      const int piece = min(a.page_size, kCachedTile);  // keys per TMA box
+      const int pieces = kCachedTile / piece;
+      int slot = 0;
+      uint32_t phase = 0;
+      int seq = 0, aux = 0;
+      bool ok = true;
+      for (int seg = 0; ok && cur.next(a); ++seg) {
+        const CachedGeom& g = cur.g;
+        const int b = cur.seg_entry / a.row_tiles, rt = cur.seg_entry - b * a.row_tiles;
+        if constexpr (!QUANT) {
+          if (seg > 0 && !warp_wait(SPLASH_KBAR(q_free, 0), (seg - 1) & 1, ctx, kCSiteLoadQ, seg)) break;
+          if (elect_one()) {
+            const int row = (b * a.kv_heads + cur.seg_head) * a.rows + rt * L::kRows;
+            mbar_arrive_expect_tx(SPLASH_KBAR(q_full, 0), L::kQBytes);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+              for (int copy = 0; copy < L::kCopies; ++copy)
+                tma_load_2d(q_u32 + c * (128 * 128) + copy * (L::kRows * 128), &tm_q, c * 64, row, SPLASH_KBAR(q_full, 0));
+          }
+        }
+        const int32_t* table = a.page_table + b * a.table_stride;
+        // Row of the cache where this lane's piece of tile i begins, -1: nobody sees it, or no page.
+        auto piece_row = [&](int i) -> int {
+          if (i >= cur.seg_n || lane >= pieces) return -1;
+          const int key = cur.key0(i) + lane * piece;
+          if (key >= g.hi || (key + piece <= g.lo && key >= g.sink_hi)) return -1;
+          const int entry = key / a.page_size;
+          const int page = table[entry];
+          if (page < 0 || page >= a.num_pages) return -1;
+          return (page * a.kv_heads + cur.seg_head) * a.page_size + (key - entry * a.page_size);
+        };
+        int row = piece_row(0), row_before = -1;
+        for (int i = 0; i <= cur.seg_n; ++i) {
+          const int row_next = piece_row(i + 1);  // its page id is on the way while this tile is loaded
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            if (kv == 0 ? i == cur.seg_n : i == 0) continue;
+            const int at = kv == 0 ? row : row_before;
+            if (seq >= L::kSlots && !warp_wait(SPLASH_KBAR(empty, slot), phase ^ 1, ctx, kCSiteLoadEmpty, seq)) { ok = false; break; }
+            const uint32_t some = __ballot_sync(0xffffffffu, at >= 0);
+            uint32_t bytes = __popc(some) * piece * L::kRowBytes;
+            if (QUANT && kv == 0) bytes += __popc(some) * piece * 2;
+            if (lane == 0) mbar_arrive_expect_tx(SPLASH_KBAR(full, slot), bytes);
+            __syncwarp();
+            if (at >= 0) {
+              const uint32_t dst = ring_u32 + slot * L::kSlotBytes + lane * piece * L::kBoxBytes;
+#pragma unroll
+              for (int c = 0; c < L::kBoxes; ++c)
+                tma_load_2d(dst + c * (kCachedTile * L::kBoxBytes), kv == 0 ? &tm_k : &tm_v, c * L::kBoxElems, at, SPLASH_KBAR(full, slot));
+              if (QUANT && kv == 0) {
+                // Exponents of the tile's keys and values.  Their slot is used again 16 tiles on; this warp is ahead of
+                // the MMA warp by the ring (at most 6 tiles), and that one of the softmax by two tiles.
+                const uint32_t x = aux_u32 + aux * (2 * kCachedTile) + lane * piece;
+                bulk_load_1d(x, a.k_exponent + at, piece, SPLASH_KBAR(full, slot));
+                bulk_load_1d(x + kCachedTile, a.v_exponent + at, piece, SPLASH_KBAR(full, slot));
+              }
+            }
+            if (kv == 0 && ++aux == kCachedAuxSlots) aux = 0;
+            ++seq;
+            if (++slot == L::kSlots) { slot = 0; phase ^= 1; }
+          }
+          if (!ok) break;
+          row_before = row;
+          row = row_next;
+        }
+      }
+    } else if (warp == 9) {
+      // ------------------------------------------ products -----------------------------------------------------------
+      constexpr uint32_t kHi = cached_desc_hi<L::kBoxBytes>();
+      constexpr uint32_t kQHi = kHi;
+      constexpr uint32_t kIdescQK = make_idesc(BF16 && !QUANT, 128, kCachedTile, false, false);
+      constexpr uint32_t kIdescPV = make_idesc(BF16 && !QUANT, 128, D, false, true);
+      constexpr int kStepsPerBox = L::kBoxBytes / 32;  // an MMA takes 32 bytes of K per row
+      int slot = 0;
+      uint32_t phase = 0;
+      uint32_t p_par[2] = {0, 0};
+      int step = 0;
+      auto advance = [&]() { if (++slot == L::kSlots) { slot = 0; phase ^= 1; } };
+      auto issue_qk = [&](int grp) -> bool {
+        if (!warp_wait(SPLASH_KBAR(full, slot), phase, ctx, kCSiteMmaFull, step)) return false;
+        tc_fence_after();
+        const uint32_t b_lo = desc_lo(ring_u32 + slot * L::kSlotBytes, 16);
+#pragma unroll
+        for (int t = 0; t < L::kTerms; ++t) {
+          const uint32_t a_lo = desc_lo(q_u32 + t * L::kQTerm, 16);
+#pragma unroll
+          for (int kk = 0; kk < L::kRowBytes / 32; ++kk) {
+            const uint32_t off = ((kk / kStepsPerBox) * (128 * L::kBoxBytes) + (kk % kStepsPerBox) * 32) >> 4;
+            if constexpr (QUANT) umma8_ss2_w(tmem + grp * 128, a_lo + off, kQHi, b_lo + off, kHi, kIdescQK, t > 0 || kk > 0);
+            else umma_ss2_w(tmem + grp * 128, a_lo + off, kQHi, b_lo + off, kHi, kIdescQK, kk > 0);
+          }
+        }
+        umma_commit_w(SPLASH_KBAR(s_ready, grp));
+        umma_commit_w(SPLASH_KBAR(empty, slot));
+        advance();
+        return true;
+      };
+      bool ok = true;
+      for (int seg = 0; ok && cur.next(a); ++seg) {
+        const int n = cur.seg_n;
+        if (!warp_wait(SPLASH_KBAR(q_full, 0), seg & 1, ctx, kCSiteMmaQ, seg)) break;
+        tc_fence_after();
+        if (!issue_qk(0)) break;
+        if (n > 1 && !issue_qk(1)) break;
+        if (n <= 2) umma_commit_w(SPLASH_KBAR(q_free, 0));
+        for (int i = 0; i < n; ++i, ++step) {
+          const int grp = i & 1;
+          if (!warp_wait(SPLASH_KBAR(full, slot), phase, ctx, kCSiteMmaFull, step) ||
+              !warp_wait(SPLASH_KBAR(p_ready, grp), p_par[grp], ctx, kCSiteMmaP, step) ||
+              // O may be written again once the previous segment's has been read.
+              (i == 0 && seg > 0 && !warp_wait(SPLASH_KBAR(o_free, 0), (seg - 1) & 1, ctx, kCSiteMmaO, seg))) { ok = false; break; }
+          p_par[grp] ^= 1;
+          tc_fence_after();
+          const uint32_t b_lo = desc_lo(ring_u32 + slot * L::kSlotBytes, kCachedTile * L::kBoxBytes);
+          constexpr int kKeysPerMma = QUANT ? 32 : 16;
+#pragma unroll
+          for (int kk = 0; kk < kCachedTile / kKeysPerMma; ++kk) {
+            const uint32_t off = (kk * kKeysPerMma * L::kBoxBytes) >> 4;
+            if constexpr (QUANT) umma8_ts2_w(tmem + L::kOCol + grp * D, tmem + grp * 128 + kk * 8, b_lo + off, kHi, kIdescPV, i > 1 || kk > 0);
+            else umma_ts2_w(tmem + L::kOCol + grp * D, tmem + grp * 128 + kk * 8, b_lo + off, kHi, kIdescPV, i > 1 || kk > 0);
+          }
+          umma_commit_w(SPLASH_KBAR(empty, slot));
+          advance();
+          if (i + 2 < n) {
+            if (!issue_qk(grp)) { ok = false; break; }
+            if (i + 3 == n) umma_commit_w(SPLASH_KBAR(q_free, 0));
+          }
+        }
+        if (ok) umma_commit_w(SPLASH_KBAR(o_done, 0));
+      }
+    } else if (QUANT && warp == 11) {
+      // ------------------------------ Q as e4m3 terms, a row of 2 * D bytes at a time -----------------------------------
+      constexpr int kPer = D / 32;  // neighbouring numbers per lane
+      for (int seg = 0; cur.next(a); ++seg) {
+        const int b = cur.seg_entry / a.row_tiles, rt = cur.seg_entry - b * a.row_tiles;
+        if (seg > 0 && !warp_wait(SPLASH_KBAR(q_free, 0), (seg - 1) & 1, ctx, kCSiteConvQ, seg)) break;
+        const long long row0 = static_cast<long long>(b * a.kv_heads + cur.seg_head) * a.rows + rt * L::kRows;
+        const int rows = min(L::kRows, a.rows - rt * L::kRows);
+        constexpr int kBatch = 8;  // rows whose loads are in flight together
+        for (int r0 = 0; r0 < L::kRows; r0 += kBatch) {
+          uint32_t w[kBatch][kPer / 2];
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) {
+            const int r = r0 + j;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) + (row0 + r) * D) + lane * (kPer / 2);
+#pragma unroll
+            for (int i = 0; i < kPer / 2; ++i) w[j][i] = r < rows ? __ldg(src + i) : 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) {
+            const int r = r0 + j;
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < kPer / 2; ++i) top = max(top, max(w[j][i] & 0x7fffu, (w[j][i] >> 16) & 0x7fffu));
+            top = __reduce_max_sync(0xffffffffu, top);
+            const bool bad = top >= (BF16 ? 0x7f80u : 0x7c00u);
+            float amax;
+            if constexpr (BF16) amax = __uint_as_float(top << 16);
+            else amax = __half2float(__ushort_as_half(static_cast<unsigned short>(top)));
+            // 2^-eq takes the largest number of the row into [128, 256).
+            const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 7, -100), 120);
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            float x[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer / 2; ++i) {
+              float2 f;
+              if constexpr (BF16) f = make_float2(__uint_as_float(w[j][i] << 16), __uint_as_float(w[j][i] & 0xffff0000u));
+              else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j][i]));
+              x[2 * i] = f.x * down;
+              x[2 * i + 1] = f.y * down;
+            }
+            if (lane == 0)
+              sts32(qscale_u32 + ((seg & 1) * 128 + r) * 4, bad ? 0x7fc00000u : static_cast<uint32_t>(e + 127) << 23);
+#pragma unroll
+            for (int t = 0; t < L::kTerms; ++t) {
+              uint32_t code[kPer / 2];
+#pragma unroll
+              for (int i = 0; i < kPer / 2; ++i) {
+                code[i] = e4m3x2(x[2 * i], x[2 * i + 1]);
+                const float2 f = e4m3x2_to_f32(code[i]);
+                x[2 * i] -= f.x;
+                x[2 * i + 1] -= f.y;
+              }
+              const uint32_t byte = lane * kPer;
+#pragma unroll
+              for (int copy = 0; copy < L::kCopies; ++copy) {
+                const uint32_t dst = q_u32 + t * L::kQTerm + cached_swz<L::kBoxBytes>(copy * L::kRows + r, byte >> 4) + (byte & 15u);
+                if constexpr (kPer == 4) sts32(dst, code[0] | (code[1] << 16));
+                else asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst), "h"(static_cast<uint16_t>(code[0])) : "memory");
+              }
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(SPLASH_KBAR(q_full, 0));
+      }
+    }
+  } else {
+    // ============================================ softmax ==============================================================
+    setmaxnreg_inc<L::kSoftmaxRegs>();
+    const int grp = warp >> 2;
+    const int row_lane = (warp & 3) * 32 + lane;
+    const int copy = row_lane / L::kRows;                   // (the same for a warp: copies are 32 rows or more)
+    const int r = row_lane % L::kRows;
+    const int part = QUANT ? copy >> 1 : copy;              // which part of a tile's keys
+    const bool low_term = QUANT && (copy & 1);
+    const int col0 = part * L::kKeys;
+    const uint32_t tmem_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t s_tmem = tmem_lane + grp * 128, o_tmem = tmem_lane + L::kOCol + grp * D;
+    const uint32_t my_scales = scale_u32 + warp * (L::kKeys * 12);
+    const int piece = min(a.page_size, kCachedTile);
+    const bool tree = a.parents != nullptr;
+    const float unit = a.soft_cap > 0.f ? a.soft_cap : 1.f;
+    const float unit2 = unit * kCachedLog2e;
+    const float inv_cap = a.soft_cap > 0.f ? 1.f / a.soft_cap : 1.f;
+    constexpr float kThreshold = QUANT ? 3.f : 8.f;          // powers of 2 by which the maximum may lag behind
+    constexpr float kPScale = QUANT ? 32.f : 1.f;            // 8 bit: P up to 2^3 * 32 = 256
+    uint32_t s_par = 0, sync_par = 0;
+    int seq = 0;     // ring position of the segment's first tile
+    int aux0 = 0;    // exponent slot of the segment's first tile
+    bool ok = true;
+    uint32_t zero16[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) zero16[j] = 0;
+    auto group_sync = [&]() -> bool {
+      mbar_arrive(SPLASH_KBAR(sync, 0));
+      const bool fine = warp_wait(SPLASH_KBAR(sync, 0), sync_par, ctx, kCSiteSmxSync, 0);
+      sync_par ^= 1;
+      return fine;
+    };
+
+    for (int seg = 0; ok && cur.next(a); ++seg) {
+      const CachedGeom& g = cur.g;
+      const int n = cur.seg_n;
+      const int b = cur.seg_entry / a.row_tiles, rt = cur.seg_entry - b * a.row_tiles;
+      const int row_all = rt * L::kRows + r;       // among the rows of this (sequence, kv head)
+      const int node = row_all % a.n;
+      const bool live = row_all < a.rows && node < g.count;
+      int depth = node;
+      if (tree) {
+        // Bits of the nodes that a row sees among the drafted ones: itself and its ancestors, as far as the window goes.
+        const int t = threadIdx.x;
+        if (t < a.n) sts32(parents_u32 + t * 4, static_cast<uint32_t>(a.parents[b * a.parents_stride + t]));
+        if (!group_sync()) { ok = false; break; }
+        depth = 0;
+        if (live) {
+          for (int x = node, up; ; x = up, ++depth) {
+            up = static_cast<int>(lds32(parents_u32 + x * 4));
+            if (up < 0 || up >= x) break;  // a parent stands before its child; anything else is the context
+          }
+        }
+        if (grp == 0) {
+#pragma unroll
+          for (int w = 0; w < 8; ++w) sts32(above_u32 + (row_lane * 8 + w) * 4, 0);
+          if (live) {
+            int d = depth;
+            for (int x = node;; --d) {
+              if (a.window < 0 || d >= depth - a.window || g.before + d < a.sinks) {
+                const uint32_t at = above_u32 + (row_lane * 8 + 1 + (x >> 5)) * 4;
+                sts32(at, lds32(at) | (1u << (x & 31)));
+              }
+              const int up = static_cast<int>(lds32(parents_u32 + x * 4));
+              if (up < 0 || up >= x) break;
+              x = up;
+            }
+          }
+        }
+        if (!group_sync()) { ok = false; break; }
+      }
+      // Keys of the context (tree) or of context and run that this row sees: [v_lo, v_hi) and [0, v_sink).
+      const int position = g.before + depth;
+      const int v_hi = !live ? 0 : (tree ? g.before : position + 1);
+      const int v_lo = a.window < 0 ? 0 : max(0, position - a.window);
+      const int v_sink = a.window < 0 ? 0 : min(a.sinks, v_hi);
+      const int seen_by_all = g.before + (tree ? 0 : g.i0 + 1);  // keys in front of this are behind no row
+      const int all_from = a.window < 0 ? 0 : g.before + g.i1 - 1 - a.window;
+      const int32_t* table = a.page_table + b * a.table_stride;
+      float q_mul = inv_cap;  // what takes a score to the argument of the soft-cap
+      float mul = unit2;      // ... and what it holds then to powers of 2
+      float m_run = -INFINITY, l_run = 0.f;  // powers of 2; 8 bit: the maximum of s + ev
+      const int pages = kCachedTile / piece;
+      auto page_of = [&](int i) -> int {  // lane p: page id of piece p of tile i (anything for pieces nobody sees)
+        if (i >= n || lane >= pages) return 0;
+        const int key = cur.key0(i) + lane * piece;
+        return key < g.hi ? table[key / a.page_size] : 0;
+      };
+      int page = page_of(grp);
+
+      for (int i = grp; i < n; i += 2) {
+        const int key0 = cur.key0(i);
+        const uint32_t good = __ballot_sync(0xffffffffu, page >= 0 && page < a.num_pages);  // pieces that have a page
+        page = page_of(i + 2);
+        const bool plain = key0 + kCachedTile <= seen_by_all && (key0 >= all_from || key0 + kCachedTile <= g.sink_hi) &&
+                           good == 0xffffffffu;
+        // Whether key `at` of the tile is there for some row; the others may hold anything, and nothing was loaded for some.
+        auto there = [&](int at) {
+          const int key = key0 + at;
+          return key < g.hi && (key >= g.lo || key < g.sink_hi) && ((good >> (at / piece)) & 1u);
+        };
+        if (!warp_wait(SPLASH_KBAR(s_ready, grp), s_par, ctx, kCSiteSmxS, i)) { ok = false; break; }
+        s_par ^= 1;
+        tc_fence_after();
+        float sv[L::kKeys];
+        {
+          uint32_t* raw = reinterpret_cast<uint32_t*>(sv);
+#pragma unroll
+          for (int c = 0; c < L::kKeys / 32; ++c) tmem_ld32(s_tmem + col0 + c * 32, raw + c * 32);
+        }
+        if constexpr (QUANT) {
+          // Scales of this warp's keys in shared memory of its own: 2^ek | ev | 2^ev * 32, while the scores arrive.
+          // (The exponents came with the keys, for which the scores waited.)
+          if (i == grp) {
+            const float q_scale = __uint_as_float(lds32(qscale_u32 + ((seg & 1) * 128 + r) * 4));
+            q_mul = q_scale * inv_cap;
+            mul = a.soft_cap > 0.f ? unit2 : unit2 * q_scale;
+          }
+          const uint32_t x = aux_u32 + ((aux0 + i) % kCachedAuxSlots) * (2 * kCachedTile) + col0;
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < L::kKeys / 32; ++c) {
+            const int at = c * 32 + lane;
+            int ek = 0, ev = 0;
+            if (plain || there(col0 + at)) {
+              ek = lds_s8(x + at);
+              ev = lds_s8(x + kCachedTile + at);
+            }
+            sts32(my_scales + at * 4, __float_as_uint(exponent_scale(ek)));
+            sts32(my_scales + (L::kKeys + at) * 4, __float_as_uint(static_cast<float>(ev)));
+            sts32(my_scales + (2 * L::kKeys + at) * 4, __float_as_uint(exponent_scale(ev) * kPScale));
+          }
+          __syncwarp();
+        }
+        tmem_wait_ld();
+        if constexpr (QUANT) {
+#pragma unroll
+          for (int j = 0; j < L::kKeys; j += 4) {
+            const uint4 k4 = lds128(my_scales + j * 4);
+            sv[j] *= __uint_as_float(k4.x);
+            sv[j + 1] *= __uint_as_float(k4.y);
+            sv[j + 2] *= __uint_as_float(k4.z);
+            sv[j + 3] *= __uint_as_float(k4.w);
+          }
+        }
+        if (a.soft_cap > 0.f) {
+#pragma unroll
+          for (int j = 0; j < L::kKeys; ++j) sv[j] = tanh_approx(sv[j] * q_mul);
+        }
+        if (!plain) {
+#pragma unroll
+          for (int c = 0; c < L::kKeys / 32; ++c) {
+            const int at = col0 + c * 32, kb = key0 + at;
+            uint32_t vis = bit_run(v_lo - kb, v_hi - kb) | bit_run(-kb, v_sink - kb);
+            const int d0 = kb - g.before;
+            if (tree && d0 > -32 && d0 < kCachedMaxTree) {
+              const uint32_t w = above_u32 + (row_lane * 8 + 1 + (d0 >> 5)) * 4;
+              vis |= __funnelshift_r(lds32(w), lds32(w + 4), d0 & 31);
+            }
+            if (piece >= 32) {
+              if (!((good >> (at / piece)) & 1u)) vis = 0;
+            } else {
+              if (!((good >> (at / 16)) & 1u)) vis &= 0xffff0000u;
+              if (!((good >> (at / 16 + 1)) & 1u)) vis &= 0x0000ffffu;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (!((vis >> j) & 1u)) sv[c * 32 + j] = -INFINITY;
+          }
+          // Values that no row sees are cleared: their probability is 0, and 0 times what lies there may be NaN.
+          const bool clear = !there(row_lane);
+          if (__any_sync(0xffffffffu, clear)) {
+            const int at = seq + (i + 1 < n ? 2 * i + 2 : 2 * n - 1);  // place of V(i) among the loads
+            const int slot = at % L::kSlots;
+            if (!warp_wait(SPLASH_KBAR(full, slot), (at / L::kSlots) & 1, ctx, kCSiteSmxV, i)) { ok = false; break; }
+            if (clear) {
+              const uint32_t dst = ring_u32 + slot * L::kSlotBytes + row_lane * L::kBoxBytes;
+#pragma unroll
+              for (int c = 0; c < L::kBoxes; ++c)
+#pragma unroll
+                for (int k = 0; k < L::kBoxBytes / 16; ++k)
+                  sts128(dst + c * (kCachedTile * L::kBoxBytes) + k * 16, make_uint4(0, 0, 0, 0));
+            }
+            fence_proxy_async_smem();
+          }
+        }
+
+        // ---- online softmax with a maximum that may lag behind ----
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < L::kKeys; j += 4) {
+          if constexpr (QUANT) {
+            const uint4 e4 = lds128(my_scales + (L::kKeys + j) * 4);
+            mx[0] = fmaxf(mx[0], fmaf(sv[j], mul, __uint_as_float(e4.x)));
+            mx[1] = fmaxf(mx[1], fmaf(sv[j + 1], mul, __uint_as_float(e4.y)));
+            mx[2] = fmaxf(mx[2], fmaf(sv[j + 2], mul, __uint_as_float(e4.z)));
+            mx[3] = fmaxf(mx[3], fmaf(sv[j + 3], mul, __uint_as_float(e4.w)));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], sv[j + k]);
+          }
+        }
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if constexpr (!QUANT) top *= mul;
+        const float m_new = fmaxf(m_run, top);
+        const bool moved = m_new - m_run > kThreshold;  // false for NaN (-inf - -inf)
+        float alpha = 1.f;
+        if (moved) {
+          alpha = ex2_approx(m_run - m_new);  // 0 when m_run was -inf
+          m_run = m_new;
+          l_run *= alpha;
+        }
+        const float shift = m_run == -INFINITY ? 0.f : -m_run;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (QUANT) {
+          // 128 codes are 32 columns.
+          uint32_t pk[L::kKeys / 4];
+#pragma unroll
+          for (int j = 0; j < L::kKeys; j += 4) {
+            const uint4 v4 = lds128(my_scales + (2 * L::kKeys + j) * 4);
+            const float vs[4] = {__uint_as_float(v4.x), __uint_as_float(v4.y), __uint_as_float(v4.z), __uint_as_float(v4.w)};
+            float p[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float e = ex2_approx(fmaf(sv[j + k], mul, shift));
+              sum[k] += e;
+              p[k] = e * vs[k];
+            }
+            uint32_t c0 = e4m3x2(p[0], p[1]), c1 = e4m3x2(p[2], p[3]);
+            if (low_term) {
+              const float2 f0 = e4m3x2_to_f32(c0), f1 = e4m3x2_to_f32(c1);
+              c0 = e4m3x2((p[0] - f0.x) * 16.f, (p[1] - f0.y) * 16.f);
+              c1 = e4m3x2((p[2] - f1.x) * 16.f, (p[3] - f1.y) * 16.f);
+            }
+            pk[j / 4] = c0 | (c1 << 16);
+          }
+#pragma unroll
+          for (int c = 0; c < 32 / 16; ++c) {
+            if (c * 16 >= col0 / 4 && c * 16 < (col0 + L::kKeys) / 4) {
+              if constexpr (L::kKeys == 128) tmem_st16(s_tmem + c * 16, pk + c * 16);
+              else tmem_st16(s_tmem + c * 16, pk);
+            } else {
+              tmem_st16(s_tmem + c * 16, zero16);
+            }
+          }
+        } else {
+          // 128 probabilities of 16 bits are 64 columns; those of the other copies' keys are zero here.
+#pragma unroll
+          for (int c = 0; c < L::kKeys / 32; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float e0 = ex2_approx(fmaf(sv[c * 32 + 2 * j], mul, shift));
+              const float e1 = ex2_approx(fmaf(sv[c * 32 + 2 * j + 1], mul, shift));
+              sum[j & 3] += e0 + e1;
+              pk[j] = pack2<BF16>(e0, e1);
+            }
+            tmem_st16(s_tmem + col0 / 2 + c * 16, pk);
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c * 16 < col0 / 2 || c * 16 >= (col0 + L::kKeys) / 2) tmem_st16(s_tmem + c * 16, zero16);
+        }
+        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // The scores of this tile came after P.V of the warpgroup's previous one: O stands still.
+        if (i >= 2 && __any_sync(0xffffffffu, moved)) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_tmem + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st32(o_tmem + c * 32, o);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(SPLASH_KBAR(p_ready, grp));
+      }
+      if (!ok) break;
+
+      // ---- the parts of a row, added up: two warpgroups, and the copies of the rows ----
+      sts32(ml_u32 + threadIdx.x * 8, __float_as_uint(m_run));
+      sts32(ml_u32 + threadIdx.x * 8 + 4, __float_as_uint(l_run));
+      if (!warp_wait(SPLASH_KBAR(o_done, 0), seg & 1, ctx, kCSiteSmxDone, seg)) { ok = false; break; }
+      tc_fence_after();
+      if (!group_sync()) { ok = false; break; }
+      float m_tot = -INFINITY, l_tot = 0.f;
+#pragma unroll
+      for (int src = 0; src < 2 * KG; ++src) {
+        const uint32_t at = ml_u32 + ((src / KG) * 128 + (src % KG) * (QUANT ? 2 : 1) * L::kRows + r) * 8;
+        m_tot = fmaxf(m_tot, __uint_as_float(lds32(at)));
+      }
+#pragma unroll
+      for (int src = 0; src < 2 * KG; ++src) {
+        const uint32_t at = ml_u32 + ((src / KG) * 128 + (src % KG) * (QUANT ? 2 : 1) * L::kRows + r) * 8;
+        const float m = __uint_as_float(lds32(at)), l = __uint_as_float(lds32(at + 4));
+        if (l != 0.f) l_tot += m == -INFINITY ? l : l * ex2_approx(m - m_tot);
+      }
+      const bool whole = cur.whole;
+      float w = m_run == -INFINITY ? 0.f : ex2_approx(m_run - m_tot);
+      w *= (low_term ? 1.f / 16 : 1.f) / kPScale;
+      if (l_run != l_run) w = l_run;  // NaN: no maximum may have been met
+      if (whole) w *= l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
+      const long long out_row0 = static_cast<long long>(b * a.kv_heads + cur.seg_head) * a.rows + rt * L::kRows;
+      const long long part0 = static_cast<long long>(2 * blockIdx.x + (seg > 0)) * L::kRows;
+      if (grp == 0 && copy == 0) {
+        if (!whole) a.part_ml[part0 + r] = make_float2(m_tot, l_tot);
+        else if (a.lse_out && row_all < a.rows)
+          a.lse_out[out_row0 + r] = live && l_tot != 0.f ? (m_tot + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
+      }
+      constexpr int kPerRow = 256 / L::kRows;   // threads that add up one row of a chunk of 32 columns
+      constexpr int kQuads = 8 / kPerRow;       // groups of four columns each of them has
+      const int sum_row = threadIdx.x / kPerRow, sum_sub = threadIdx.x % kPerRow;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (grp < n) {
+          tmem_ld32(o_tmem + c * 32, o);
+          tmem_wait_ld();
+        }
+        if (c == D / 32 - 1) {
+          tc_fence_before();
+          mbar_arrive(SPLASH_KBAR(o_free, 0));
+        }
+        const uint32_t dst = stage_u32 + threadIdx.x * (L::kStageStride * 4);
+        const bool any = grp < n && live;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (any) {
+            x.x = __float_as_uint(__uint_as_float(o[k * 4]) * w);
+            x.y = __float_as_uint(__uint_as_float(o[k * 4 + 1]) * w);
+            x.z = __float_as_uint(__uint_as_float(o[k * 4 + 2]) * w);
+            x.w = __float_as_uint(__uint_as_float(o[k * 4 + 3]) * w);
+          }
+          sts128(dst + k * 16, x);
+        }
+        if (!group_sync()) { ok = false; break; }
+#pragma unroll
+        for (int k = 0; k < kQuads; ++k) {
+          const int col = (sum_sub * kQuads + k) * 4;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int src = 0; src < 2 * L::kCopies; ++src) {
+            const int from = (src / L::kCopies) * 128 + (src % L::kCopies) * L::kRows + sum_row;
+            const uint4 x = lds128(stage_u32 + (from * L::kStageStride + col) * 4);
+            acc.x += __uint_as_float(x.x);
+            acc.y += __uint_as_float(x.y);
+            acc.z += __uint_as_float(x.z);
+            acc.w += __uint_as_float(x.w);
+          }
+          if (!whole) {
+            *reinterpret_cast<float4*>(a.part_o + (part0 + sum_row) * D + c * 32 + col) = acc;
+          } else if (rt * L::kRows + sum_row < a.rows) {
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (out_row0 + sum_row) * D + c * 32 + col) =
+                make_uint2(pack2<BF16>(acc.x, acc.y), pack2<BF16>(acc.z, acc.w));
+          }
+        }
+        if (!group_sync()) { ok = false; break; }
+      }
+      seq += 2 * n;
+      aux0 += n;
+    }
+  }
+
+  // ---- teardown: every thread of every role ends up here ----
+  tc_fence_before();
+  __syncthreads();
+  if (const uint32_t gave_up = lds32(SPLASH_KWORD(abort_flag))) {
+    if (threadIdx.x == 0) report_abort(a.status, gave_up);
+    // Copies still in flight land before the shared memory goes to another CTA.
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000) {}
+  }
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+#undef SPLASH_KBAR
+#undef SPLASH_KWORD
+
+}  // namespace splash

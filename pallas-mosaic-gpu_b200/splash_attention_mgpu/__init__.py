@@ -3,6 +3,7 @@
 Same import surface as the reference package (`splash_attention_mgpu/__init__.py:4-21`).
 """
 
+from .cached_attention import CachedAttentionKernel, make_splash_cached
 from .config import DEFAULT_MASK_VALUE, BlockSizes, SegmentIds
 from .kv_cache import KVCache, make_kv_cache
 from .mask_info import GpuMaskInfo, process_mask
@@ -25,8 +26,8 @@ from .splash_attention_mask import (
 )
 
 __all__ = [
-    "BlockSizes", "CausalMask", "ChunkedCausalMask", "DEFAULT_MASK_VALUE",
+    "BlockSizes", "CachedAttentionKernel", "CausalMask", "ChunkedCausalMask", "DEFAULT_MASK_VALUE",
     "FullMask", "GpuMaskInfo", "KVCache", "LocalMask", "Mask", "MultiHeadMask",
     "NumpyMask", "RotaryEmbedding", "SegmentIds", "SplashAttentionKernel", "attention_reference",
-    "check_device_status", "make_kv_cache", "make_rotary", "make_splash_mha", "make_splash_mqa", "process_mask",
+    "check_device_status", "make_kv_cache", "make_rotary", "make_splash_cached", "make_splash_mha", "make_splash_mqa", "process_mask",
 ]

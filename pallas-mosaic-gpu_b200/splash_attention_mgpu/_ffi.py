@@ -48,6 +48,8 @@ EXPORTED_SYMBOLS = (
     "splash_rotary",
     "splash_cache_write",
     "splash_cache_read",
+    "splash_cached_fwd",
+    "splash_cached_workspace_bytes",
 )
 
 
@@ -101,6 +103,21 @@ class SplashCacheParams(Structure):
       ("batch", c_int32), ("kv_heads", c_int32), ("len", c_int32), ("head_dim", c_int32),
       ("num_pages", c_int32), ("page_size", c_int32), ("table_width", c_int32),
       ("dtype", c_int32), ("quantized", c_int32),
+  ]
+
+
+class SplashCachedParams(Structure):
+  """Mirror of `struct SplashCachedParams`."""
+
+  _fields_ = [
+      ("q", c_void_p), ("k_cache", c_void_p), ("v_cache", c_void_p), ("k_exponent", c_void_p), ("v_exponent", c_void_p),
+      ("page_table", c_void_p), ("lengths", c_void_p), ("counts", c_void_p), ("parents", c_void_p),
+      ("out", c_void_p), ("lse_out", c_void_p), ("status", c_void_p),
+      ("table_stride", c_int64), ("parents_stride", c_int64),
+      ("batch", c_int32), ("heads", c_int32), ("kv_heads", c_int32), ("n", c_int32), ("head_dim", c_int32),
+      ("num_pages", c_int32), ("page_size", c_int32), ("table_width", c_int32),
+      ("dtype", c_int32), ("quantized", c_int32), ("window_left", c_int32), ("num_sinks", c_int32),
+      ("mask_value", c_float), ("soft_cap", c_float),
   ]
 
 
@@ -158,6 +175,10 @@ def load():
     fn = getattr(lib, name)
     fn.argtypes = [POINTER(params), c_void_p]
     fn.restype = c_int
+  lib.splash_cached_workspace_bytes.argtypes = [POINTER(SplashCachedParams)]
+  lib.splash_cached_workspace_bytes.restype = c_int64
+  lib.splash_cached_fwd.argtypes = [POINTER(SplashCachedParams), c_void_p, c_int64, c_void_p]
+  lib.splash_cached_fwd.restype = c_int
   _lib = lib
   return lib
 
