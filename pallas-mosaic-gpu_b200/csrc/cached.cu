@@ -6,64 +6,77 @@
 namespace splash {
 
 // Second pass: units that several CTAs shared,
-//   m = max_i m_i, w_i = 2^(m_i - m), l = sum_i w_i l_i, out = sum_i w_i O_i / l, lse = (m + log2 l) ln 2,
-// and zeros for units whose rows see no key at all.  One block per unit (most have nothing to do and leave), one warp per
-// row, the parts in the order of the keys.
+//   m = max_i m_i, w_i = 2^(m_i - m), l = sum_i w_i l_i, out = sum_i w_i O_i / l, lse = (m + log2 l) ln 2.
+// A block per cut between two CTAs and 8 rows; the first cut of a unit has the work, the parts in the order of the keys,
+// a warp per row.  Bound by latency: the weights of up to 32 parts come first, a lane each, then the rows of O together.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) cached_finish_kernel(const CachedArgs a, int grid) {
+__global__ void __launch_bounds__(256) cached_finish_kernel(const CachedArgs a, int ctas) {
+  wait_for_prerequisites();
+  const int c = blockIdx.x + 1, lane = threadIdx.x & 31;
+  const int4 before = a.cuts[c - 1], cut = a.cuts[c];
   if (a.status[0] != 0) return;  // a wait ran out: the parts are not to be read
-  const int unit = blockIdx.x;
-  const int entry = unit / a.kv_heads, head = unit - entry * a.kv_heads;
-  const int begin = a.starts[entry], all = a.starts[entry + 1] - begin, total = a.starts[a.batch * a.row_tiles];
-  const int tiles = all / a.kv_heads, ctas = min(grid, total);
-  const int us = begin + head * tiles, ue = us + tiles;
-  int c0 = 0, c1 = -1;
-  if (tiles > 0) {
-    // The CTA whose share holds tile x: the last c with floor(c * total / ctas) <= x.
-    c0 = static_cast<int>(((us + 1ll) * ctas - 1) / total);
-    c1 = static_cast<int>((static_cast<long long>(ue) * ctas - 1) / total);
-    if (c0 == c1) return;
+  if (cut.x < 0 || cut.z == 0) return;  // no unit goes on here
+  const bool same = before.x == cut.x && before.y == cut.y;
+  if (same && before.z > 0) return;     // not its first cut
+  int last = c;  // the CTA that has the unit's end
+  for (int c0 = c + 1; c0 < ctas; c0 += 32) {
+    bool goes_on = false;
+    if (c0 + lane < ctas) {
+      const int4 x = a.cuts[c0 + lane];
+      goes_on = x.x == cut.x && x.y == cut.y && x.z > 0;
+    }
+    const uint32_t ends = ~__ballot_sync(0xffffffffu, goes_on);
+    if (ends) {
+      last = c0 + __ffs(ends) - 2;
+      break;
+    }
+    last = c0 + 31;
   }
-  const int b = entry / a.row_tiles, rt = entry - b * a.row_tiles;
-  const int rows = min(a.row_cap, a.rows - rt * a.row_cap);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int count = cached_geom(a, entry).count;
-  const long long row0 = static_cast<long long>(b * a.kv_heads + head) * a.rows + rt * a.row_cap;
-  for (int r = warp; r < rows; r += 8) {
-    const bool live = (rt * a.row_cap + r) % a.n < count;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live && tiles > 0) {
-      auto part = [&](int c) {
-        return (2ll * c + (cached_share(c, total, ctas) < us ? 1 : 0)) * a.row_cap + r;
-      };
-      for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_ml[part(c)].x);
+  const int b = cut.x / a.row_tiles, rt = cut.x - b * a.row_tiles;
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (r >= min(a.row_cap, a.rows - rt * a.row_cap)) return;
+  const long long row = static_cast<long long>(b * a.kv_heads + cut.y) * a.rows + rt * a.row_cap + r;
+  const bool live = (rt * a.row_cap + r) % a.n < cached_geom(a, cut.x).count;
+  const int parts = last - c + 2;
+  // Where part i lies: what CTA c - 1 began is its first or its last segment, the others' are their first.
+  auto place = [&](int i) { return (2ll * (c - 1 + i) + (i == 0 && !same ? 1 : 0)) * a.row_cap + r; };
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      const int n = min(32, parts - i0);
+      const float2 ml = lane < n ? a.part_ml[place(i0 + lane)] : make_float2(-INFINITY, 0.f);
+      float top = ml.x;
 #pragma unroll
-      for (int d = 16; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-#pragma unroll 4
-      for (int c = c0; c <= c1; ++c) {
-        const long long at = part(c);
-        const float2 ml = a.part_ml[at];
-        const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : ex2_approx(ml.x - m);  // (a NaN sum stays one)
+      for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float m_new = fmaxf(m, top);
+      const float scale = m == -INFINITY ? (l == l ? 0.f : l) : ex2_approx(m - m_new);  // (a NaN sum stays one)
+      float w = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : ex2_approx(ml.x - m_new);
+      float sum = ml.y * w;
+#pragma unroll
+      for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      m = m_new;
+      l = l * scale + sum;
+      o.x *= scale; o.y *= scale; o.z *= scale; o.w *= scale;
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, i);
         if (lane < D / 4) {
-          const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * D + lane * 4);
-          o.x = fmaf(x.x, w, o.x);
-          o.y = fmaf(x.y, w, o.y);
-          o.z = fmaf(x.z, w, o.z);
-          o.w = fmaf(x.w, w, o.w);
+          const float4 x = *reinterpret_cast<const float4*>(a.part_o + place(i0 + i) * D + lane * 4);
+          o.x = fmaf(x.x, wi, o.x);
+          o.y = fmaf(x.y, wi, o.y);
+          o.z = fmaf(x.z, wi, o.z);
+          o.w = fmaf(x.w, wi, o.w);
         }
-        l = fmaf(ml.y, w, l);
       }
     }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    if (lane < D / 4)
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (row0 + r) * D + lane * 4) =
-          make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
-    if (a.lse_out && lane == 0) a.lse_out[row0 + r] = l != 0.f ? (m + lg2_approx(l)) * kCachedLn2 : a.mask_value;
   }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  if (lane < D / 4)
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * D + lane * 4) =
+        make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
+  if (a.lse_out && lane == 0) a.lse_out[row] = l != 0.f ? (m + lg2_approx(l)) * kCachedLn2 : a.mask_value;
 }
-
-static int64_t round16(int64_t x) { return (x + 15) / 16 * 16; }
 
 static int check_cached(const SplashCachedParams* p) {
   if (!p) return fail(SPLASH_INVALID_ARGUMENT, "params is null");
@@ -85,7 +98,7 @@ static int check_cached(const SplashCachedParams* p) {
   if (rows >= (1ll << 30) || static_cast<int64_t>(p->batch) * p->kv_heads * rows >= limit)
     return fail(SPLASH_INVALID_ARGUMENT, "batch * heads * new tokens must fit in 31 bits");
   const int64_t units = (rows + 31) / 32 * p->batch * p->kv_heads;
-  if (units * (capacity / kCachedTile + 2) >= limit)
+  if (units * (capacity / kCachedTile + 2 + kCachedUnitCost) >= limit)
     return fail(SPLASH_INVALID_ARGUMENT, "batch * kv heads * tiles of rows * tiles of keys must fit in 31 bits");
   return SPLASH_OK;
 }
@@ -94,13 +107,13 @@ static int check_cached(const SplashCachedParams* p) {
 static CachedPlan cached_plan(const SplashCachedParams& p) {
   CachedPlan plan;
   const int64_t rows = static_cast<int64_t>(p.heads / p.kv_heads) * p.n;
-  plan.row_cap = rows <= 32 ? 32 : (rows <= 64 || p.quantized) ? 64 : 128;
+  plan.row_cap = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   plan.row_tiles = static_cast<int>((rows + plan.row_cap - 1) / plan.row_cap);
   const int64_t entries = static_cast<int64_t>(p.batch) * plan.row_tiles;
   const int64_t capacity = static_cast<int64_t>(p.table_width) * p.page_size;
   const int64_t most = entries * p.kv_heads * ((capacity + kCachedTile - 1) / kCachedTile);  // tiles there can be
   plan.ctas = static_cast<int>(most < 1 ? 1 : most < sm_count() ? most : sm_count());
-  plan.part_o = round16((entries + 1) * 4);
+  plan.part_o = static_cast<int64_t>(plan.ctas) * 16;
   plan.part_ml = plan.part_o + static_cast<int64_t>(2) * plan.ctas * plan.row_cap * p.head_dim * 4;
   plan.bytes = plan.part_ml + static_cast<int64_t>(2) * plan.ctas * plan.row_cap * 8;
   return plan;
@@ -136,7 +149,7 @@ extern "C" int splash_cached_fwd(const SplashCachedParams* p, void* workspace, i
   a.out = p->out;
   a.lse_out = p->lse_out;
   a.status = p->status;
-  a.starts = static_cast<int32_t*>(workspace);
+  a.cuts = static_cast<int4*>(workspace);
   a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.part_o);
   a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.part_ml);
   a.table_stride = p->table_stride;
@@ -162,7 +175,17 @@ extern "C" int splash_cached_fwd(const SplashCachedParams* p, void* workspace, i
   if (rc) return rc;
   auto finish = p->head_dim == 64 ? (bf16 ? cached_finish_kernel<64, true> : cached_finish_kernel<64, false>)
                                   : (bf16 ? cached_finish_kernel<128, true> : cached_finish_kernel<128, false>);
-  finish<<<static_cast<unsigned>(static_cast<int64_t>(p->batch) * plan.row_tiles * p->kv_heads), 256, 0, st>>>(a, plan.ctas);
+  if (plan.ctas == 1) return SPLASH_OK;  // nothing is cut
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(plan.ctas - 1, ((a.rows < plan.row_cap ? a.rows : plan.row_cap) + 7) / 8);
+  config.blockDim = dim3(256);
+  config.stream = st;
+  cudaLaunchAttribute dependent[1];
+  dependent[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  dependent[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = dependent;
+  config.numAttrs = 1;
+  SPLASH_CUDA_CHECK(cudaLaunchKernelEx(&config, finish, a, plan.ctas));
   SPLASH_CUDA_CHECK(cudaGetLastError());
   return SPLASH_OK;
 }

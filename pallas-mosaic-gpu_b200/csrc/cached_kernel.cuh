@@ -18,10 +18,11 @@
 // 8-bit caches are not widened on the way: e4m3 keys and values are operands of the MMA as they lie in the cache, and
 // the 16-bit Q and the probabilities are split into e4m3 terms instead, which are few:
 //   * q * 2^-eq = q1 + q2 (+ q3 for f16), each term what the ones before leave; S sums their products.  bf16 has 8 bits,
-//     a term 4: nothing is lost but below 2^-19 of the row's largest number.
+//     a term 4: nothing is lost but below 2^-18 of the row's largest number.
 //   * 2^ek of a key scales its column of S; 2^ev of a value scales its column of P, and the running maximum is one of
-//     s + ev, so that the scaled probabilities stay within 2^8.
-//   * P = p1 + p2 / 16 with p1, p2 e4m3: about 8 bits, as a bf16 P has.  Half of the copies of the rows carry p1, half p2.
+//     s + ev and lags behind by a factor of 2 at most, so that the scaled probabilities end between 128 and 256.
+//   * P = p1 + p2 with p1, p2 e4m3: 8 bits as a bf16 P has, down to 2^-10 of the row's largest scaled probability; below
+//     that the steps stay at 2^-17 of it.
 #pragma once
 
 #include <stddef.h>
@@ -36,6 +37,8 @@ constexpr int kCachedTile = 128;        // keys per tile
 constexpr int kCachedMaxSlots = 12;
 constexpr int kCachedAuxSlots = 16;     // exponents of a tile; more than tiles can be on their way (see the producer)
 constexpr int kCachedMaxTree = 128;     // nodes of a drafted tree
+// What a unit costs besides its tiles, in tiles (its start, and the sum of its parts): it stands that much longer in the line.
+constexpr int kCachedUnitCost = 2;
 constexpr float kCachedLog2e = 1.4426950408889634f;
 constexpr float kCachedLn2 = 0.6931471805599453f;
 
@@ -50,7 +53,7 @@ struct CachedArgs {
   void* out;
   float* lse_out;
   int32_t* status;
-  int32_t* starts;    // [batch * row_tiles + 1] first tile of each (sequence, row tile) in the line, and its length
+  int4* cuts;         // [CTAs] first segment of each: entry (-1: none), kv head, first tile, tiles of the unit
   float* part_o;      // [2 * CTAs, R, D]
   float2* part_ml;    // [2 * CTAs, R]: maximum (powers of 2) and sum
   int64_t table_stride, parents_stride;
@@ -92,41 +95,46 @@ __device__ __forceinline__ CachedGeom cached_geom(const CachedArgs& a, int entry
   return g;
 }
 
-// First tile of CTA c's share of a line of `total` tiles cut for `ctas` CTAs.
-__host__ __device__ __forceinline__ int cached_share(int c, int total, int ctas) {
-  return static_cast<int>(static_cast<long long>(c) * total / ctas);
+// Where CTA c's share of a line of this length begins, cut for `ctas` CTAs.
+__device__ __forceinline__ int cached_share(int c, int length, int ctas) {
+  return static_cast<int>(static_cast<long long>(c) * length / ctas);
 }
 
 // A CTA's way along its share: one segment (a unit or the part of it that falls into the share) after the other.
 struct CachedCursor {
-  int entry, head, tile, left;  // of the next segment; tiles left in the share
+  int entry, head, offset, left;  // the next unit, where in it the share goes on, what is left of the share
   CachedGeom g;
-  int seg_tile, seg_n, seg_entry, seg_head;  // the current segment
+  int seg_tile, seg_n, seg_entry, seg_head;  // the current segment: its unit's tiles seg_tile .. seg_tile + seg_n - 1
   bool whole;                                // it is all of its unit
 
-  __device__ __forceinline__ void start(const CachedArgs& a, int e, int h, int t, int n) {
-    entry = e; head = h; tile = t; left = n;
+  __device__ __forceinline__ void start(const CachedArgs& a, int e, int h, int o, int n) {
+    entry = e; head = h; offset = o; left = n;
     if (left > 0) g = cached_geom(a, entry);
   }
   __device__ __forceinline__ bool next(const CachedArgs& a) {
-    if (left <= 0) return false;
-    if (head == a.kv_heads) {
-      head = 0;
-      const int entries = a.batch * a.row_tiles;
-      do {
-        if (++entry >= entries) return false;
-        g = cached_geom(a, entry);
-      } while (g.tiles == 0);
+    while (left > 0) {
+      if (head == a.kv_heads) {
+        head = 0;
+        const int entries = a.batch * a.row_tiles;
+        do {
+          if (++entry >= entries) return false;
+          g = cached_geom(a, entry);
+        } while (g.tiles == 0);
+      }
+      const int from = max(offset - kCachedUnitCost, 0), to = min(offset + left - kCachedUnitCost, g.tiles);
+      seg_entry = entry;
+      seg_head = head;
+      left -= g.tiles + kCachedUnitCost - offset;
+      offset = 0;
+      ++head;
+      if (to > from) {
+        seg_tile = from;
+        seg_n = to - from;
+        whole = seg_n == g.tiles;
+        return true;
+      }
     }
-    seg_entry = entry;
-    seg_head = head;
-    seg_tile = tile;
-    seg_n = min(g.tiles - tile, left);
-    whole = tile == 0 && seg_n == g.tiles;
-    left -= seg_n;
-    tile = 0;
-    ++head;
-    return true;
+    return false;
   }
   // First key of the segment's i-th tile.
   __device__ __forceinline__ int key0(int i) const {
@@ -137,13 +145,12 @@ struct CachedCursor {
 
 enum CachedSite : int {
   kCSiteLoadEmpty = 301, kCSiteLoadQ, kCSiteMmaQ, kCSiteMmaFull, kCSiteMmaP, kCSiteMmaO, kCSiteSmxS, kCSiteSmxV,
-  kCSiteSmxSync, kCSiteSmxDone, kCSiteConvQ, kCSiteSmxAux,
+  kCSiteSmxSync, kCSiteSmxDone, kCSiteConvQ, kCSiteTree, kCSiteSmxTree,
 };
 
 template <int D, bool BF16, bool QUANT, int KG>
 struct CachedLayout {
-  static constexpr int kCopies = QUANT ? 2 * KG : KG;      // copies of the rows among the 128 of an MMA
-  static constexpr int kRows = 128 / kCopies;              // R
+  static constexpr int kRows = 128 / KG;                   // R: KG copies of the rows are the 128 of an MMA
   static constexpr int kKeys = kCachedTile / KG;           // keys whose probabilities a row's thread computes
   static constexpr int kItem = QUANT ? 1 : 2;
   static constexpr int kRowBytes = D * kItem;              // of a key
@@ -162,7 +169,7 @@ struct CachedLayout {
   static constexpr int kAuxBytes = QUANT ? kCachedAuxSlots * 2 * kCachedTile : 0;
   static constexpr int kScaleBytes = QUANT ? 8 * kKeys * 12 : 0;  // per warp: three numbers for each of its keys
   static constexpr int kQScaleBytes = QUANT ? 2 * 128 * 4 : 0;
-  static constexpr int kTreeBytes = kCachedMaxTree * 4 + 128 * 8 * 4;
+  static constexpr int kTreeBytes = kCachedMaxTree * 8 + 2 * kCachedMaxTree * 8 * 4;  // parents, pointers | two trees
   static constexpr int kFixed = 1024 + kQBytes + kStageBytes + kMlBytes + kBarBytes + kAuxBytes + kScaleBytes + kQScaleBytes + kTreeBytes;
   static constexpr int kSlotsFit = (227 * 1024 - kFixed) / kSlotBytes;
   static constexpr int kSlots = kSlotsFit < kCachedMaxSlots ? kSlotsFit : kCachedMaxSlots;
@@ -178,8 +185,9 @@ struct CachedBarriers {
   uint64_t full[kCachedMaxSlots], empty[kCachedMaxSlots];
   uint64_t s_ready[2], p_ready[2];
   uint64_t q_full, q_free, o_done, o_free, sync;
+  uint64_t tree_full[2], tree_free[2];
   uint32_t tmem_base, abort_flag, dead;
-  int32_t first_entry, first_head, first_tile, num_tiles;
+  int32_t first_entry, first_head, first_offset, share;
 };
 static_assert(sizeof(CachedBarriers) <= 512, "");
 
@@ -241,6 +249,10 @@ __device__ __forceinline__ uint32_t cached_swz(uint32_t row, uint32_t chunk) {
   else return row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4);
 }
 
+// Programmatic dependent launch: the second pass may be set up while this one runs; it waits for its end itself.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ int lds_s8(uint32_t addr) {
   int v;
   asm volatile("ld.shared.s8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -273,7 +285,9 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   const uint32_t scale_u32 = aux_u32 + L::kAuxBytes;
   const uint32_t qscale_u32 = scale_u32 + L::kScaleBytes;
   const uint32_t parents_u32 = qscale_u32 + L::kQScaleBytes;
-  const uint32_t above_u32 = parents_u32 + kCachedMaxTree * 4;  // [128 rows][8 words]: 0, four words of bits, 0
+  const uint32_t ups_u32 = parents_u32 + kCachedMaxTree * 4;
+  // Two trees of [128 nodes][8 words]: 0, four words of the nodes it sees, 0, unused, depth.
+  const uint32_t trees_u32 = ups_u32 + kCachedMaxTree * 4;
 
   const int warp = uniform_warp_index();
   const int lane = threadIdx.x & 31;
@@ -285,12 +299,14 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     for (uint32_t i = lane; i < kNumBarriers; i += 32) {
       const uint32_t off = 8u * i;
       uint32_t count = 1;
-      if (off >= offsetof(CachedBarriers, p_ready) && off < offsetof(CachedBarriers, q_full)) count = 128;
-      if (off == offsetof(CachedBarriers, q_full)) count = QUANT ? 32 : 1;
-      if (off == offsetof(CachedBarriers, o_free) || off == offsetof(CachedBarriers, sync)) count = 256;
+      // The softmax warps arrive once each: 32 arrivals of a warp would be taken one after the other.
+      if (off >= offsetof(CachedBarriers, p_ready) && off < offsetof(CachedBarriers, q_full)) count = 4;
+      if (off == offsetof(CachedBarriers, o_free) || off == offsetof(CachedBarriers, sync)) count = 8;
+      if (off >= offsetof(CachedBarriers, tree_free) && off < offsetof(CachedBarriers, tmem_base)) count = 8;
       mbar_init(bars_u32 + off, count);
     }
     if (lane == 0) {
+      launch_dependents();
       sts32(SPLASH_KWORD(abort_flag), 0);
       sts32(SPLASH_KWORD(dead), a.status[0] != 0);
       prefetch_tensormap(&tm_k);
@@ -304,28 +320,20 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     tmem_relinquish();
   } else if (warp == 0) {
     const int entries = a.batch * a.row_tiles;
+    auto line = [&](int e) -> int {  // what (sequence, row tile) e takes of the line, all kv heads
+      if (e >= entries) return 0;
+      const int tiles = cached_geom(a, e).tiles;
+      return tiles > 0 ? (tiles + kCachedUnitCost) * a.kv_heads : 0;
+    };
     int total = 0;
-    for (int e0 = 0; e0 < entries; e0 += 32) {
-      const int mine = e0 + lane < entries ? cached_geom(a, e0 + lane).tiles * a.kv_heads : 0;
-      if (blockIdx.x == 0) {
-        int before = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-          const int x = __shfl_up_sync(0xffffffffu, before, d);
-          if (lane >= d) before += x;
-        }
-        if (e0 + lane < entries) a.starts[e0 + lane] = total + before - mine;
-      }
-      total += __reduce_add_sync(0xffffffffu, mine);
-    }
-    if (blockIdx.x == 0 && lane == 0) a.starts[entries] = total;
-    const int ctas = min(static_cast<int>(gridDim.x), total);  // a tile at least to each that takes part
+    for (int e0 = 0; e0 < entries; e0 += 32) total += __reduce_add_sync(0xffffffffu, line(e0 + lane));
+    const int ctas = min(static_cast<int>(gridDim.x), total);
     const int c = blockIdx.x;
     const int begin = c < ctas ? cached_share(c, total, ctas) : 0, end = c < ctas ? cached_share(c + 1, total, ctas) : 0;
     if (begin < end) {
       int passed = 0;
       for (int e0 = 0; e0 < entries; e0 += 32) {
-        const int mine = e0 + lane < entries ? cached_geom(a, e0 + lane).tiles * a.kv_heads : 0;
+        const int mine = line(e0 + lane);
         const int sum = __reduce_add_sync(0xffffffffu, mine);
         if (begin < passed + sum) {
           int upto = mine;
@@ -336,17 +344,17 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           }
           const int from = passed + upto - mine;
           if (begin >= from && begin < from + mine) {
-            const int tiles = mine / a.kv_heads;
+            const int unit = mine / a.kv_heads;
             sts32(SPLASH_KWORD(first_entry), e0 + lane);
-            sts32(SPLASH_KWORD(first_head), (begin - from) / tiles);
-            sts32(SPLASH_KWORD(first_tile), (begin - from) % tiles);
+            sts32(SPLASH_KWORD(first_head), (begin - from) / unit);
+            sts32(SPLASH_KWORD(first_offset), (begin - from) % unit);
           }
           break;
         }
         passed += sum;
       }
     }
-    if (lane == 0) sts32(SPLASH_KWORD(num_tiles), end - begin);
+    if (lane == 0) sts32(SPLASH_KWORD(share), end - begin);
   }
   tc_fence_before();
   __syncthreads();
@@ -360,8 +368,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     return;
   }
   CachedCursor cur;
-  cur.start(a, lds32(SPLASH_KWORD(first_entry)), lds32(SPLASH_KWORD(first_head)), lds32(SPLASH_KWORD(first_tile)),
-            lds32(SPLASH_KWORD(num_tiles)));
+  cur.start(a, lds32(SPLASH_KWORD(first_entry)), lds32(SPLASH_KWORD(first_head)), lds32(SPLASH_KWORD(first_offset)),
+            lds32(SPLASH_KWORD(share)));
 
   if (warp >= 8) {
     setmaxnreg_dec<L::kLoadRegs>();
@@ -386,7 +394,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
 #pragma unroll
             for (int c = 0; c < D / 64; ++c)
 #pragma unroll
-              for (int copy = 0; copy < L::kCopies; ++copy)
+              for (int copy = 0; copy < KG; ++copy)
                 tma_load_2d(q_u32 + c * (128 * 128) + copy * (L::kRows * 128), &tm_q, c * 64, row, SPLASH_KBAR(q_full, 0));
           }
         }
@@ -485,9 +493,10 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           tc_fence_after();
           const uint32_t b_lo = desc_lo(ring_u32 + slot * L::kSlotBytes, kCachedTile * L::kBoxBytes);
           constexpr int kKeysPerMma = QUANT ? 32 : 16;
+          // P is 8 columns an MMA; 8 bit: its second term follows in columns 32 .. 63, on the same values.
 #pragma unroll
-          for (int kk = 0; kk < kCachedTile / kKeysPerMma; ++kk) {
-            const uint32_t off = (kk * kKeysPerMma * L::kBoxBytes) >> 4;
+          for (int kk = 0; kk < (QUANT ? 2 : 1) * kCachedTile / kKeysPerMma; ++kk) {
+            const uint32_t off = ((kk * kKeysPerMma) % kCachedTile * L::kBoxBytes) >> 4;
             if constexpr (QUANT) umma8_ts2_w(tmem + L::kOCol + grp * D, tmem + grp * 128 + kk * 8, b_lo + off, kHi, kIdescPV, i > 1 || kk > 0);
             else umma_ts2_w(tmem + L::kOCol + grp * D, tmem + grp * 128 + kk * 8, b_lo + off, kHi, kIdescPV, i > 1 || kk > 0);
           }
@@ -555,7 +564,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
               }
               const uint32_t byte = lane * kPer;
 #pragma unroll
-              for (int copy = 0; copy < L::kCopies; ++copy) {
+              for (int copy = 0; copy < KG; ++copy) {
                 const uint32_t dst = q_u32 + t * L::kQTerm + cached_swz<L::kBoxBytes>(copy * L::kRows + r, byte >> 4) + (byte & 15u);
                 if constexpr (kPer == 4) sts32(dst, code[0] | (code[1] << 16));
                 else asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst), "h"(static_cast<uint16_t>(code[0])) : "memory");
@@ -564,18 +573,93 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           }
         }
         fence_proxy_async_smem();
-        mbar_arrive(SPLASH_KBAR(q_full, 0));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(SPLASH_KBAR(q_full, 0));
+      }
+    } else if (warp == 10 && a.parents != nullptr) {
+      // ------------------------------ drafted trees, a sequence ahead of the softmax ------------------------------------
+      // Which nodes each node sees -- itself and its ancestors -- by doubling: what a node sees is what it and the node
+      // `up` steps above it see, for up = 1, 2, 4, ...
+      int trees = 0, last = -1;
+      for (int seg = 0; cur.next(a); ++seg) {
+        const int b = cur.seg_entry / a.row_tiles;
+        if (b == last) continue;
+        last = b;
+        const int buf = trees & 1;
+        if (trees >= 2 && !warp_wait(SPLASH_KBAR(tree_free, buf), ((trees >> 1) & 1) ^ 1, ctx, kCSiteTree, trees)) break;
+        ++trees;
+        const uint32_t tree = trees_u32 + buf * (kCachedMaxTree * 32);
+        constexpr int kPer = kCachedMaxTree / 32;
+        uint32_t bits[kPer][4];
+        int up[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int i = j * 32 + lane;
+          up[j] = i < a.n ? a.parents[b * a.parents_stride + i] : -1;
+          if (up[j] >= i || up[j] < 0) up[j] = -1;  // a parent stands before its child; anything else is the context
+#pragma unroll
+          for (int w = 0; w < 4; ++w) bits[j][w] = w == j ? 1u << lane : 0u;
+          sts32(parents_u32 + i * 4, static_cast<uint32_t>(up[j]));
+          sts32(ups_u32 + i * 4, static_cast<uint32_t>(up[j]));
+#pragma unroll
+          for (int w = 0; w < 8; ++w) sts32(tree + (i * 8 + w) * 4, w >= 1 && w <= 4 ? bits[j][w - 1] : 0u);
+        }
+        __syncwarp();
+        for (int steps = 1; steps < a.n; steps *= 2) {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            if (up[j] < 0) continue;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) bits[j][w] |= lds32(tree + (up[j] * 8 + 1 + w) * 4);
+            up[j] = static_cast<int>(lds32(ups_u32 + up[j] * 4));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            const int i = j * 32 + lane;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) sts32(tree + (i * 8 + 1 + w) * 4, bits[j][w]);
+            sts32(ups_u32 + i * 4, static_cast<uint32_t>(up[j]));
+          }
+          __syncwarp();
+        }
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int i = j * 32 + lane;
+          const int depth = __popc(bits[j][0]) + __popc(bits[j][1]) + __popc(bits[j][2]) + __popc(bits[j][3]) - 1;
+          sts32(tree + (i * 8 + 7) * 4, static_cast<uint32_t>(depth));
+          if (a.window >= 0 && depth > a.window) {
+            // Ancestors in front of the window: only as sinks.
+#pragma unroll
+            for (int w = 0; w < 4; ++w) bits[j][w] = 0;
+            int x = i;
+            for (int d = depth; d >= 0; --d) {
+              if (d >= depth - a.window || cur.g.before + d < a.sinks) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                  if (w == (x >> 5)) bits[j][w] |= 1u << (x & 31);
+              }
+              x = static_cast<int>(lds32(parents_u32 + x * 4));
+            }
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) sts32(tree + ((j * 32 + lane) * 8 + 1 + w) * 4, bits[j][w]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(SPLASH_KBAR(tree_full, buf));
       }
     }
   } else {
     // ============================================ softmax ==============================================================
     setmaxnreg_inc<L::kSoftmaxRegs>();
+    if (threadIdx.x == 0) a.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);  // (its first segment overwrites it)
     const int grp = warp >> 2;
     const int row_lane = (warp & 3) * 32 + lane;
-    const int copy = row_lane / L::kRows;                   // (the same for a warp: copies are 32 rows or more)
+    const int part = row_lane / L::kRows;                   // which copy of the rows, and which part of a tile's keys
     const int r = row_lane % L::kRows;
-    const int part = QUANT ? copy >> 1 : copy;              // which part of a tile's keys
-    const bool low_term = QUANT && (copy & 1);
     const int col0 = part * L::kKeys;
     const uint32_t tmem_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_tmem = tmem_lane + grp * 128, o_tmem = tmem_lane + L::kOCol + grp * D;
@@ -585,8 +669,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     const float unit = a.soft_cap > 0.f ? a.soft_cap : 1.f;
     const float unit2 = unit * kCachedLog2e;
     const float inv_cap = a.soft_cap > 0.f ? 1.f / a.soft_cap : 1.f;
-    constexpr float kThreshold = QUANT ? 3.f : 8.f;          // powers of 2 by which the maximum may lag behind
-    constexpr float kPScale = QUANT ? 32.f : 1.f;            // 8 bit: P up to 2^3 * 32 = 256
+    constexpr float kThreshold = QUANT ? 1.f : 8.f;          // powers of 2 by which the maximum may lag behind
+    constexpr float kPScale = QUANT ? 128.f : 1.f;           // 8 bit: P up to 2 * 128 of e4m3's 448
     uint32_t s_par = 0, sync_par = 0;
     int seq = 0;     // ring position of the segment's first tile
     int aux0 = 0;    // exponent slot of the segment's first tile
@@ -594,8 +678,13 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     uint32_t zero16[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) zero16[j] = 0;
+    int trees = 0, last_b = -1;
+    auto arrive = [&](uint32_t bar) {  // of a warp, for what all its lanes have done
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
     auto group_sync = [&]() -> bool {
-      mbar_arrive(SPLASH_KBAR(sync, 0));
+      arrive(SPLASH_KBAR(sync, 0));
       const bool fine = warp_wait(SPLASH_KBAR(sync, 0), sync_par, ctx, kCSiteSmxSync, 0);
       sync_par ^= 1;
       return fine;
@@ -609,35 +698,16 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       const int node = row_all % a.n;
       const bool live = row_all < a.rows && node < g.count;
       int depth = node;
+      uint32_t above = 0;  // the words of this row's node
       if (tree) {
-        // Bits of the nodes that a row sees among the drafted ones: itself and its ancestors, as far as the window goes.
-        const int t = threadIdx.x;
-        if (t < a.n) sts32(parents_u32 + t * 4, static_cast<uint32_t>(a.parents[b * a.parents_stride + t]));
-        if (!group_sync()) { ok = false; break; }
-        depth = 0;
-        if (live) {
-          for (int x = node, up; ; x = up, ++depth) {
-            up = static_cast<int>(lds32(parents_u32 + x * 4));
-            if (up < 0 || up >= x) break;  // a parent stands before its child; anything else is the context
-          }
+        if (b != last_b) {
+          if (last_b >= 0) arrive(SPLASH_KBAR(tree_free, (trees - 1) & 1));
+          last_b = b;
+          if (!warp_wait(SPLASH_KBAR(tree_full, trees & 1), (trees >> 1) & 1, ctx, kCSiteSmxTree, seg)) { ok = false; break; }
+          ++trees;
         }
-        if (grp == 0) {
-#pragma unroll
-          for (int w = 0; w < 8; ++w) sts32(above_u32 + (row_lane * 8 + w) * 4, 0);
-          if (live) {
-            int d = depth;
-            for (int x = node;; --d) {
-              if (a.window < 0 || d >= depth - a.window || g.before + d < a.sinks) {
-                const uint32_t at = above_u32 + (row_lane * 8 + 1 + (x >> 5)) * 4;
-                sts32(at, lds32(at) | (1u << (x & 31)));
-              }
-              const int up = static_cast<int>(lds32(parents_u32 + x * 4));
-              if (up < 0 || up >= x) break;
-              x = up;
-            }
-          }
-        }
-        if (!group_sync()) { ok = false; break; }
+        above = trees_u32 + (((trees - 1) & 1) * kCachedMaxTree + node) * 32;
+        depth = static_cast<int>(lds32(above + 28));
       }
       // Keys of the context (tree) or of context and run that this row sees: [v_lo, v_hi) and [0, v_sink).
       const int position = g.before + depth;
@@ -660,6 +730,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
 
       for (int i = grp; i < n; i += 2) {
         const int key0 = cur.key0(i);
+        asm volatile("" : "+r"(page));  // looked at here and not where it was asked for, a tile ago
         const uint32_t good = __ballot_sync(0xffffffffu, page >= 0 && page < a.num_pages);  // pieces that have a page
         page = page_of(i + 2);
         const bool plain = key0 + kCachedTile <= seen_by_all && (key0 >= all_from || key0 + kCachedTile <= g.sink_hi) &&
@@ -707,10 +778,9 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
 #pragma unroll
           for (int j = 0; j < L::kKeys; j += 4) {
             const uint4 k4 = lds128(my_scales + j * 4);
-            sv[j] *= __uint_as_float(k4.x);
-            sv[j + 1] *= __uint_as_float(k4.y);
-            sv[j + 2] *= __uint_as_float(k4.z);
-            sv[j + 3] *= __uint_as_float(k4.w);
+            const float2 x = mul2(make_float2(sv[j], sv[j + 1]), make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)));
+            const float2 y = mul2(make_float2(sv[j + 2], sv[j + 3]), make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)));
+            sv[j] = x.x; sv[j + 1] = x.y; sv[j + 2] = y.x; sv[j + 3] = y.y;
           }
         }
         if (a.soft_cap > 0.f) {
@@ -724,8 +794,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             uint32_t vis = bit_run(v_lo - kb, v_hi - kb) | bit_run(-kb, v_sink - kb);
             const int d0 = kb - g.before;
             if (tree && d0 > -32 && d0 < kCachedMaxTree) {
-              const uint32_t w = above_u32 + (row_lane * 8 + 1 + (d0 >> 5)) * 4;
-              vis |= __funnelshift_r(lds32(w), lds32(w + 4), d0 & 31);
+              const uint32_t w = above + (1 + (d0 >> 5)) * 4;
+              if (live) vis |= __funnelshift_r(lds32(w), lds32(w + 4), d0 & 31);
             }
             if (piece >= 32) {
               if (!((good >> (at / piece)) & 1u)) vis = 0;
@@ -738,39 +808,41 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
               if (!((vis >> j) & 1u)) sv[c * 32 + j] = -INFINITY;
           }
           // Values that no row sees are cleared: their probability is 0, and 0 times what lies there may be NaN.
-          const bool clear = !there(row_lane);
-          if (__any_sync(0xffffffffu, clear)) {
+          const uint32_t clear = __ballot_sync(0xffffffffu, !there(row_lane));
+          if (clear) {
             const int at = seq + (i + 1 < n ? 2 * i + 2 : 2 * n - 1);  // place of V(i) among the loads
             const int slot = at % L::kSlots;
             if (!warp_wait(SPLASH_KBAR(full, slot), (at / L::kSlots) & 1, ctx, kCSiteSmxV, i)) { ok = false; break; }
-            if (clear) {
-              const uint32_t dst = ring_u32 + slot * L::kSlotBytes + row_lane * L::kBoxBytes;
+            // The warp's 32 rows of the tile, 32 pieces of 16 bytes at a time.
+            constexpr int kChunks = L::kBoxBytes / 16, kAtOnce = 32 / kChunks;
+            const uint32_t dst = ring_u32 + slot * L::kSlotBytes + (warp & 3) * 32 * L::kBoxBytes + (lane % kChunks) * 16;
+#pragma unroll 1
+            for (int k = lane / kChunks; k < 32; k += kAtOnce)
+              if ((clear >> k) & 1u)
 #pragma unroll
-              for (int c = 0; c < L::kBoxes; ++c)
-#pragma unroll
-                for (int k = 0; k < L::kBoxBytes / 16; ++k)
-                  sts128(dst + c * (kCachedTile * L::kBoxBytes) + k * 16, make_uint4(0, 0, 0, 0));
-            }
+                for (int c = 0; c < L::kBoxes; ++c)
+                  sts128(dst + c * (kCachedTile * L::kBoxBytes) + k * L::kBoxBytes, make_uint4(0, 0, 0, 0));
             fence_proxy_async_smem();
           }
         }
 
         // ---- online softmax with a maximum that may lag behind ----
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const float2 mul_2 = make_float2(mul, mul);
+        float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
         for (int j = 0; j < L::kKeys; j += 4) {
           if constexpr (QUANT) {
             const uint4 e4 = lds128(my_scales + (L::kKeys + j) * 4);
-            mx[0] = fmaxf(mx[0], fmaf(sv[j], mul, __uint_as_float(e4.x)));
-            mx[1] = fmaxf(mx[1], fmaf(sv[j + 1], mul, __uint_as_float(e4.y)));
-            mx[2] = fmaxf(mx[2], fmaf(sv[j + 2], mul, __uint_as_float(e4.z)));
-            mx[3] = fmaxf(mx[3], fmaf(sv[j + 3], mul, __uint_as_float(e4.w)));
+            const float2 x = fma2(make_float2(sv[j], sv[j + 1]), mul_2, make_float2(__uint_as_float(e4.x), __uint_as_float(e4.y)));
+            const float2 y = fma2(make_float2(sv[j + 2], sv[j + 3]), mul_2, make_float2(__uint_as_float(e4.z), __uint_as_float(e4.w)));
+            mx0 = max3(mx0, x.x, x.y);
+            mx1 = max3(mx1, y.x, y.y);
           } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], sv[j + k]);
+            mx0 = max3(mx0, sv[j], sv[j + 1]);
+            mx1 = max3(mx1, sv[j + 2], sv[j + 3]);
           }
         }
-        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        float top = fmaxf(mx0, mx1);
         if constexpr (!QUANT) top *= mul;
         const float m_new = fmaxf(m_run, top);
         const bool moved = m_new - m_run > kThreshold;  // false for NaN (-inf - -inf)
@@ -781,57 +853,57 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           l_run *= alpha;
         }
         const float shift = m_run == -INFINITY ? 0.f : -m_run;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (QUANT) {
-          // 128 codes are 32 columns.
-          uint32_t pk[L::kKeys / 4];
+        const float2 shift_2 = make_float2(shift, shift);
+        float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
+        // P lies over S, 32 keys at a time: 16 columns of 16-bit numbers, or 8 columns of either e4m3 term, the second
+        // term 32 columns behind the first.  It is zero for the keys of the other copies.
 #pragma unroll
-          for (int j = 0; j < L::kKeys; j += 4) {
-            const uint4 v4 = lds128(my_scales + (2 * L::kKeys + j) * 4);
-            const float vs[4] = {__uint_as_float(v4.x), __uint_as_float(v4.y), __uint_as_float(v4.z), __uint_as_float(v4.w)};
-            float p[4];
+        for (int c = 0; c < L::kKeys / 32; ++c) {
+          if constexpr (QUANT) {
+            uint32_t p1[8], p2[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float e = ex2_approx(fmaf(sv[j + k], mul, shift));
-              sum[k] += e;
-              p[k] = e * vs[k];
+            for (int j = 0; j < 8; ++j) {
+              const int at = c * 32 + j * 4;
+              const uint4 v4 = lds128(my_scales + (2 * L::kKeys + at) * 4);
+              const float2 x = fma2(make_float2(sv[at], sv[at + 1]), mul_2, shift_2);
+              const float2 y = fma2(make_float2(sv[at + 2], sv[at + 3]), mul_2, shift_2);
+              const float2 ex = make_float2(ex2_approx(x.x), ex2_approx(x.y)), ey = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+              sum_a = add2(sum_a, ex);
+              sum_b = add2(sum_b, ey);
+              const float2 px = mul2(ex, make_float2(__uint_as_float(v4.x), __uint_as_float(v4.y)));
+              const float2 py = mul2(ey, make_float2(__uint_as_float(v4.z), __uint_as_float(v4.w)));
+              const uint32_t cx = e4m3x2(px.x, px.y), cy = e4m3x2(py.x, py.y);
+              const float2 rx = sub2(px, e4m3x2_to_f32(cx)), ry = sub2(py, e4m3x2_to_f32(cy));
+              p1[j] = cx | (cy << 16);
+              p2[j] = e4m3x2(rx.x, rx.y) | (e4m3x2(ry.x, ry.y) << 16);
             }
-            uint32_t c0 = e4m3x2(p[0], p[1]), c1 = e4m3x2(p[2], p[3]);
-            if (low_term) {
-              const float2 f0 = e4m3x2_to_f32(c0), f1 = e4m3x2_to_f32(c1);
-              c0 = e4m3x2((p[0] - f0.x) * 16.f, (p[1] - f0.y) * 16.f);
-              c1 = e4m3x2((p[2] - f1.x) * 16.f, (p[3] - f1.y) * 16.f);
+            tmem_st8(s_tmem + col0 / 4 + c * 8, p1);
+            tmem_st8(s_tmem + 32 + col0 / 4 + c * 8, p2);
+          } else {
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 x = fma2(make_float2(sv[c * 32 + 2 * j], sv[c * 32 + 2 * j + 1]), mul_2, shift_2);
+              const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+              if (j & 1) sum_b = add2(sum_b, e); else sum_a = add2(sum_a, e);
+              pk[j] = pack2<BF16>(e.x, e.y);
             }
-            pk[j / 4] = c0 | (c1 << 16);
+            tmem_st16(s_tmem + col0 / 2 + c * 16, pk);
           }
+        }
+        if constexpr (KG > 1) {
 #pragma unroll
-          for (int c = 0; c < 32 / 16; ++c) {
-            if (c * 16 >= col0 / 4 && c * 16 < (col0 + L::kKeys) / 4) {
-              if constexpr (L::kKeys == 128) tmem_st16(s_tmem + c * 16, pk + c * 16);
-              else tmem_st16(s_tmem + c * 16, pk);
+          for (int c = 0; c < 4; ++c) {
+            if (c * 32 >= col0 && c * 32 < col0 + L::kKeys) continue;
+            if constexpr (QUANT) {
+              tmem_st8(s_tmem + c * 8, zero16);
+              tmem_st8(s_tmem + 32 + c * 8, zero16);
             } else {
               tmem_st16(s_tmem + c * 16, zero16);
             }
           }
-        } else {
-          // 128 probabilities of 16 bits are 64 columns; those of the other copies' keys are zero here.
-#pragma unroll
-          for (int c = 0; c < L::kKeys / 32; ++c) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float e0 = ex2_approx(fmaf(sv[c * 32 + 2 * j], mul, shift));
-              const float e1 = ex2_approx(fmaf(sv[c * 32 + 2 * j + 1], mul, shift));
-              sum[j & 3] += e0 + e1;
-              pk[j] = pack2<BF16>(e0, e1);
-            }
-            tmem_st16(s_tmem + col0 / 2 + c * 16, pk);
-          }
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (c * 16 < col0 / 2 || c * 16 >= (col0 + L::kKeys) / 2) tmem_st16(s_tmem + c * 16, zero16);
         }
-        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l_run += (sum_a.x + sum_a.y) + (sum_b.x + sum_b.y);
         // The scores of this tile came after P.V of the warpgroup's previous one: O stands still.
         if (i >= 2 && __any_sync(0xffffffffu, moved)) {
 #pragma unroll 1
@@ -846,7 +918,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(SPLASH_KBAR(p_ready, grp));
+        arrive(SPLASH_KBAR(p_ready, grp));
       }
       if (!ok) break;
 
@@ -859,23 +931,24 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       float m_tot = -INFINITY, l_tot = 0.f;
 #pragma unroll
       for (int src = 0; src < 2 * KG; ++src) {
-        const uint32_t at = ml_u32 + ((src / KG) * 128 + (src % KG) * (QUANT ? 2 : 1) * L::kRows + r) * 8;
+        const uint32_t at = ml_u32 + ((src / KG) * 128 + (src % KG) * L::kRows + r) * 8;
         m_tot = fmaxf(m_tot, __uint_as_float(lds32(at)));
       }
 #pragma unroll
       for (int src = 0; src < 2 * KG; ++src) {
-        const uint32_t at = ml_u32 + ((src / KG) * 128 + (src % KG) * (QUANT ? 2 : 1) * L::kRows + r) * 8;
+        const uint32_t at = ml_u32 + ((src / KG) * 128 + (src % KG) * L::kRows + r) * 8;
         const float m = __uint_as_float(lds32(at)), l = __uint_as_float(lds32(at + 4));
         if (l != 0.f) l_tot += m == -INFINITY ? l : l * ex2_approx(m - m_tot);
       }
       const bool whole = cur.whole;
       float w = m_run == -INFINITY ? 0.f : ex2_approx(m_run - m_tot);
-      w *= (low_term ? 1.f / 16 : 1.f) / kPScale;
+      w *= 1.f / kPScale;
       if (l_run != l_run) w = l_run;  // NaN: no maximum may have been met
       if (whole) w *= l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
       const long long out_row0 = static_cast<long long>(b * a.kv_heads + cur.seg_head) * a.rows + rt * L::kRows;
       const long long part0 = static_cast<long long>(2 * blockIdx.x + (seg > 0)) * L::kRows;
-      if (grp == 0 && copy == 0) {
+      if (seg == 0 && threadIdx.x == 0) a.cuts[blockIdx.x] = make_int4(cur.seg_entry, cur.seg_head, cur.seg_tile, g.tiles);
+      if (grp == 0 && part == 0) {
         if (!whole) a.part_ml[part0 + r] = make_float2(m_tot, l_tot);
         else if (a.lse_out && row_all < a.rows)
           a.lse_out[out_row0 + r] = live && l_tot != 0.f ? (m_tot + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
@@ -892,7 +965,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
         if (c == D / 32 - 1) {
           tc_fence_before();
-          mbar_arrive(SPLASH_KBAR(o_free, 0));
+          arrive(SPLASH_KBAR(o_free, 0));
         }
         const uint32_t dst = stage_u32 + threadIdx.x * (L::kStageStride * 4);
         const bool any = grp < n && live;
@@ -913,8 +986,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           const int col = (sum_sub * kQuads + k) * 4;
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int src = 0; src < 2 * L::kCopies; ++src) {
-            const int from = (src / L::kCopies) * 128 + (src % L::kCopies) * L::kRows + sum_row;
+          for (int src = 0; src < 2 * KG; ++src) {
+            const int from = (src / KG) * 128 + (src % KG) * L::kRows + sum_row;
             const uint4 x = lds128(stage_u32 + (from * L::kStageStride + col) * 4);
             acc.x += __uint_as_float(x.x);
             acc.y += __uint_as_float(x.y);
@@ -932,6 +1005,19 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       }
       seq += 2 * n;
       aux0 += n;
+    }
+    // Units whose rows see no key stand nowhere in the line: zeros.
+    for (int e = blockIdx.x; ok && e < a.batch * a.row_tiles; e += gridDim.x) {
+      if (cached_geom(a, e).tiles > 0) continue;
+      const int b = e / a.row_tiles, rt = e - b * a.row_tiles;
+      const int rows = min(L::kRows, a.rows - rt * L::kRows);
+      for (int h = 0; h < a.kv_heads; ++h) {
+        const long long row0 = static_cast<long long>(b * a.kv_heads + h) * a.rows + rt * L::kRows;
+        for (int x = threadIdx.x; x < rows * (D / 8); x += 256)
+          reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row0 * D)[x] = make_uint4(0, 0, 0, 0);
+        if (a.lse_out)
+          for (int x = threadIdx.x; x < rows; x += 256) a.lse_out[row0 + x] = a.mask_value;
+      }
     }
   }
 

@@ -29,9 +29,11 @@ int launch_cached_form(const SplashCachedParams& p, const CachedPlan& plan, Cach
 
 template <int D, bool BF16>
 int launch_cached(const SplashCachedParams& p, const CachedPlan& plan, const CachedArgs& a, cudaStream_t stream) {
-  if (p.quantized)
-    return plan.row_cap == 32 ? launch_cached_form<D, BF16, true, 2>(p, plan, a, stream)
-                              : launch_cached_form<D, BF16, true, 1>(p, plan, a, stream);
+  if (p.quantized) {
+    if (plan.row_cap == 32) return launch_cached_form<D, BF16, true, 4>(p, plan, a, stream);
+    if (plan.row_cap == 64) return launch_cached_form<D, BF16, true, 2>(p, plan, a, stream);
+    return launch_cached_form<D, BF16, true, 1>(p, plan, a, stream);
+  }
   if (plan.row_cap == 32) return launch_cached_form<D, BF16, false, 4>(p, plan, a, stream);
   if (plan.row_cap == 64) return launch_cached_form<D, BF16, false, 2>(p, plan, a, stream);
   return launch_cached_form<D, BF16, false, 1>(p, plan, a, stream);
