@@ -266,6 +266,7 @@ typedef struct SplashCachedParams {
   void* out;                  /* [batch, heads, n, head_dim], 16-byte aligned                   */
   float* lse_out;             /* [batch, heads, n] natural log, or NULL                         */
   int32_t* status;            /* 4 x int32, see above                                           */
+  int32_t* status_host;       /* pinned host copy that a kernel which gives up a wait writes too, or NULL */
   int64_t table_stride, parents_stride;
   int32_t batch, heads, kv_heads, n, head_dim;
   int32_t num_pages, page_size, table_width;

@@ -149,6 +149,7 @@ extern "C" int splash_cached_fwd(const SplashCachedParams* p, void* workspace, i
   a.out = p->out;
   a.lse_out = p->lse_out;
   a.status = p->status;
+  a.status_host = p->status_host;
   a.cuts = static_cast<int4*>(workspace);
   a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.part_o);
   a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.part_ml);
@@ -162,7 +163,7 @@ extern "C" int splash_cached_fwd(const SplashCachedParams* p, void* workspace, i
   a.row_tiles = plan.row_tiles;
   a.row_cap = plan.row_cap;
   a.num_pages = p->num_pages;
-  a.page_size = p->page_size;
+  for (a.page_shift = 4; (1 << a.page_shift) < p->page_size; ++a.page_shift) {}
   a.table_width = p->table_width;
   a.window = p->window_left < 0 ? -1 : p->window_left < (1 << 30) ? p->window_left : (1 << 30);
   a.sinks = p->num_sinks < (1 << 30) ? p->num_sinks : (1 << 30);

@@ -53,12 +53,13 @@ struct CachedArgs {
   void* out;
   float* lse_out;
   int32_t* status;
+  int32_t* status_host;
   int4* cuts;         // [CTAs] first segment of each: entry (-1: none), kv head, first tile, tiles of the unit
   float* part_o;      // [2 * CTAs, R, D]
   float2* part_ml;    // [2 * CTAs, R]: maximum (powers of 2) and sum
   int64_t table_stride, parents_stride;
   int32_t batch, heads, kv_heads, n, rows, row_tiles, row_cap;  // rows = heads / kv_heads * n
-  int32_t num_pages, page_size, table_width;
+  int32_t num_pages, page_shift, table_width;  // pages of 2^page_shift tokens
   int32_t window, sinks;  // window < 0: none
   float mask_value, soft_cap;
 };
@@ -74,7 +75,7 @@ struct CachedGeom {
 __device__ __forceinline__ CachedGeom cached_geom(const CachedArgs& a, int entry) {
   CachedGeom g;
   const int b = entry / a.row_tiles, rt = entry - b * a.row_tiles;
-  const int capacity = a.table_width * a.page_size;  // (checked on the host to fit)
+  const int capacity = a.table_width << a.page_shift;  // (checked on the host to fit)
   const int len = min(max(a.lengths[b], 0), capacity);
   g.count = min(a.counts ? min(max(a.counts[b], 0), a.n) : a.n, len);
   g.before = len - g.count;
@@ -204,6 +205,12 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t two) {
 }
 __device__ __forceinline__ float exponent_scale(int e) {  // -128 marks a row that was not finite
   return e == -128 ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+// Rounded to four significant bits.
+__device__ __forceinline__ float2 four_bits(float2 x) {
+  return make_float2(__uint_as_float((__float_as_uint(x.x) + 0x80000u) & 0xfff00000u),
+                     __uint_as_float((__float_as_uint(x.y) + 0x80000u) & 0xfff00000u));
 }
 
 // Warp-collective forms as in ptx.cuh, for 8-bit operands (kind::f8f6f4, e4m3 by e4m3).
@@ -377,8 +384,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       // ------------------------------------------ loads --------------------------------------------------------------
       // Order of the tiles in the ring, for T tiles of a segment: K0 K1 V0 K2 V1 ... K(T-1) V(T-2) V(T-1), which is the
       // order in which the MMA warp uses them.  A lane has one page of a tile.
-      const int piece = min(a.page_size, kCachedTile);  // keys per TMA box
-      const int pieces = kCachedTile / piece;
+      const int piece_shift = min(a.page_shift, 7), piece = 1 << piece_shift;  // keys per TMA box
+      const int pieces = kCachedTile >> piece_shift;
       int slot = 0;
       uint32_t phase = 0;
       int seq = 0, aux = 0;
@@ -404,10 +411,9 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           if (i >= cur.seg_n || lane >= pieces) return -1;
           const int key = cur.key0(i) + lane * piece;
           if (key >= g.hi || (key + piece <= g.lo && key >= g.sink_hi)) return -1;
-          const int entry = key / a.page_size;
-          const int page = table[entry];
+          const int page = table[key >> a.page_shift];
           if (page < 0 || page >= a.num_pages) return -1;
-          return (page * a.kv_heads + cur.seg_head) * a.page_size + (key - entry * a.page_size);
+          return ((page * a.kv_heads + cur.seg_head) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
         };
         int row = piece_row(0), row_before = -1;
         for (int i = 0; i <= cur.seg_n; ++i) {
@@ -664,7 +670,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     const uint32_t tmem_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_tmem = tmem_lane + grp * 128, o_tmem = tmem_lane + L::kOCol + grp * D;
     const uint32_t my_scales = scale_u32 + warp * (L::kKeys * 12);
-    const int piece = min(a.page_size, kCachedTile);
+    const int piece_shift = min(a.page_shift, 7);
     const bool tree = a.parents != nullptr;
     const float unit = a.soft_cap > 0.f ? a.soft_cap : 1.f;
     const float unit2 = unit * kCachedLog2e;
@@ -720,11 +726,13 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       float q_mul = inv_cap;  // what takes a score to the argument of the soft-cap
       float mul = unit2;      // ... and what it holds then to powers of 2
       float m_run = -INFINITY, l_run = 0.f;  // powers of 2; 8 bit: the maximum of s + ev
-      const int pages = kCachedTile / piece;
+      const int pages = kCachedTile >> piece_shift;
       auto page_of = [&](int i) -> int {  // lane p: page id of piece p of tile i (anything for pieces nobody sees)
         if (i >= n || lane >= pages) return 0;
-        const int key = cur.key0(i) + lane * piece;
-        return key < g.hi ? table[key / a.page_size] : 0;
+        const int key = cur.key0(i) + (lane << piece_shift);
+        int id = 0;  // (asked for here, whatever the compiler thinks of its use a tile later)
+        if (key < g.hi) asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(id) : "l"(table + (key >> a.page_shift)));
+        return id;
       };
       int page = page_of(grp);
 
@@ -738,7 +746,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         // Whether key `at` of the tile is there for some row; the others may hold anything, and nothing was loaded for some.
         auto there = [&](int at) {
           const int key = key0 + at;
-          return key < g.hi && (key >= g.lo || key < g.sink_hi) && ((good >> (at / piece)) & 1u);
+          return key < g.hi && (key >= g.lo || key < g.sink_hi) && ((good >> (at >> piece_shift)) & 1u);
         };
         if (!warp_wait(SPLASH_KBAR(s_ready, grp), s_par, ctx, kCSiteSmxS, i)) { ok = false; break; }
         s_par ^= 1;
@@ -797,8 +805,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
               const uint32_t w = above + (1 + (d0 >> 5)) * 4;
               if (live) vis |= __funnelshift_r(lds32(w), lds32(w + 4), d0 & 31);
             }
-            if (piece >= 32) {
-              if (!((good >> (at / piece)) & 1u)) vis = 0;
+            if (piece_shift >= 5) {
+              if (!((good >> (at >> piece_shift)) & 1u)) vis = 0;
             } else {
               if (!((good >> (at / 16)) & 1u)) vis &= 0xffff0000u;
               if (!((good >> (at / 16 + 1)) & 1u)) vis &= 0x0000ffffu;
@@ -872,9 +880,10 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
               sum_b = add2(sum_b, ey);
               const float2 px = mul2(ex, make_float2(__uint_as_float(v4.x), __uint_as_float(v4.y)));
               const float2 py = mul2(ey, make_float2(__uint_as_float(v4.z), __uint_as_float(v4.w)));
-              const uint32_t cx = e4m3x2(px.x, px.y), cy = e4m3x2(py.x, py.y);
-              const float2 rx = sub2(px, e4m3x2_to_f32(cx)), ry = sub2(py, e4m3x2_to_f32(cy));
-              p1[j] = cx | (cy << 16);
+              // The first term is P rounded to four bits, in integer arithmetic: its code need not be read back.
+              const float2 hx = four_bits(px), hy = four_bits(py);
+              const float2 rx = sub2(px, hx), ry = sub2(py, hy);
+              p1[j] = e4m3x2(hx.x, hx.y) | (e4m3x2(hy.x, hy.y) << 16);
               p2[j] = e4m3x2(rx.x, rx.y) | (e4m3x2(ry.x, ry.y) << 16);
             }
             tmem_st8(s_tmem + col0 / 4 + c * 8, p1);
@@ -953,9 +962,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         else if (a.lse_out && row_all < a.rows)
           a.lse_out[out_row0 + r] = live && l_tot != 0.f ? (m_tot + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
       }
-      constexpr int kPerRow = 256 / L::kRows;   // threads that add up one row of a chunk of 32 columns
-      constexpr int kQuads = 8 / kPerRow;       // groups of four columns each of them has
-      const int sum_row = threadIdx.x / kPerRow, sum_sub = threadIdx.x % kPerRow;
+      const int col = (threadIdx.x % 8) * 4;  // of a chunk of 32: eight threads add up a row of it, 128 bytes
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -982,22 +989,23 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
         if (!group_sync()) { ok = false; break; }
 #pragma unroll
-        for (int k = 0; k < kQuads; ++k) {
-          const int col = (sum_sub * kQuads + k) * 4;
+        for (int k = 0; k < L::kRows / 32; ++k) {
+          const int row = k * 32 + threadIdx.x / 8;
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int src = 0; src < 2 * KG; ++src) {
-            const int from = (src / KG) * 128 + (src % KG) * L::kRows + sum_row;
+            const int from = (src / KG) * 128 + (src % KG) * L::kRows + row;
             const uint4 x = lds128(stage_u32 + (from * L::kStageStride + col) * 4);
             acc.x += __uint_as_float(x.x);
             acc.y += __uint_as_float(x.y);
             acc.z += __uint_as_float(x.z);
             acc.w += __uint_as_float(x.w);
           }
+          if (rt * L::kRows + row >= a.rows) continue;
           if (!whole) {
-            *reinterpret_cast<float4*>(a.part_o + (part0 + sum_row) * D + c * 32 + col) = acc;
-          } else if (rt * L::kRows + sum_row < a.rows) {
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (out_row0 + sum_row) * D + c * 32 + col) =
+            *reinterpret_cast<float4*>(a.part_o + (part0 + row) * D + c * 32 + col) = acc;
+          } else {
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (out_row0 + row) * D + c * 32 + col) =
                 make_uint2(pack2<BF16>(acc.x, acc.y), pack2<BF16>(acc.z, acc.w));
           }
         }
@@ -1025,7 +1033,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   tc_fence_before();
   __syncthreads();
   if (const uint32_t gave_up = lds32(SPLASH_KWORD(abort_flag))) {
-    if (threadIdx.x == 0) report_abort(a.status, gave_up);
+    if (threadIdx.x == 0) report_abort(a.status, gave_up, a.status_host);
     // Copies still in flight land before the shared memory goes to another CTA.
     const uint64_t t0 = global_timer_ns();
     while (global_timer_ns() - t0 < 200000) {}

@@ -132,11 +132,19 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const W
 }
 
 // Teardown: one thread publishes what a waiter of this CTA stored (first CTA wins).
-__device__ __forceinline__ void report_abort(int* status, uint32_t word) {
+// `host`: a copy of the record in pinned host memory, or null.
+__device__ __forceinline__ void report_abort(int* status, uint32_t word, volatile int* host = nullptr) {
   if (atomicCAS(status, 0, kDevWaitTimeout) == 0) {
     status[1] = static_cast<int>((word >> 20) & 0x7ffu);
     status[2] = static_cast<int>(blockIdx.x);
     status[3] = static_cast<int>(word & 0xfffffu);
+    if (host) {
+      host[1] = status[1];
+      host[2] = status[2];
+      host[3] = status[3];
+      __threadfence_system();
+      host[0] = kDevWaitTimeout;
+    }
   }
   __threadfence();
 }

@@ -112,7 +112,7 @@ class SplashCachedParams(Structure):
   _fields_ = [
       ("q", c_void_p), ("k_cache", c_void_p), ("v_cache", c_void_p), ("k_exponent", c_void_p), ("v_exponent", c_void_p),
       ("page_table", c_void_p), ("lengths", c_void_p), ("counts", c_void_p), ("parents", c_void_p),
-      ("out", c_void_p), ("lse_out", c_void_p), ("status", c_void_p),
+      ("out", c_void_p), ("lse_out", c_void_p), ("status", c_void_p), ("status_host", c_void_p),
       ("table_stride", c_int64), ("parents_stride", c_int64),
       ("batch", c_int32), ("heads", c_int32), ("kv_heads", c_int32), ("n", c_int32), ("head_dim", c_int32),
       ("num_pages", c_int32), ("page_size", c_int32), ("table_width", c_int32),

@@ -17,13 +17,14 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
 
 import torch
 
 from . import _ffi
 from .config import DEFAULT_MASK_VALUE
-from .kv_cache import KVCache, _index_tensor
-from .splash_attention import (_TORCH_DTYPES, _maybe_check, _on_device, _poll_status, _raw_stream, _status_word)
+from .kv_cache import KVCache, _index_tensor, _remember, _signature
+from .splash_attention import (_TORCH_DTYPES, _launch, _poll_status, _status_host, _status_word, check_device_status)
 
 MAX_TREE = 128
 
@@ -36,6 +37,7 @@ class CachedAttentionKernel:
     self.num_sinks = num_sinks
     self.attn_logits_soft_cap = attn_logits_soft_cap
     self.mask_value = mask_value
+    self._calls: dict = {}
 
   def __repr__(self):
     return (f"CachedAttentionKernel(window_left={self.window_left}, num_sinks={self.num_sinks},"
@@ -52,19 +54,68 @@ class CachedAttentionKernel:
       front of the new ones.  It sees those, its ancestors and itself, and its position is one behind its parent's.
       None: token i follows token i - 1.
     """
-    if not isinstance(q, torch.Tensor):
-      raise TypeError("q must be a torch tensor")
+    for x in (q, page_table, lengths):
+      if not isinstance(x, torch.Tensor):
+        raise TypeError("q, page_table and lengths must be torch tensors")
     if not isinstance(cache, KVCache):
       raise TypeError(f"cache must be a KVCache, got {type(cache).__name__}")
+    if q.requires_grad and torch.is_grad_enabled():
+      raise NotImplementedError("attention over the cache has no backward pass; call it under torch.no_grad()")
+    if q.ndim == 3:
+      out = self(q[None], cache, page_table, lengths, counts=counts, parents=parents, save_residuals=save_residuals)
+      return (out[0][0], (out[1][0][0],)) if save_residuals else out[0]
+    # What a call is made of besides its pointers, checked and filled in once per class of calls.
+    key = (q.shape, q.stride(), q.dtype, q.device, cache.k.shape, cache.k.dtype, cache.k.device, page_table.shape,
+           page_table.stride(), page_table.dtype, page_table.device, lengths.shape, lengths.stride(), lengths.dtype, lengths.device,
+           None if counts is None else _signature(counts), None if parents is None else _signature(parents))
+    known = self._calls.get(key)
+    if known is None:
+      as_given = (q, page_table, lengths, counts, parents)
+      p, *arguments = self._params(*as_given, cache)
+      if any(x is not y for x, y in zip(as_given, arguments)):  # copies that the kernels can read
+        q, page_table, lengths, counts, parents = arguments
+        return self(q, cache, page_table, lengths, counts=counts, parents=parents, save_residuals=save_residuals)
+      # The workspace of a call is made like this tensor of one byte, spread over its size.
+      with torch.cuda.device(q.device):
+        nbytes = int(_ffi.load().splash_cached_workspace_bytes(ctypes.byref(p)))
+      spread = torch.empty(1, dtype=torch.uint8, device=q.device).expand(max(nbytes, 16))
+      known = _remember(self._calls, key, (bytes(p), nbytes, spread))
+    template, nbytes, spread = known
+    if q.data_ptr() % 16:
+      q = q.clone()
+    device = q.device
+    out = torch.empty_like(q)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if save_residuals else None
+    p = _ffi.SplashCachedParams.from_buffer_copy(template)
+    if p.batch and p.n:
+      _poll_status(device)
+      p.q, p.k_cache, p.v_cache, p.out = q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), out.data_ptr()
+      if p.quantized:
+        p.k_exponent, p.v_exponent = cache.k_exponent.data_ptr(), cache.v_exponent.data_ptr()
+      p.page_table, p.lengths = page_table.data_ptr(), lengths.data_ptr()
+      if counts is not None:
+        p.counts = counts.data_ptr()
+      if parents is not None:
+        p.parents = parents.data_ptr()
+      if lse is not None:
+        p.lse_out = lse.data_ptr()
+      mode = os.environ.get("SPLASH_CHECK_STATUS", "async")
+      p.status = _status_word(device).data_ptr()
+      p.status_host = _status_host(device) if mode != "0" else None
+      workspace = torch.empty_like(spread, memory_format=torch.contiguous_format)
+      rc = _launch(device, _ffi.load().splash_cached_fwd, ctypes.byref(p), workspace.data_ptr(), nbytes)
+      if rc:
+        _ffi.check(rc, "attention over the cache")
+      if mode == "1":
+        check_device_status(device)
+    return (out, (lse,)) if save_residuals else out
+
+  def _params(self, q, page_table, lengths, counts, parents, cache):
+    """The parameter block of a call of this class without its pointers, and the arguments as the kernels read them."""
     if not q.is_cuda:
       raise RuntimeError("attention over the cache runs only on a CUDA (sm_100a) device; there is no CPU path.")
-    if torch.is_grad_enabled() and q.requires_grad:
-      raise NotImplementedError("attention over the cache has no backward pass; call it under torch.no_grad()")
-    batched = q.ndim == 4
-    if q.ndim not in (3, 4):
+    if q.ndim != 4:
       raise ValueError(f"q must be [(batch,) heads, n, head_dim], got {tuple(q.shape)}")
-    if not batched:
-      q = q[None]
     batch, heads, n, head_dim = q.shape
     device = q.device
     if cache.k.device != device:
@@ -83,43 +134,20 @@ class CachedAttentionKernel:
     p = _ffi.SplashCachedParams()
     if counts is not None:
       counts = _index_tensor(counts, "counts", device, (batch,))
-      p.counts = counts.data_ptr()
     if parents is not None:
       if n > MAX_TREE:
         raise NotImplementedError(f"a tree has at most {MAX_TREE} nodes, got {n}")
-      each = isinstance(parents, torch.Tensor) and parents.ndim == 2
+      each = parents.ndim == 2
       parents = _index_tensor(parents, "parents", device, (batch, n) if each else (n,))
-      p.parents, p.parents_stride = parents.data_ptr(), parents.stride(0) if each else 0
-    q = q.contiguous()
-    if q.data_ptr() % 16:
-      q = q.clone()
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if save_residuals else None
-    if out.numel():
-      lib = _ffi.load()
-      _poll_status(device)
-      p.q, p.k_cache, p.v_cache = q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr()
-      if cache.quantized:
-        p.k_exponent, p.v_exponent, p.quantized = cache.k_exponent.data_ptr(), cache.v_exponent.data_ptr(), 1
-      p.page_table, p.lengths, p.out = page_table.data_ptr(), lengths.data_ptr(), out.data_ptr()
-      if lse is not None:
-        p.lse_out = lse.data_ptr()
-      p.status = _status_word(device).data_ptr()
-      p.table_stride, p.table_width = page_table.stride(0), page_table.shape[1]
-      p.batch, p.heads, p.kv_heads, p.n, p.head_dim = batch, heads, kv_heads, n, head_dim
-      p.num_pages, p.page_size, p.dtype = num_pages, page_size, _TORCH_DTYPES[q.dtype]
-      p.window_left = -1 if self.window_left is None else self.window_left
-      p.num_sinks, p.mask_value = self.num_sinks, self.mask_value
-      p.soft_cap = self.attn_logits_soft_cap or 0.0
-      with _on_device(device):
-        nbytes = int(lib.splash_cached_workspace_bytes(ctypes.byref(p)))
-        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
-        rc = lib.splash_cached_fwd(ctypes.byref(p), workspace.data_ptr(), nbytes, _raw_stream(device))
-        _ffi.check(rc, "attention over the cache")
-      _maybe_check(device)
-    if not batched:
-      out, lse = out[0], None if lse is None else lse[0]
-    return (out, (lse,)) if save_residuals else out
+      p.parents = 1  # (any address: the library sizes a call by whether there is one)
+      p.parents_stride = parents.stride(0) if each else 0
+    p.table_stride, p.table_width = page_table.stride(0), page_table.shape[1]
+    p.batch, p.heads, p.kv_heads, p.n, p.head_dim = batch, heads, kv_heads, n, head_dim
+    p.num_pages, p.page_size, p.dtype, p.quantized = num_pages, page_size, _TORCH_DTYPES[q.dtype], cache.quantized
+    p.window_left = -1 if self.window_left is None else self.window_left
+    p.num_sinks, p.mask_value = self.num_sinks, self.mask_value
+    p.soft_cap = self.attn_logits_soft_cap or 0.0
+    return p, q.contiguous(), page_table, lengths, counts, parents
 
 
 def make_splash_cached(*, window_left: int | None = None, num_sinks: int = 0, attn_logits_soft_cap: float | None = None,

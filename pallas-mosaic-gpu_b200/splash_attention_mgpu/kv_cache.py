@@ -23,7 +23,7 @@ import dataclasses
 import torch
 
 from . import _ffi
-from .splash_attention import _TORCH_DTYPES, _on_device, _raw_stream
+from .splash_attention import _TORCH_DTYPES, _launch
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
@@ -43,6 +43,20 @@ def _index_tensor(x, name, device, shape):
   return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
 
 
+def _signature(x):
+  """What a call depends on of an argument besides its address."""
+  if not isinstance(x, torch.Tensor):
+    raise TypeError(f"expected a torch tensor, got {type(x).__name__}")
+  return x.shape, x.stride(), x.dtype, x.device
+
+
+def _remember(known: dict, key, value):
+  if len(known) >= 256:
+    known.clear()
+  known[key] = value
+  return value
+
+
 @dataclasses.dataclass(frozen=True, eq=False)
 class KVCache:
   """Buffers of a paged cache; `make_kv_cache` allocates them.
@@ -55,6 +69,7 @@ class KVCache:
   v: torch.Tensor
   k_exponent: torch.Tensor | None = None
   v_exponent: torch.Tensor | None = None
+  _calls: dict = dataclasses.field(default_factory=dict, init=False, repr=False)
 
   def __post_init__(self):
     for x in (self.k, self.v):
@@ -129,27 +144,44 @@ class KVCache:
     page_table: int32 [B, pages per sequence]; start: int32 [B]
     counts: int32 [B], how many of the n tokens each sequence has (None: all)
     """
-    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
-      raise TypeError("k and v must be torch tensors")
-    if k.ndim == 3:
-      k, v = k[None], v[None]
-    if k.ndim != 4 or k.shape != v.shape or k.shape[1] != self.num_kv_heads or k.shape[3] != self.head_dim:
-      raise ValueError(f"k and v must be [(batch,) {self.num_kv_heads}, n, {self.head_dim}], got {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.dtype != v.dtype or k.device != self.k.device or v.device != self.k.device:
-      raise ValueError(f"k and v differ from the cache: {k.dtype} on {k.device}, {v.dtype} on {v.device}")
-    batch, _, n, _ = k.shape
-    device = self.k.device
-    page_table = _index_tensor(page_table, "page_table", device, (batch, None))
-    start = _index_tensor(start, "start", device, (batch,))
-    p = self._params(page_table, start, batch, n, k.dtype)
+    for x in (k, v, page_table, start):
+      if not isinstance(x, torch.Tensor):
+        raise TypeError("k, v, page_table and start must be torch tensors")
+    # What a call is made of besides its pointers, checked and filled in once per class of calls.
+    key = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, page_table.shape, page_table.stride(),
+           page_table.dtype, page_table.device, start.shape, start.stride(), start.dtype, start.device,
+           None if counts is None else _signature(counts))
+    template = self._calls.get(key)
+    if template is None:
+      if k.ndim == 3:
+        return self.write(k[None], v[None], page_table, start, counts=counts)
+      if k.ndim != 4 or k.shape != v.shape or k.shape[1] != self.num_kv_heads or k.shape[3] != self.head_dim:
+        raise ValueError(f"k and v must be [(batch,) {self.num_kv_heads}, n, {self.head_dim}], got {tuple(k.shape)}, {tuple(v.shape)}")
+      if k.dtype != v.dtype or k.device != self.k.device or v.device != self.k.device:
+        raise ValueError(f"k and v differ from the cache: {k.dtype} on {k.device}, {v.dtype} on {v.device}")
+      batch, _, n, _ = k.shape
+      device = self.k.device
+      as_given = (page_table, start, counts)
+      page_table = _index_tensor(page_table, "page_table", device, (batch, None))
+      start = _index_tensor(start, "start", device, (batch,))
+      if counts is not None:
+        counts = _index_tensor(counts, "counts", device, (batch,))
+      p = self._params(page_table, start, batch, n, k.dtype)
+      in_place = lambda x: x.stride(-1) == 1 and not any(s % 8 for s in x.stride()[:-1])
+      if not (in_place(k) and in_place(v)) or any(x is not y for x, y in zip(as_given, (page_table, start, counts))):
+        k, v = (x if in_place(x) else x.clone(memory_format=torch.contiguous_format) for x in (k, v))
+        return self.write(k, v, page_table, start, counts=counts)
+      p.k_stride, p.v_stride = k.stride()[:3], v.stride()[:3]
+      template = _remember(self._calls, key, bytes(p))
+    if k.data_ptr() % 16 or v.data_ptr() % 16:
+      return self.write(*(x.clone(memory_format=torch.contiguous_format) for x in (k, v)), page_table, start, counts=counts)
+    p = _ffi.SplashCacheParams.from_buffer_copy(template)
+    p.k, p.v, p.page_table, p.lengths = k.data_ptr(), v.data_ptr(), page_table.data_ptr(), start.data_ptr()
     if counts is not None:
-      counts = _index_tensor(counts, "counts", device, (batch,))
       p.counts = counts.data_ptr()
-    k, v = _aligned(k), _aligned(v)
-    p.k, p.v = k.data_ptr(), v.data_ptr()
-    p.k_stride, p.v_stride = k.stride()[:3], v.stride()[:3]
-    with _on_device(device):
-      _ffi.check(_ffi.load().splash_cache_write(ctypes.byref(p), _raw_stream(device)), "cache write")
+    rc = _launch(self.k.device, _ffi.load().splash_cache_write, ctypes.byref(p))
+    if rc:
+      _ffi.check(rc, "cache write")
 
   def read(self, page_table, lengths, max_len: int, *, dtype=None):
     """The first lengths[b] tokens of every sequence, (k, v) [B, kv_heads, max_len, head_dim] with zeros behind them.
@@ -169,16 +201,8 @@ class KVCache:
     shape = (batch, self.num_kv_heads, max_len, self.head_dim)
     k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
     p.k_out, p.v_out = k.data_ptr(), v.data_ptr()
-    with _on_device(device):
-      _ffi.check(_ffi.load().splash_cache_read(ctypes.byref(p), _raw_stream(device)), "cache read")
+    _ffi.check(_launch(device, _ffi.load().splash_cache_read, ctypes.byref(p)), "cache read")
     return k, v
-
-
-def _aligned(x):
-  """x itself where its rows can be read 16 bytes at a time, else a contiguous copy."""
-  if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and not any(s % 8 for s in x.stride()[:-1]):
-    return x
-  return x.clone(memory_format=torch.contiguous_format)
 
 
 def make_kv_cache(num_pages: int, num_kv_heads: int, head_dim: int, *, page_size: int = 64, dtype=torch.bfloat16,

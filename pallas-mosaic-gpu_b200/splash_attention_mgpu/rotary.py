@@ -22,18 +22,16 @@ import numpy as np
 import torch
 
 from . import _ffi
-from .splash_attention import _TORCH_DTYPES, _on_device, _raw_stream
+from .splash_attention import _TORCH_DTYPES, _launch
 
 
 def _batched_strides(x, batched):
   return tuple(x.stride()[:3]) if batched else (0, *x.stride()[:2])
 
 
-def _readable(x):
-  """x itself where the kernel can read it (rows contiguous, 8-byte aligned), else a contiguous copy."""
-  if x.stride(-1) == 1 and x.data_ptr() % 8 == 0 and not any(s % 4 for s in x.stride()[:-1]):
-    return x
-  return x.clone(memory_format=torch.contiguous_format)
+def _in_place(x):
+  """Whether the kernel can read x where it lies: rows contiguous, their starts 8-byte aligned (the base apart)."""
+  return x.stride(-1) == 1 and not any(s % 4 for s in x.stride()[:-1])
 
 
 class RotaryEmbedding:
@@ -120,8 +118,6 @@ class RotaryEmbedding:
     return p
 
   def _run(self, q, k, positions, *, inverse):
-    q = _readable(q)
-    k = None if k is None else _readable(k)
     # What a call is made of besides its pointers, checked and filled in once per class of calls.
     key = (q.shape, q.stride(), q.dtype, q.device, positions.shape, positions.stride(), positions.dtype, positions.device,
            inverse, None if k is None else (k.shape, k.stride(), k.dtype, k.device))
@@ -129,17 +125,23 @@ class RotaryEmbedding:
     if known is None:
       if len(self._calls) >= 256:
         self._calls.clear()
-      known = self._calls[key] = bytes(self._params(q, k, positions, inverse))
-    p = _ffi.SplashRotaryParams.from_buffer_copy(known)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None
+      known = self._calls[key] = (bytes(self._params(q, k, positions, inverse)), _in_place(q), k is None or _in_place(k))
+    template, q_in_place, k_in_place = known
+    if not q_in_place or q.data_ptr() % 8:
+      return self._run(q.clone(memory_format=torch.contiguous_format), k, positions, inverse=inverse)
+    if k is not None and (not k_in_place or k.data_ptr() % 8):
+      return self._run(q, k.clone(memory_format=torch.contiguous_format), positions, inverse=inverse)
+    p = _ffi.SplashRotaryParams.from_buffer_copy(template)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     p.q, p.q_out, p.positions = q.data_ptr(), q_out.data_ptr(), positions.data_ptr()
+    k_out = None
     if k is not None:
-      k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+      k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
       p.k, p.k_out = k.data_ptr(), k_out.data_ptr()
-    if q_out.numel():
-      with _on_device(q.device):
-        _ffi.check(_ffi.load().splash_rotary(ctypes.byref(p), _raw_stream(q.device)), "rotary positions")
+    if p.batch and p.len:
+      rc = _launch(q.device, _ffi.load().splash_rotary, ctypes.byref(p))
+      if rc:
+        _ffi.check(rc, "rotary positions")
     return q_out, k_out
 
 
@@ -154,6 +156,7 @@ class _RotaryFn(torch.autograd.Function):
     return plan._run(q, k, positions, inverse=False)
 
   @staticmethod
+  @torch.autograd.function.once_differentiable
   def backward(ctx, dq, dk):
     (positions,) = ctx.saved_tensors
     dq, dk = ctx.plan._run(dq, dk, positions, inverse=True)

@@ -88,6 +88,26 @@ def _raw_stream(device: torch.device) -> int:
   return torch._C._cuda_getCurrentRawStream(device.index)  # what current_stream(device).cuda_stream wraps
 
 
+def _launch(device: torch.device, entry, *args) -> int:
+  """Calls a library entry point whose last argument is the current stream of `device`, with that device current."""
+  if torch._C._cuda_getDevice() == device.index:
+    return entry(*args, torch._C._cuda_getCurrentRawStream(device.index))
+  with torch.cuda.device(device):
+    return entry(*args, torch._C._cuda_getCurrentRawStream(device.index))
+
+
+def _status_host(device: torch.device) -> int:
+  """Address of the pinned copy of the status word, for kernels that write it themselves when they give up a wait (then
+  no copy has to be queued behind them); 0 where it would have to be made during a stream capture."""
+  key = (device.type, device.index)
+  mirror = _status_mirrors.get(key)
+  if mirror is None:
+    if torch.cuda.is_current_stream_capturing():
+      return 0
+    mirror = _status_mirrors[key] = _StatusMirror(device)
+  return mirror.host.data_ptr()
+
+
 def _raise_device_status(word: torch.Tensor, host) -> None:
   """Clears the device word (later launches would return at entry while it is set) and raises."""
   code, site, block, step = (int(x) for x in host)
