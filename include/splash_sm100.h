@@ -151,6 +151,13 @@ int splash_bwd_dkv(const SplashParams* p, void* stream);
  * splash_attention_mgpu/splash_attention.py:289-290). */
 int splash_bwd_fused(const SplashParams* p, void* stream);
 
+/* splash_bwd_fused with the `heavy` first KV blocks of the column schedule's launch order shared by `parts` CTAs each: for
+ * masks with a few columns that are much longer than the others (keys that stay visible behind a window).  Their dK and dV
+ * are sums of f32 shares in `workspace` (16-byte aligned, splash_bwd_fused_shared_bytes() bytes), added in order.  heavy 0
+ * or parts 1: what splash_bwd_fused does.  No counterpart in the reference. */
+int64_t splash_bwd_fused_shared_bytes(const SplashParams* p, int32_t heavy, int32_t parts);
+int splash_bwd_fused_shared(const SplashParams* p, int32_t heavy, int32_t parts, void* workspace, int64_t bytes, void* stream);
+
 /* Bytes of `dq_acc` scratch splash_bwd_fused needs for these shapes: the f32 accumulator
  * batch * heads * q_len * head_dim * 4, and at head_dim 64 another 32 bytes per q row behind it
  * (lse and delta split into 16-bit parts, operands of the 128-row kernel). */

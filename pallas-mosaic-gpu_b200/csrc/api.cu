@@ -208,11 +208,10 @@ extern "C" int64_t splash_bwd_fused_workspace_bytes(const SplashParams* p) {
   return dq_acc_bytes(p) + fold_operand_bytes(*p);
 }
 
-extern "C" int splash_bwd_fused(const SplashParams* p, void* stream) {
+static int bwd_fused(const SplashParams* p, int heavy, int parts, void* part_out, cudaStream_t st) {
   if (int rc = check_bwd_fused(p)) return rc;
   if (!p->dq || !p->dk || !p->dv || !p->dq_acc) return fail(SPLASH_INVALID_ARGUMENT, "dq, dk, dv and dq_acc must be non-null");
 
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (int rc = launch_seg_ranges(*p, st)) return rc;
   if (p->out) {
     // One pass streams O and dO for delta, clears the accumulator on the way and (head_dim 64) writes
@@ -228,9 +227,29 @@ extern "C" int splash_bwd_fused(const SplashParams* p, void* stream) {
         return rc;
     }
   }
-  if (int rc = launch_bwd_wide(*p, st)) return rc;
+  if (int rc = launch_bwd_wide(*p, heavy, parts, part_out, st)) return rc;
   return launch_dq_cast(p->dq_acc, p->dq, static_cast<long long>(p->batch) * p->heads, p->head_dim, p->q_len,
                                   p->dtype, st);
+}
+
+extern "C" int splash_bwd_fused(const SplashParams* p, void* stream) {
+  return bwd_fused(p, 0, 1, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int64_t splash_bwd_fused_shared_bytes(const SplashParams* p, int32_t heavy, int32_t parts) {
+  if (!p || heavy <= 0 || parts <= 1) return 0;
+  return static_cast<int64_t>(p->batch) * p->kv_heads * heavy * parts * 2 * 128 * p->head_dim * 4;
+}
+
+extern "C" int splash_bwd_fused_shared(const SplashParams* p, int32_t heavy, int32_t parts, void* workspace, int64_t bytes,
+                                       void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (heavy <= 0 || parts <= 1) return bwd_fused(p, 0, 1, nullptr, st);
+  if (int rc = check_bwd_fused(p)) return rc;
+  if (heavy > p->kv_len / 128 || parts > 1024) return fail(SPLASH_INVALID_ARGUMENT, "more shared columns than KV blocks, or over 1024 shares");
+  if (!workspace || bytes < splash_bwd_fused_shared_bytes(p, heavy, parts) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail(SPLASH_INVALID_ARGUMENT, "the workspace of a shared backward is null, too small or not 16-byte aligned");
+  return bwd_fused(p, heavy, parts, workspace, st);
 }
 
 // ---------------------------------------------------------------------------

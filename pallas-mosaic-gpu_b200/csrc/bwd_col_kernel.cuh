@@ -58,6 +58,10 @@ struct BwdArgs {
   int32_t has_dense, has_seg;
   int32_t head_group;  // heads whose blocks are interleaved in the launch order
   float mask_value, soft_cap;
+  // Fused backward with shared columns: the `heavy` first KV blocks of the launch order have `parts` CTAs each, which leave
+  // dK and dV here: [batch * kv_heads, heavy, parts, 2, 128, head_dim].
+  int32_t heavy, parts;
+  float* part_out;
 };
 
 enum BwdSite : int {

@@ -43,6 +43,9 @@ inline void fill_bwd_args(BwdArgs& a, const SplashParams& p, bool dense, bool se
   a.head_group = 4;
   a.mask_value = p.mask_value;
   a.soft_cap = p.soft_cap;
+  a.heavy = 0;
+  a.parts = 1;
+  a.part_out = nullptr;
 }
 
 template <int D, int DV, bool BF16>

@@ -215,6 +215,15 @@ struct WideSteps {
     n = steps_of(0);
     if (count > 0) seek(0);
   }
+  // The walk from step `first` on.
+  __device__ __forceinline__ void skip_to(int first) {
+    if (!skipping) {
+      e = first;
+      if (e < count) seek(0);
+    } else {
+      while (e < first) next();
+    }
+  }
   __device__ __forceinline__ bool valid() const { return e < count; }
   __device__ __forceinline__ void next() {
     if (++e < count) seek(i + 1);
@@ -252,7 +261,10 @@ static_assert(sizeof(WideBarriers) <= WideLayout<128>::kBarBytes, "barrier block
 // waits: 2 KB per block pair do not need a shared-memory ring, for which there is no room.
 // (Array mask, batch 2, 16/4 heads, seq 4096, D = 128: backward call 447 us in the 64-row kernel
 // with a ring, 357 us here.)
-template <int HEAD_DIM, bool PLAIN, bool BF16>
+// SHARED: the columns of a few keys that nearly every query sees (sinks beside a window) would each be the work of one
+// CTA, many times as long as the others'; they are cut into a.parts shares of their steps, whose dK and dV bwd_parts_kernel
+// adds up (window 1024, 4 sinks, 8/2 heads, seq 8192, D = 128: 540 -> 92 us).  Compiled apart.
+template <int HEAD_DIM, bool PLAIN, bool BF16, bool SHARED>
 __global__ void __launch_bounds__(WideLayout<HEAD_DIM>::kThreads, 1)
 splash_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -296,7 +308,20 @@ splash_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   // ---- which KV block ----------------------------------------------------------
   const int group = a.heads / a.kv_heads;
   int hb, order_idx;
-  decode_work_item(blockIdx.x, a.kv_blocks, a.kv_heads * a.batch, a.head_group, hb, order_idx);
+  int part = 0, parts = 1;
+  if constexpr (SHARED) {
+    int item;
+    decode_work_item(blockIdx.x, a.kv_blocks + a.heavy * (a.parts - 1), a.kv_heads * a.batch, a.head_group, hb, item);
+    if (item < a.heavy * a.parts) {
+      parts = a.parts;
+      order_idx = item / parts;
+      part = item - order_idx * parts;
+    } else {
+      order_idx = item - a.heavy * (a.parts - 1);
+    }
+  } else {
+    decode_work_item(blockIdx.x, a.kv_blocks, a.kv_heads * a.batch, a.head_group, hb, order_idx);
+  }
   const int kvh = hb % a.kv_heads;
   const int b = hb / a.kv_heads;
   const int head0 = kvh * group;
@@ -364,8 +389,15 @@ splash_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   tc_fence_after();
   const uint32_t tmem = lds32(tmem_slot_u32);
   const WaitCtx ctx{abort_u32};
-  const int total = skipping ? static_cast<int>(lds32(neff_u32)) : scheduled;
-  it.start(steps_u32, skipping, total);
+  int total = skipping ? static_cast<int>(lds32(neff_u32)) : scheduled;
+  if constexpr (SHARED) {
+    const int share = (total + parts - 1) / parts, first = part * share;
+    total = max(0, min(share, total - first));
+    it.start(steps_u32, skipping, total > 0 ? first + total : 0);
+    it.skip_to(first);
+  } else {
+    it.start(steps_u32, skipping, total);
+  }
   if (lds32(dead_u32)) {
     if (warp == kProducerWarp0 + 1) {
       __syncwarp();
@@ -607,7 +639,16 @@ splash_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const uint32_t tmem_row = tmem + (static_cast<uint32_t>(wq * 32) << 16);
     const int col0 = w * 64;                 // first q column this thread handles
 
-    if (total == 0) {
+    // This thread's row of a share's dK (warpgroup 0) or dV (1).
+    float4* part_row = nullptr;
+    if constexpr (SHARED) {
+      if (parts > 1)
+        part_row = reinterpret_cast<float4*>(
+            a.part_out + ((((static_cast<size_t>(hb) * a.heavy + order_idx) * parts + part) * 2 + w) * kRows + row) * D);
+    }
+    if (SHARED && parts > 1 && total == 0) {
+      for (int c = 0; c < D / 4; ++c) part_row[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else if (total == 0) {
       // No q block sees this KV block: its gradients are zero.
       uint8_t* base = static_cast<uint8_t*>(w == 0 ? a.dk : a.dv);
       uint4* dst = reinterpret_cast<uint4*>(base + static_cast<size_t>(kv_row0 + row) * (D * 2));
@@ -825,7 +866,20 @@ splash_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
       // ---- epilogue: dK by warpgroup 0, dV by warpgroup 1 ---------------------------
       if (alive) alive = warp_wait(SPLASH_WBAR(acc_done, 0), 0, ctx, kWSiteEwDone, total);
-      if (alive) {
+      if (SHARED && alive && parts > 1) {
+        tc_fence_after();
+        const uint32_t acc_tmem = tmem_row + (w == 0 ? L::kColDk : L::kColDv);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(acc_tmem + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            part_row[c * 8 + g] = make_float4(__uint_as_float(o[g * 4]), __uint_as_float(o[g * 4 + 1]),
+                                              __uint_as_float(o[g * 4 + 2]), __uint_as_float(o[g * 4 + 3]));
+        }
+      } else if (alive) {
         tc_fence_after();
         const uint32_t stage = w == 0 ? k_u32 : v_u32;  // K / V tiles are dead once every MMA has finished
         const uint32_t acc_tmem = tmem_row + (w == 0 ? L::kColDk : L::kColDv);

@@ -28,8 +28,9 @@ size_t bwd_row_smem(const SplashParams& p);
 // Puts the parts of a split forward together: out and, when asked for, lse.
 int launch_fwd_combine(const SplashParams& p, int splits, const void* workspace, cudaStream_t stream);
 
-// Fused backward, 128 q rows per step (head_dim == head_dim_v, 64 or 128).
-int launch_bwd_wide(const SplashParams& p, cudaStream_t stream);
+// Fused backward, 128 q rows per step (head_dim == head_dim_v, 64 or 128).  heavy > 0: that many of the longest columns
+// are shared by `parts` CTAs each, with their f32 dK and dV in `part_out`.
+int launch_bwd_wide(const SplashParams& p, int heavy, int parts, void* part_out, cudaStream_t stream);
 
 // delta = rowsum(dO * O); dq = cast(dq_acc), transposed where the accumulator is.
 // When `zero` is non-null the same pass also clears zero_floats_per_row floats per row of it, and when

@@ -39,6 +39,8 @@ EXPORTED_SYMBOLS = (
     "splash_bwd_fused",
     "splash_bwd_fused_workspace_bytes",
     "splash_bwd_fused_static",
+    "splash_bwd_fused_shared",
+    "splash_bwd_fused_shared_bytes",
     "splash_seg_ranges_bytes",
     "splash_read_status",
     "splash_status_copy",
@@ -170,6 +172,10 @@ def load():
                                        c_int32, c_int32, c_int32, c_int32,
                                        c_void_p, c_void_p]
   lib.splash_selftest_umma.restype = c_int
+  lib.splash_bwd_fused_shared.argtypes = [POINTER(SplashParams), c_int32, c_int32, c_void_p, c_int64, c_void_p]
+  lib.splash_bwd_fused_shared.restype = c_int
+  lib.splash_bwd_fused_shared_bytes.argtypes = [POINTER(SplashParams), c_int32, c_int32]
+  lib.splash_bwd_fused_shared_bytes.restype = c_int64
   for name, params in (("splash_rotary", SplashRotaryParams), ("splash_cache_write", SplashCacheParams),
                        ("splash_cache_read", SplashCacheParams)):
     fn = getattr(lib, name)

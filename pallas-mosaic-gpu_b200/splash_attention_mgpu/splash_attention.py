@@ -419,6 +419,21 @@ class SplashAttentionKernel:
     bs = self.requested_block_sizes
     return bs.num_stages is not None and bs.block_q is not None and bs.block_kv is not None
 
+  @functools.cached_property
+  def _shared_columns(self) -> tuple[int, int]:
+    """(heavy, parts): how many of the longest columns of the backward are shared by several CTAs, and by how many.
+
+    Sinks behind a window make columns that nearly all q blocks visit beside short ones; a share is about as long as the
+    longest of the others.  By the mask alone, so that a unit's bits do not depend on the call."""
+    masks = self.mask.masks if isinstance(self.mask, mask_lib.MultiHeadMask) else (self.mask,)
+    sinks = max(getattr(m, "num_sinks", 0) for m in masks)
+    steps = np.sort(self.info.dkv_num_steps, axis=-1)[:, ::-1].max(axis=0)  # longest first, as they are launched
+    heavy = -(-sinks // cfg.TILE_ROWS)
+    if not 0 < heavy < len(steps):
+      return 0, 1
+    parts = min(256, int(steps[0]) // max(1, int(steps[heavy])))
+    return (heavy, parts) if parts > 1 else (0, 1)
+
   # -- device schedules ------------------------------------------------------
   def _fwd_schedule(self, bs: BlockSizes, device) -> _DeviceSchedule:
     key = ("fwd", bs.block_q, bs.block_kv, device.type, device.index)
@@ -706,8 +721,14 @@ def _backward(kernel: SplashAttentionKernel, bs: BlockSizes, q, k, v,
       acc = torch.empty(max(int(nbytes), 4) // 4, dtype=torch.float32,
                         device=q.device)
       p.dq_acc = acc.data_ptr()
-      _ffi.check(lib.splash_bwd_fused(ctypes.byref(p), stream),
-                 "splash attention fused backward")
+      heavy, parts = kernel._shared_columns
+      if parts > 1:
+        nbytes = int(lib.splash_bwd_fused_shared_bytes(ctypes.byref(p), heavy, parts))
+        shares = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        rc = lib.splash_bwd_fused_shared(ctypes.byref(p), heavy, parts, shares.data_ptr(), nbytes, stream)
+      else:
+        rc = lib.splash_bwd_fused(ctypes.byref(p), stream)
+      _ffi.check(rc, "splash attention fused backward")
     else:
       def pick(requested, tmem_fn, smem_fn, name):
         sb = requested or cfg.largest_fitting_sub_block(tmem_fn, smem_fn) or 64
