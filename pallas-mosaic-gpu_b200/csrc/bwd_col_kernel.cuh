@@ -484,12 +484,8 @@ splash_bwd_col_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           } else {
             uint32_t vis = 0xffffffffu;  // bit i: column i of this chunk is visible
             if (partial && !has_dense) {
-              const int d0 = kv_pos - (q0 + c * 32);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const int d = d0 - i;
-                if (d < band_lo || d > band_hi) vis &= ~(1u << i);
-              }
+              const int d0 = kv_pos - (q0 + c * 32);  // column i is visible iff band_lo <= d0 - i <= band_hi
+              vis &= bit_run(d0 - band_hi, d0 - band_lo + 1);
             }
             if (partial && has_dense) {
               // Transposed block, one bit per element: 16 bytes per kv row, bit = q column.

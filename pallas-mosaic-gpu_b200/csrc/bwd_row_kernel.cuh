@@ -315,13 +315,9 @@ splash_bwd_row_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           tmem_wait_ld();
           uint32_t vis = row_on ? 0xffffffffu : 0u;
           if (partial && !a.has_dense) {
-            const int d0 = kv0 + c * 32 - q_pos;
-            const int sink_cols = sinks - (kv0 + c * 32);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int d = d0 + i;
-              if ((d < band_lo && i >= sink_cols) || d > band_hi) vis &= ~(1u << i);
-            }
+            // Two runs of columns: the window, and the sinks as far as its right edge.
+            const int first = kv0 + c * 32, hi = band_hi + q_pos - first + 1;
+            vis &= bit_run(band_lo + q_pos - first, hi) | bit_run(0, min(sinks - first, hi));
           }
           if (partial && a.has_dense) {
             // One bit per element: 16 bytes per q row, bit = kv column inside the block.

@@ -266,13 +266,6 @@ __device__ __forceinline__ int lds_s8(uint32_t addr) {
   return v;
 }
 
-// Bits [from, to) of a word.
-__device__ __forceinline__ uint32_t bit_run(int from, int to) {
-  from = max(from, 0);
-  to = min(to, 32);
-  return from < to ? (0xffffffffu >> (32 - to)) & (0xffffffffu << from) : 0u;
-}
-
 #define SPLASH_KBAR(field, idx) \
   (bars_u32 + static_cast<uint32_t>(offsetof(CachedBarriers, field)) + 8u * static_cast<uint32_t>(idx))
 #define SPLASH_KWORD(field) (bars_u32 + static_cast<uint32_t>(offsetof(CachedBarriers, field)))

@@ -578,34 +578,24 @@ splash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           if (!warp_wait(SPLASH_BAR(aux_full, slot), phase, ctx, kSiteSmxAux, s)) { alive = false; break; }
         }
         const bool partial = kind_now == SPLASH_BLOCK_PARTIAL;
-        if (partial && !has_dense) {
-          const int d0 = j_now * BKV - q_pos;
-          const int sink_cols = sinks - j_now * BKV;  // columns of this block that are sinks
-          if (sink_cols <= 0) {
-#pragma unroll
-            for (int i = 0; i < BKV; ++i) {
-              const int d = d0 + i;
-              if (d < band_lo || d > band_hi) sv[i] = -INFINITY;
-            }
-          } else {
-            // Apart from the blocks without sinks, whose two comparisons per element it would make three.
-#pragma unroll
-            for (int i = 0; i < BKV; ++i) {
-              const int d = d0 + i;
-              if ((d < band_lo && i >= sink_cols) || d > band_hi) sv[i] = -INFINITY;
-            }
-          }
-        }
-        if (partial && has_dense) {
-          // One bit per element, BKV / 8 bytes per q row, rows of the tile(s) back to back.
-          const uint32_t mrow = mask_u32 + slot * L::kMaskStage + (t * kTile + row) * (BKV / 8);
+        if (partial) {
+          // One bit per element of the row: two runs (the window, and the sinks as far as its right edge), or a row of
+          // BKV / 8 bytes of the streamed block, rows of the tile(s) back to back.
           uint32_t bits[BKV / 32];
-          if constexpr (BKV == 128) {
-            const uint4 w = lds128(mrow);
-            bits[0] = w.x; bits[1] = w.y; bits[2] = w.z; bits[3] = w.w;
+          if (!has_dense) {
+            const int lo = band_lo + q_pos - j_now * BKV, hi = band_hi + q_pos - j_now * BKV + 1;
+            const int sink_cols = min(sinks - j_now * BKV, hi);
+#pragma unroll
+            for (int c = 0; c < BKV / 32; ++c) bits[c] = bit_run(lo - c * 32, hi - c * 32) | bit_run(0, sink_cols - c * 32);
           } else {
-            bits[0] = lds32(mrow);
-            bits[1] = lds32(mrow + 4);
+            const uint32_t mrow = mask_u32 + slot * L::kMaskStage + (t * kTile + row) * (BKV / 8);
+            if constexpr (BKV == 128) {
+              const uint4 w = lds128(mrow);
+              bits[0] = w.x; bits[1] = w.y; bits[2] = w.z; bits[3] = w.w;
+            } else {
+              bits[0] = lds32(mrow);
+              bits[1] = lds32(mrow + 4);
+            }
           }
 #pragma unroll
           for (int i = 0; i < BKV; ++i)

@@ -545,6 +545,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
+// Bits [from, to) of a word, as far as there are any.
+__device__ __forceinline__ uint32_t bit_run(int from, int to) {
+  from = max(from, 0);
+  to = min(to, 32);
+  return from < to ? (0xffffffffu >> (32 - to)) & (0xffffffffu << from) : 0u;
+}
+
 // Byte offset of 16-byte chunk `chunk` (0..7) of row `row` inside a tile of
 // 128-byte rows laid out with the 128-byte swizzle, tile base 1024-byte aligned.
 __device__ __forceinline__ uint32_t swz128(uint32_t row, uint32_t chunk) {
