@@ -784,11 +784,11 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             sv[j] = x.x; sv[j + 1] = x.y; sv[j + 2] = y.x; sv[j + 3] = y.y;
           }
         }
-        if (a.soft_cap > 0.f) {
+        if (__builtin_expect(a.soft_cap > 0.f, 0)) {
 #pragma unroll
           for (int j = 0; j < L::kKeys; ++j) sv[j] = tanh_approx(sv[j] * q_mul);
         }
-        if (!plain) {
+        if (__builtin_expect(!plain, 0)) {
 #pragma unroll
           for (int c = 0; c < L::kKeys / 32; ++c) {
             const int at = col0 + c * 32, kb = key0 + at;
@@ -907,7 +907,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
         l_run += (sum_a.x + sum_a.y) + (sum_b.x + sum_b.y);
         // The scores of this tile came after P.V of the warpgroup's previous one: O stands still.
-        if (i >= 2 && __any_sync(0xffffffffu, moved)) {
+        if (__builtin_expect(i >= 2 && __any_sync(0xffffffffu, moved), 0)) {
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];

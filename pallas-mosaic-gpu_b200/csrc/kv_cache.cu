@@ -48,88 +48,119 @@ __device__ __forceinline__ float2 wide2(uint32_t w) {
   else return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// LPR lanes per row of head_dim = 8 * LPR numbers; blockIdx.y: 0 keys, 1 values.
-template <int LPR, bool BF16, bool QUANT>
+// A block has ROWS * 256 / LPR consecutive tokens of one (sequence, head), LPR lanes per row of head_dim = 8 * LPR numbers and
+// ROWS rows of a thread in flight together; blockIdx.y: 0 keys, 1 values.
+struct CacheBlock {
+  int b, h, t0;  // t0: first token of this thread
+};
+template <int LPR, int ROWS>
+__device__ __forceinline__ CacheBlock cache_block(const SplashCacheParams& p) {
+  constexpr int kTokens = ROWS * kCacheThreads / LPR;
+  const int chunks = (p.len + kTokens - 1) / kTokens;
+  const int bh = blockIdx.x / chunks, chunk = blockIdx.x - bh * chunks;
+  const int b = bh / p.kv_heads;
+  return {b, bh - b * p.kv_heads, chunk * kTokens + static_cast<int>(threadIdx.x) / LPR};
+}
+
+template <int LPR, int ROWS, bool BF16, bool QUANT>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const SplashCacheParams p) {
-  const long long id = static_cast<long long>(blockIdx.x) * (kCacheThreads / LPR) + threadIdx.x / LPR;
+  constexpr int kStep = kCacheThreads / LPR;
+  const CacheBlock at = cache_block<LPR, ROWS>(p);
   const int sub = threadIdx.x % LPR;
   const bool is_v = blockIdx.y != 0;
-  const long long per_head = p.len;
-  const long long bh = id / per_head;
-  const int t = static_cast<int>(id - bh * per_head);
-  const int b = static_cast<int>(bh / p.kv_heads);
-  const int h = static_cast<int>(bh - static_cast<long long>(b) * p.kv_heads);
-  bool live = b < p.batch;
-  long long row = -1;
-  uint4 x = make_uint4(0, 0, 0, 0);
-  if (live && (!p.counts || t < p.counts[b])) row = cache_row(p, b, static_cast<long long>(p.lengths[b]) + t, h);
-  live = live && row >= 0;
-  if (live) {
-    const int64_t* st = is_v ? p.v_stride : p.k_stride;
-    const uint16_t* src = static_cast<const uint16_t*>(is_v ? p.v : p.k) + b * st[0] + h * st[1] + t * st[2];
-    x = *reinterpret_cast<const uint4*>(src + sub * 8);
+  const int count = p.counts ? min(p.counts[at.b], p.len) : p.len;
+  if (at.t0 - static_cast<int>(threadIdx.x) / LPR >= count) return;  // the whole block
+  const long long start = p.lengths[at.b];
+  const int64_t* st = is_v ? p.v_stride : p.k_stride;
+  const uint16_t* src = static_cast<const uint16_t*>(is_v ? p.v : p.k) + at.b * st[0] + at.h * st[1] + sub * 8;
+  long long row[ROWS];
+  uint4 x[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int t = at.t0 + i * kStep;
+    x[i] = make_uint4(0, 0, 0, 0);
+    row[i] = -1;
+    if (t < count) {
+      x[i] = *reinterpret_cast<const uint4*>(src + t * st[2]);
+      row[i] = cache_row(p, at.b, start + t, at.h);
+    }
   }
-  if constexpr (!QUANT) {
-    if (live) *reinterpret_cast<uint4*>(static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + row * (16 * LPR) + sub * 16) = x;
-  } else {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
-    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+  for (int i = 0; i < ROWS; ++i) {
+    if constexpr (!QUANT) {
+      if (row[i] >= 0) *reinterpret_cast<uint4*>(static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + row[i] * (16 * LPR) + sub * 16) = x[i];
+    } else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&x[i]);
+      uint32_t top = 0;
 #pragma unroll
-    for (int d = LPR / 2; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (!live) return;  // (after the shuffles, in which every lane of the warp takes part)
-    const bool bad = top >= (BF16 ? 0x7f80u : 0x7c00u);
-    int e = kMinExponent;
-    if (top != 0) {
-      const uint32_t bits = __float_as_uint(wide2<BF16>(top).x);
-      // |x| = 1.f * 2^E: 448 = 1.75 * 2^8.
-      e = static_cast<int>(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7);
-      e = min(max(e, kMinExponent), kMaxExponent);
+      for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+#pragma unroll
+      for (int d = LPR / 2; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+      if (row[i] < 0) continue;  // (after the shuffles, in which every lane of the warp takes part)
+      const bool bad = top >= (BF16 ? 0x7f80u : 0x7c00u);
+      int e = kMinExponent;
+      if (top != 0) {
+        const uint32_t bits = __float_as_uint(wide2<BF16>(top).x);
+        // |x| = 1.f * 2^E: 448 = 1.75 * 2^8.
+        e = static_cast<int>(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7);
+        e = min(max(e, kMinExponent), kMaxExponent);
+      }
+      const float scale = pow2(-e);
+      uint32_t code[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = wide2<BF16>(w[k]);
+        code[k] = bad ? 0x7f7fu : to_e4m3x2(f.x * scale, f.y * scale);
+      }
+      uint8_t* dst = static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + row[i] * (8 * LPR) + sub * 8;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(code[0] | (code[1] << 16), code[2] | (code[3] << 16));
+      if (sub == 0) (is_v ? p.v_exponent : p.k_exponent)[row[i]] = static_cast<int8_t>(bad ? kBadExponent : e);
     }
-    const float scale = pow2(-e);
-    uint32_t code[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = wide2<BF16>(w[i]);
-      code[i] = bad ? 0x7f7fu : to_e4m3x2(f.x * scale, f.y * scale);
-    }
-    uint8_t* dst = static_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + row * (8 * LPR) + sub * 8;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(code[0] | (code[1] << 16), code[2] | (code[3] << 16));
-    if (sub == 0) (is_v ? p.v_exponent : p.k_exponent)[row] = static_cast<int8_t>(bad ? kBadExponent : e);
   }
 }
 
-template <int LPR, bool BF16, bool QUANT>
+template <int LPR, int ROWS, bool BF16, bool QUANT>
 __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const SplashCacheParams p) {
-  const long long id = static_cast<long long>(blockIdx.x) * (kCacheThreads / LPR) + threadIdx.x / LPR;
+  constexpr int kStep = kCacheThreads / LPR;
+  const CacheBlock at = cache_block<LPR, ROWS>(p);
   const int sub = threadIdx.x % LPR;
   const bool is_v = blockIdx.y != 0;
-  const long long bh = id / p.len;
-  const int t = static_cast<int>(id - bh * p.len);
-  const int b = static_cast<int>(bh / p.kv_heads);
-  const int h = static_cast<int>(bh - static_cast<long long>(b) * p.kv_heads);
-  if (b >= p.batch) return;
-  const long long row = t < p.lengths[b] ? cache_row(p, b, t, h) : -1;
-  uint4 y = make_uint4(0, 0, 0, 0);
-  if (row >= 0) {
-    const uint8_t* src = static_cast<const uint8_t*>(is_v ? p.v_cache : p.k_cache);
+  const int count = min(p.lengths[at.b], p.len);
+  const uint8_t* src = static_cast<const uint8_t*>(is_v ? p.v_cache : p.k_cache);
+  const int8_t* exponents = is_v ? p.v_exponent : p.k_exponent;
+  uint4 y[ROWS];  // 8 bit: the codes in the first half, their exponent in z
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int t = at.t0 + i * kStep;
+    const long long row = t < count ? cache_row(p, at.b, t, at.h) : -1;
+    y[i] = make_uint4(0, 0, 0, 0);
+    if (row < 0) continue;
     if constexpr (!QUANT) {
-      y = *reinterpret_cast<const uint4*>(src + row * (16 * LPR) + sub * 16);
+      y[i] = *reinterpret_cast<const uint4*>(src + row * (16 * LPR) + sub * 16);
     } else {
       const uint2 c = *reinterpret_cast<const uint2*>(src + row * (8 * LPR) + sub * 8);
-      const int e = (is_v ? p.v_exponent : p.k_exponent)[row];
-      const float scale = e == kBadExponent ? __uint_as_float(0x7fc00000u) : pow2(e);
-      uint32_t* w = reinterpret_cast<uint32_t*>(&y);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = from_e4m3x2(((i < 2 ? c.x : c.y) >> (16 * (i & 1))) & 0xffffu);
-        w[i] = pack2<BF16>(f.x * scale, f.y * scale);
-      }
+      y[i] = make_uint4(c.x, c.y, static_cast<uint32_t>(static_cast<int32_t>(exponents[row])), 0);
     }
   }
-  uint16_t* dst = static_cast<uint16_t*>(is_v ? p.v_out : p.k_out) + id * (8 * LPR) + sub * 8;
-  *reinterpret_cast<uint4*>(dst) = y;
+  uint16_t* dst = static_cast<uint16_t*>(is_v ? p.v_out : p.k_out) +
+                  (static_cast<long long>(at.b) * p.kv_heads + at.h) * p.len * (8 * LPR) + sub * 8;
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int t = at.t0 + i * kStep;
+    if (t >= p.len) continue;
+    if constexpr (QUANT) {
+      const int e = static_cast<int32_t>(y[i].z);
+      const float scale = e == kBadExponent ? __uint_as_float(0x7fc00000u) : pow2(e);
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = from_e4m3x2(((k < 2 ? y[i].x : y[i].y) >> (16 * (k & 1))) & 0xffffu);
+        w[k] = pack2<BF16>(f.x * scale, f.y * scale);
+      }
+      y[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    *reinterpret_cast<uint4*>(dst + static_cast<long long>(t) * (8 * LPR)) = y[i];
+  }
 }
 
 static int check_cache(const SplashCacheParams* p) {
@@ -147,25 +178,42 @@ static int check_cache(const SplashCacheParams* p) {
   return SPLASH_OK;
 }
 
-static int cache_grid(const SplashCacheParams& p, dim3& grid) {
-  const long long rows = static_cast<long long>(p.batch) * p.kv_heads * p.len;
-  const int per_block = kCacheThreads / (p.head_dim / 8);
-  const long long blocks = (rows + per_block - 1) / per_block;
+// Eight rows of a thread in flight where there are enough tokens (4 prompts of up to 8192 tokens, 8 bit: DRAM latency
+// bounds one row a thread, 46 us), one where a call is short.
+constexpr int kCacheRows = 8;
+
+template <int LPR, int ROWS>
+static int cache_blocks(const SplashCacheParams& p) {
+  constexpr int kTokens = ROWS * kCacheThreads / LPR;
+  return (p.len + kTokens - 1) / kTokens;
+}
+
+template <int LPR, int ROWS, bool WRITE>
+static int launch_cache(const SplashCacheParams& p, cudaStream_t stream) {
+  const long long blocks = static_cast<long long>(cache_blocks<LPR, ROWS>(p)) * p.batch * p.kv_heads;
   if (blocks >= (1ll << 31)) return fail(SPLASH_INVALID_ARGUMENT, "too many tokens for one call");
-  grid = dim3(static_cast<unsigned>(blocks), 2);
+  const bool bf16 = p.dtype == SPLASH_DTYPE_BF16;
+  auto kernel = WRITE ? (p.quantized ? (bf16 ? cache_write_kernel<LPR, ROWS, true, true> : cache_write_kernel<LPR, ROWS, false, true>)
+                                     : (bf16 ? cache_write_kernel<LPR, ROWS, true, false> : cache_write_kernel<LPR, ROWS, false, false>))
+                      : (p.quantized ? (bf16 ? cache_read_kernel<LPR, ROWS, true, true> : cache_read_kernel<LPR, ROWS, false, true>)
+                                     : (bf16 ? cache_read_kernel<LPR, ROWS, true, false> : cache_read_kernel<LPR, ROWS, false, false>));
+  kernel<<<dim3(static_cast<unsigned>(blocks), 2), kCacheThreads, 0, stream>>>(p);
+  SPLASH_CUDA_CHECK(cudaGetLastError());
   return SPLASH_OK;
 }
 
-#define SPLASH_CACHE_LAUNCH(KERNEL)                                                                               \
-  const bool bf16 = p->dtype == SPLASH_DTYPE_BF16;                                                                \
-  auto kernel = p->head_dim == 64                                                                                 \
-                    ? (p->quantized ? (bf16 ? KERNEL<8, true, true> : KERNEL<8, false, true>)                     \
-                                    : (bf16 ? KERNEL<8, true, false> : KERNEL<8, false, false>))                  \
-                    : (p->quantized ? (bf16 ? KERNEL<16, true, true> : KERNEL<16, false, true>)                   \
-                                    : (bf16 ? KERNEL<16, true, false> : KERNEL<16, false, false>));               \
-  kernel<<<grid, kCacheThreads, 0, static_cast<cudaStream_t>(stream)>>>(*p);                                      \
-  SPLASH_CUDA_CHECK(cudaGetLastError());                                                                          \
-  return SPLASH_OK
+template <int LPR, bool WRITE>
+static int run_cache_dim(const SplashCacheParams& p, cudaStream_t st) {
+  const bool many = p.len > kCacheThreads / LPR &&
+                    static_cast<long long>(cache_blocks<LPR, kCacheRows>(p)) * p.batch * p.kv_heads >= sm_count();
+  return many ? launch_cache<LPR, kCacheRows, WRITE>(p, st) : launch_cache<LPR, 1, WRITE>(p, st);
+}
+
+template <bool WRITE>
+static int run_cache(const SplashCacheParams& p, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return p.head_dim == 64 ? run_cache_dim<8, WRITE>(p, st) : run_cache_dim<16, WRITE>(p, st);
+}
 
 }  // namespace splash
 
@@ -179,9 +227,7 @@ extern "C" int splash_cache_write(const SplashCacheParams* p, void* stream) {
     if (p->k_stride[i] % 8 || p->v_stride[i] % 8) return fail(SPLASH_INVALID_ARGUMENT, "rows of k and v must be 16-byte aligned");
   if ((reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v)) & 15)
     return fail(SPLASH_INVALID_ARGUMENT, "rows of k and v must be 16-byte aligned");
-  dim3 grid;
-  if (int rc = cache_grid(*p, grid)) return rc;
-  SPLASH_CACHE_LAUNCH(cache_write_kernel);
+  return run_cache<true>(*p, stream);
 }
 
 extern "C" int splash_cache_read(const SplashCacheParams* p, void* stream) {
@@ -190,7 +236,5 @@ extern "C" int splash_cache_read(const SplashCacheParams* p, void* stream) {
   if (!p->k_out || !p->v_out) return fail(SPLASH_INVALID_ARGUMENT, "k_out and v_out must be non-null");
   if ((reinterpret_cast<uintptr_t>(p->k_out) | reinterpret_cast<uintptr_t>(p->v_out)) & 15)
     return fail(SPLASH_INVALID_ARGUMENT, "the results must be 16-byte aligned");
-  dim3 grid;
-  if (int rc = cache_grid(*p, grid)) return rc;
-  SPLASH_CACHE_LAUNCH(cache_read_kernel);
+  return run_cache<false>(*p, stream);
 }
