@@ -12,8 +12,11 @@
 //   * Rows are few, so the 128 rows of an MMA are used otherwise: Q is laid into shared memory 128 / R times, and each
 //     copy's warps take the exponentials of their own part of the tile's keys (P is zero elsewhere); the copies' results
 //     are added like partial ones.  A softmax warp of a one-token call thus works on 32 of 128 keys.
-//   * Two warpgroups take the tiles in turn, each with maxima, sums and O columns of its own, so that one's softmax runs
-//     under the other's products.
+//   * Two softmax warpgroups take the tiles in turn.  They hand the (lagging) maxima to one another through shared memory,
+//     a tile's right after its comparison and long before its exponentials, and keep partial sums; P has columns of its
+//     own, so the scores of tile t + 2 are computed as soon as those of tile t are in registers: one warp issues the score
+//     products, another P V, and neither waits for what the other waits for.  Tensor memory: S0 S1 P0 P1 O = 128 + 128 + 64 +
+//     64 + head_dim columns.
 //
 // 8-bit caches are not widened on the way: e4m3 keys and values are operands of the MMA as they lie in the cache, and
 // the 16-bit Q and the probabilities are split into e4m3 terms instead, which are few:
@@ -146,7 +149,7 @@ struct CachedCursor {
 
 enum CachedSite : int {
   kCSiteLoadEmpty = 301, kCSiteLoadQ, kCSiteMmaQ, kCSiteMmaFull, kCSiteMmaP, kCSiteMmaO, kCSiteSmxS, kCSiteSmxV,
-  kCSiteSmxSync, kCSiteSmxDone, kCSiteConvQ, kCSiteTree, kCSiteSmxTree,
+  kCSiteSmxSync, kCSiteSmxDone, kCSiteConvQ, kCSiteTree, kCSiteSmxTree, kCSiteMmaS, kCSiteSmxM, kCSiteSmxP, kCSiteSmxO,
 };
 
 template <int D, bool BF16, bool QUANT, int KG>
@@ -165,7 +168,7 @@ struct CachedLayout {
   static constexpr int kStageStride = 36;                  // words per row of the staging area (32 used)
   static constexpr int kStageBytes = 256 * kStageStride * 4;
   // Behind the staging area: maxima and sums, barriers, then (8 bit) exponents, scales, row scales, and the tree.
-  static constexpr int kMlBytes = 256 * 8;
+  static constexpr int kMlBytes = 128 * 8 + 256 * 4;
   static constexpr int kBarBytes = 512;
   static constexpr int kAuxBytes = QUANT ? kCachedAuxSlots * 2 * kCachedTile : 0;
   static constexpr int kScaleBytes = QUANT ? 8 * kKeys * 12 : 0;  // per warp: three numbers for each of its keys
@@ -176,7 +179,7 @@ struct CachedLayout {
   static constexpr int kSlots = kSlotsFit < kCachedMaxSlots ? kSlotsFit : kCachedMaxSlots;
   static_assert(kSlots >= 4, "two tiles have to fit");
   static constexpr int kSmem = kFixed + kSlots * kSlotBytes;
-  static constexpr int kOCol = 256;  // S of the two warpgroups | O of the two
+  static constexpr int kPCol = 256, kOCol = 384;  // S of the two warpgroups | P of the two | O
   // Registers of the warpgroups: 384 * 168 at launch = 256 * 208 + 128 * 88 = 256 * 184 + 128 * 136.
   static constexpr int kSoftmaxRegs = kKeys == 128 ? 208 : 184;
   static constexpr int kLoadRegs = kKeys == 128 ? 88 : 136;
@@ -184,8 +187,9 @@ struct CachedLayout {
 
 struct CachedBarriers {
   uint64_t full[kCachedMaxSlots], empty[kCachedMaxSlots];
-  uint64_t s_ready[2], p_ready[2];
-  uint64_t q_full, q_free, o_done, o_free, sync;
+  uint64_t s_ready[2], pv_done[2];
+  uint64_t s_free[2], p_ready[2];
+  uint64_t q_full, q_free, o_free, sync;
   uint64_t tree_full[2], tree_free[2];
   uint32_t tmem_base, abort_flag, dead;
   int32_t first_entry, first_head, first_offset, share;
@@ -260,6 +264,14 @@ __device__ __forceinline__ uint32_t cached_swz(uint32_t row, uint32_t chunk) {
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.volatile.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts64(uint32_t addr, uint2 v) {
+  asm volatile("st.volatile.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
+}
 __device__ __forceinline__ int lds_s8(uint32_t addr) {
   int v;
   asm volatile("ld.shared.s8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -300,7 +312,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       const uint32_t off = 8u * i;
       uint32_t count = 1;
       // The softmax warps arrive once each: 32 arrivals of a warp would be taken one after the other.
-      if (off >= offsetof(CachedBarriers, p_ready) && off < offsetof(CachedBarriers, q_full)) count = 4;
+      if (off >= offsetof(CachedBarriers, s_free) && off < offsetof(CachedBarriers, q_full)) count = 4;
       if (off == offsetof(CachedBarriers, o_free) || off == offsetof(CachedBarriers, sync)) count = 8;
       if (off >= offsetof(CachedBarriers, tree_free) && off < offsetof(CachedBarriers, tmem_base)) count = 8;
       mbar_init(bars_u32 + off, count);
@@ -375,8 +387,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     setmaxnreg_dec<L::kLoadRegs>();
     if (warp == 8) {
       // ------------------------------------------ loads --------------------------------------------------------------
-      // Order of the tiles in the ring, for T tiles of a segment: K0 K1 V0 K2 V1 ... K(T-1) V(T-2) V(T-1), which is the
-      // order in which the MMA warp uses them.  A lane has one page of a tile.
+      // Order of the tiles in the ring, for T tiles of a segment: K0 K1 K2 V0 K3 V1 ... K(T-1) V(T-3) V(T-2) V(T-1), which is
+      // about the order in which the MMA warps use them.  A lane has one page of a tile.
       const int piece_shift = min(a.page_shift, 7), piece = 1 << piece_shift;  // keys per TMA box
       const int pieces = kCachedTile >> piece_shift;
       int slot = 0;
@@ -408,13 +420,13 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           if (page < 0 || page >= a.num_pages) return -1;
           return ((page * a.kv_heads + cur.seg_head) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
         };
-        int row = piece_row(0), row_before = -1;
-        for (int i = 0; i <= cur.seg_n; ++i) {
+        int row = piece_row(0), row_1 = -1, row_2 = -1;  // of tiles i, i - 1, i - 2
+        for (int i = 0; i < cur.seg_n + 2; ++i) {
           const int row_next = piece_row(i + 1);  // its page id is on the way while this tile is loaded
 #pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            if (kv == 0 ? i == cur.seg_n : i == 0) continue;
-            const int at = kv == 0 ? row : row_before;
+          for (int kv = 0; kv < 2; ++kv) {  // K(i), V(i - 2)
+            if (kv == 0 ? i >= cur.seg_n : i < 2) continue;
+            const int at = kv == 0 ? row : row_2;
             if (seq >= L::kSlots && !warp_wait(SPLASH_KBAR(empty, slot), phase ^ 1, ctx, kCSiteLoadEmpty, seq)) { ok = false; break; }
             const uint32_t some = __ballot_sync(0xffffffffu, at >= 0);
             uint32_t bytes = __popc(some) * piece * L::kRowBytes;
@@ -428,7 +440,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
                 tma_load_2d(dst + c * (kCachedTile * L::kBoxBytes), kv == 0 ? &tm_k : &tm_v, c * L::kBoxElems, at, SPLASH_KBAR(full, slot));
               if (QUANT && kv == 0) {
                 // Exponents of the tile's keys and values.  Their slot is used again 16 tiles on; this warp is ahead of
-                // the MMA warp by the ring (at most 6 tiles), and that one of the softmax by two tiles.
+                // P V by the ring (at most 12 loads), and that one follows the softmax.
                 const uint32_t x = aux_u32 + aux * (2 * kCachedTile) + lane * piece;
                 bulk_load_1d(x, a.k_exponent + at, piece, SPLASH_KBAR(full, slot));
                 bulk_load_1d(x + kCachedTile, a.v_exponent + at, piece, SPLASH_KBAR(full, slot));
@@ -439,153 +451,79 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             if (++slot == L::kSlots) { slot = 0; phase ^= 1; }
           }
           if (!ok) break;
-          row_before = row;
+          row_2 = row_1;
+          row_1 = row;
           row = row_next;
         }
       }
-    } else if (warp == 9) {
+    } else if (warp == 9 || warp == 10) {
       // ------------------------------------------ products -----------------------------------------------------------
       constexpr uint32_t kHi = cached_desc_hi<L::kBoxBytes>();
-      constexpr uint32_t kQHi = kHi;
       constexpr uint32_t kIdescQK = make_idesc(BF16 && !QUANT, 128, kCachedTile, false, false);
       constexpr uint32_t kIdescPV = make_idesc(BF16 && !QUANT, 128, D, false, true);
       constexpr int kStepsPerBox = L::kBoxBytes / 32;  // an MMA takes 32 bytes of K per row
-      int slot = 0;
-      uint32_t phase = 0;
-      uint32_t p_par[2] = {0, 0};
-      int step = 0;
-      auto advance = [&]() { if (++slot == L::kSlots) { slot = 0; phase ^= 1; } };
-      auto issue_qk = [&](int grp) -> bool {
-        if (!warp_wait(SPLASH_KBAR(full, slot), phase, ctx, kCSiteMmaFull, step)) return false;
-        tc_fence_after();
-        const uint32_t b_lo = desc_lo(ring_u32 + slot * L::kSlotBytes, 16);
-#pragma unroll
-        for (int t = 0; t < L::kTerms; ++t) {
-          const uint32_t a_lo = desc_lo(q_u32 + t * L::kQTerm, 16);
-#pragma unroll
-          for (int kk = 0; kk < L::kRowBytes / 32; ++kk) {
-            const uint32_t off = ((kk / kStepsPerBox) * (128 * L::kBoxBytes) + (kk % kStepsPerBox) * 32) >> 4;
-            if constexpr (QUANT) umma8_ss2_w(tmem + grp * 128, a_lo + off, kQHi, b_lo + off, kHi, kIdescQK, t > 0 || kk > 0);
-            else umma_ss2_w(tmem + grp * 128, a_lo + off, kQHi, b_lo + off, kHi, kIdescQK, kk > 0);
-          }
-        }
-        umma_commit_w(SPLASH_KBAR(s_ready, grp));
-        umma_commit_w(SPLASH_KBAR(empty, slot));
-        advance();
-        return true;
-      };
+      int step0 = 0, seq = 0;  // tiles of the CTA in front of the segment, and their loads
       bool ok = true;
       for (int seg = 0; ok && cur.next(a); ++seg) {
         const int n = cur.seg_n;
-        if (!warp_wait(SPLASH_KBAR(q_full, 0), seg & 1, ctx, kCSiteMmaQ, seg)) break;
-        tc_fence_after();
-        if (!issue_qk(0)) break;
-        if (n > 1 && !issue_qk(1)) break;
-        if (n <= 2) umma_commit_w(SPLASH_KBAR(q_free, 0));
-        for (int i = 0; i < n; ++i, ++step) {
-          const int grp = i & 1;
-          if (!warp_wait(SPLASH_KBAR(full, slot), phase, ctx, kCSiteMmaFull, step) ||
-              !warp_wait(SPLASH_KBAR(p_ready, grp), p_par[grp], ctx, kCSiteMmaP, step) ||
-              // O may be written again once the previous segment's has been read.
-              (i == 0 && seg > 0 && !warp_wait(SPLASH_KBAR(o_free, 0), (seg - 1) & 1, ctx, kCSiteMmaO, seg))) { ok = false; break; }
-          p_par[grp] ^= 1;
-          tc_fence_after();
-          const uint32_t b_lo = desc_lo(ring_u32 + slot * L::kSlotBytes, kCachedTile * L::kBoxBytes);
-          constexpr int kKeysPerMma = QUANT ? 32 : 16;
-          // P is 8 columns an MMA; 8 bit: its second term follows in columns 32 .. 63, on the same values.
-#pragma unroll
-          for (int kk = 0; kk < (QUANT ? 2 : 1) * kCachedTile / kKeysPerMma; ++kk) {
-            const uint32_t off = ((kk * kKeysPerMma) % kCachedTile * L::kBoxBytes) >> 4;
-            if constexpr (QUANT) umma8_ts2_w(tmem + L::kOCol + grp * D, tmem + grp * 128 + kk * 8, b_lo + off, kHi, kIdescPV, i > 1 || kk > 0);
-            else umma_ts2_w(tmem + L::kOCol + grp * D, tmem + grp * 128 + kk * 8, b_lo + off, kHi, kIdescPV, i > 1 || kk > 0);
-          }
-          umma_commit_w(SPLASH_KBAR(empty, slot));
-          advance();
-          if (i + 2 < n) {
-            if (!issue_qk(grp)) { ok = false; break; }
-            if (i + 3 == n) umma_commit_w(SPLASH_KBAR(q_free, 0));
-          }
-        }
-        if (ok) umma_commit_w(SPLASH_KBAR(o_done, 0));
-      }
-    } else if (QUANT && warp == 11) {
-      // ------------------------------ Q as e4m3 terms, a row of 2 * D bytes at a time -----------------------------------
-      constexpr int kPer = D / 32;  // neighbouring numbers per lane
-      for (int seg = 0; cur.next(a); ++seg) {
-        const int b = cur.seg_entry / a.row_tiles, rt = cur.seg_entry - b * a.row_tiles;
-        if (seg > 0 && !warp_wait(SPLASH_KBAR(q_free, 0), (seg - 1) & 1, ctx, kCSiteConvQ, seg)) break;
-        const long long row0 = static_cast<long long>(b * a.kv_heads + cur.seg_head) * a.rows + rt * L::kRows;
-        const int rows = min(L::kRows, a.rows - rt * L::kRows);
-        constexpr int kBatch = 8;  // rows whose loads are in flight together
-        for (int r0 = 0; r0 < L::kRows; r0 += kBatch) {
-          uint32_t w[kBatch][kPer / 2];
-#pragma unroll
-          for (int j = 0; j < kBatch; ++j) {
-            const int r = r0 + j;
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) + (row0 + r) * D) + lane * (kPer / 2);
-#pragma unroll
-            for (int i = 0; i < kPer / 2; ++i) w[j][i] = r < rows ? __ldg(src + i) : 0u;
-          }
-#pragma unroll
-          for (int j = 0; j < kBatch; ++j) {
-            const int r = r0 + j;
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < kPer / 2; ++i) top = max(top, max(w[j][i] & 0x7fffu, (w[j][i] >> 16) & 0x7fffu));
-            top = __reduce_max_sync(0xffffffffu, top);
-            const bool bad = top >= (BF16 ? 0x7f80u : 0x7c00u);
-            float amax;
-            if constexpr (BF16) amax = __uint_as_float(top << 16);
-            else amax = __half2float(__ushort_as_half(static_cast<unsigned short>(top)));
-            // 2^-eq takes the largest number of the row into [128, 256).
-            const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 7, -100), 120);
-            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-            float x[kPer];
-#pragma unroll
-            for (int i = 0; i < kPer / 2; ++i) {
-              float2 f;
-              if constexpr (BF16) f = make_float2(__uint_as_float(w[j][i] << 16), __uint_as_float(w[j][i] & 0xffff0000u));
-              else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j][i]));
-              x[2 * i] = f.x * down;
-              x[2 * i + 1] = f.y * down;
-            }
-            if (lane == 0)
-              sts32(qscale_u32 + ((seg & 1) * 128 + r) * 4, bad ? 0x7fc00000u : static_cast<uint32_t>(e + 127) << 23);
+        if (warp == 9) {
+          if (!warp_wait(SPLASH_KBAR(q_full, 0), seg & 1, ctx, kCSiteMmaQ, seg)) break;
+          for (int i = 0; i < n; ++i) {
+            const int step = step0 + i, buf = step & 1;
+            const int at = seq + i + max(i - 2, 0), slot = at % L::kSlots;  // place of K(i) among the loads
+            if (!warp_wait(SPLASH_KBAR(full, slot), (at / L::kSlots) & 1, ctx, kCSiteMmaFull, step) ||
+                (step >= 2 && !warp_wait(SPLASH_KBAR(s_free, buf), ((step - 2) >> 1) & 1, ctx, kCSiteMmaS, step))) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t b_lo = desc_lo(ring_u32 + slot * L::kSlotBytes, 16);
 #pragma unroll
             for (int t = 0; t < L::kTerms; ++t) {
-              uint32_t code[kPer / 2];
+              const uint32_t a_lo = desc_lo(q_u32 + t * L::kQTerm, 16);
 #pragma unroll
-              for (int i = 0; i < kPer / 2; ++i) {
-                code[i] = e4m3x2(x[2 * i], x[2 * i + 1]);
-                const float2 f = e4m3x2_to_f32(code[i]);
-                x[2 * i] -= f.x;
-                x[2 * i + 1] -= f.y;
-              }
-              const uint32_t byte = lane * kPer;
-#pragma unroll
-              for (int copy = 0; copy < KG; ++copy) {
-                const uint32_t dst = q_u32 + t * L::kQTerm + cached_swz<L::kBoxBytes>(copy * L::kRows + r, byte >> 4) + (byte & 15u);
-                if constexpr (kPer == 4) sts32(dst, code[0] | (code[1] << 16));
-                else asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst), "h"(static_cast<uint16_t>(code[0])) : "memory");
+              for (int kk = 0; kk < L::kRowBytes / 32; ++kk) {
+                const uint32_t off = ((kk / kStepsPerBox) * (128 * L::kBoxBytes) + (kk % kStepsPerBox) * 32) >> 4;
+                if constexpr (QUANT) umma8_ss2_w(tmem + buf * 128, a_lo + off, kHi, b_lo + off, kHi, kIdescQK, t > 0 || kk > 0);
+                else umma_ss2_w(tmem + buf * 128, a_lo + off, kHi, b_lo + off, kHi, kIdescQK, kk > 0);
               }
             }
+            umma_commit_w(SPLASH_KBAR(s_ready, buf));
+            umma_commit_w(SPLASH_KBAR(empty, slot));
+          }
+          if (ok) umma_commit_w(SPLASH_KBAR(q_free, 0));
+        } else {
+          // O may be written again once the previous segment's has been read.
+          if (seg > 0 && !warp_wait(SPLASH_KBAR(o_free, 0), (seg - 1) & 1, ctx, kCSiteMmaO, seg)) break;
+          for (int i = 0; i < n; ++i) {
+            const int step = step0 + i, buf = step & 1;
+            const int at = seq + i + min(i + 3, n), slot = at % L::kSlots;  // place of V(i)
+            if (!warp_wait(SPLASH_KBAR(full, slot), (at / L::kSlots) & 1, ctx, kCSiteMmaFull, step) ||
+                !warp_wait(SPLASH_KBAR(p_ready, buf), (step >> 1) & 1, ctx, kCSiteMmaP, step)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t b_lo = desc_lo(ring_u32 + slot * L::kSlotBytes, kCachedTile * L::kBoxBytes);
+            const uint32_t p_tmem = tmem + L::kPCol + buf * 64;
+            constexpr int kKeysPerMma = QUANT ? 32 : 16;
+            // P is 8 columns an MMA; 8 bit: its second term follows in columns 32 .. 63, on the same values.
+#pragma unroll
+            for (int kk = 0; kk < (QUANT ? 2 : 1) * kCachedTile / kKeysPerMma; ++kk) {
+              const uint32_t off = ((kk * kKeysPerMma) % kCachedTile * L::kBoxBytes) >> 4;
+              if constexpr (QUANT) umma8_ts2_w(tmem + L::kOCol, p_tmem + kk * 8, b_lo + off, kHi, kIdescPV, i > 0 || kk > 0);
+              else umma_ts2_w(tmem + L::kOCol, p_tmem + kk * 8, b_lo + off, kHi, kIdescPV, i > 0 || kk > 0);
+            }
+            umma_commit_w(SPLASH_KBAR(empty, slot));
+            umma_commit_w(SPLASH_KBAR(pv_done, buf));
           }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(SPLASH_KBAR(q_full, 0));
+        step0 += n;
+        seq += 2 * n;
       }
-    } else if (warp == 10 && a.parents != nullptr) {
-      // ------------------------------ drafted trees, a sequence ahead of the softmax ------------------------------------
+    } else if (warp == 11 && (QUANT || a.parents != nullptr)) {
+      // ------------------------------ drafted trees, and Q as e4m3 terms, ahead of their use ------------------------------
+      int trees = 0, last = -1;
       // Which nodes each node sees -- itself and its ancestors -- by doubling: what a node sees is what it and the node
       // `up` steps above it see, for up = 1, 2, 4, ...
-      int trees = 0, last = -1;
-      for (int seg = 0; cur.next(a); ++seg) {
-        const int b = cur.seg_entry / a.row_tiles;
-        if (b == last) continue;
+      auto make_tree = [&](int b) -> bool {
         last = b;
         const int buf = trees & 1;
-        if (trees >= 2 && !warp_wait(SPLASH_KBAR(tree_free, buf), ((trees >> 1) & 1) ^ 1, ctx, kCSiteTree, trees)) break;
+        if (trees >= 2 && !warp_wait(SPLASH_KBAR(tree_free, buf), ((trees >> 1) & 1) ^ 1, ctx, kCSiteTree, trees)) return false;
         ++trees;
         const uint32_t tree = trees_u32 + buf * (kCachedMaxTree * 32);
         constexpr int kPer = kCachedMaxTree / 32;
@@ -649,11 +587,86 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           for (int w = 0; w < 4; ++w) sts32(tree + ((j * 32 + lane) * 8 + 1 + w) * 4, bits[j][w]);
         __syncwarp();
         if (lane == 0) mbar_arrive(SPLASH_KBAR(tree_full, buf));
+        return true;
+      };
+      auto split_q = [&](int seg, int b, int rt) -> bool {  // a row of 2 * D bytes at a time
+        constexpr int kPer = D / 32;  // neighbouring numbers per lane
+        if (seg > 0 && !warp_wait(SPLASH_KBAR(q_free, 0), (seg - 1) & 1, ctx, kCSiteConvQ, seg)) return false;
+        const long long row0 = static_cast<long long>(b * a.kv_heads + cur.seg_head) * a.rows + rt * L::kRows;
+        const int rows = min(L::kRows, a.rows - rt * L::kRows);
+        constexpr int kBatch = 8;  // rows whose loads are in flight together
+        for (int r0 = 0; r0 < L::kRows; r0 += kBatch) {
+          if (seg > 1 && a.row_tiles == 1 && r0 >= rows) break;  // zeros, as the first two segments have left them
+          uint32_t w[kBatch][kPer / 2];
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) {
+            const int r = r0 + j;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) + (row0 + r) * D) + lane * (kPer / 2);
+#pragma unroll
+            for (int i = 0; i < kPer / 2; ++i) w[j][i] = r < rows ? __ldg(src + i) : 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) {
+            const int r = r0 + j;
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < kPer / 2; ++i) top = max(top, max(w[j][i] & 0x7fffu, (w[j][i] >> 16) & 0x7fffu));
+            top = __reduce_max_sync(0xffffffffu, top);
+            const bool bad = top >= (BF16 ? 0x7f80u : 0x7c00u);
+            float amax;
+            if constexpr (BF16) amax = __uint_as_float(top << 16);
+            else amax = __half2float(__ushort_as_half(static_cast<unsigned short>(top)));
+            // 2^-eq takes the largest number of the row into [128, 256).
+            const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 7, -100), 120);
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            float x[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer / 2; ++i) {
+              float2 f;
+              if constexpr (BF16) f = make_float2(__uint_as_float(w[j][i] << 16), __uint_as_float(w[j][i] & 0xffff0000u));
+              else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j][i]));
+              x[2 * i] = f.x * down;
+              x[2 * i + 1] = f.y * down;
+            }
+            if (lane == 0)
+              sts32(qscale_u32 + ((seg & 1) * 128 + r) * 4, bad ? 0x7fc00000u : static_cast<uint32_t>(e + 127) << 23);
+#pragma unroll
+            for (int t = 0; t < L::kTerms; ++t) {
+              uint32_t code[kPer / 2];
+#pragma unroll
+              for (int i = 0; i < kPer / 2; ++i) {
+                code[i] = e4m3x2(x[2 * i], x[2 * i + 1]);
+                const float2 f = e4m3x2_to_f32(code[i]);
+                x[2 * i] -= f.x;
+                x[2 * i + 1] -= f.y;
+              }
+              const uint32_t byte = lane * kPer;
+#pragma unroll
+              for (int copy = 0; copy < KG; ++copy) {
+                const uint32_t dst = q_u32 + t * L::kQTerm + cached_swz<L::kBoxBytes>(copy * L::kRows + r, byte >> 4) + (byte & 15u);
+                if constexpr (kPer == 4) sts32(dst, code[0] | (code[1] << 16));
+                else asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst), "h"(static_cast<uint16_t>(code[0])) : "memory");
+              }
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(SPLASH_KBAR(q_full, 0));
+        return true;
+      };
+      for (int seg = 0; cur.next(a); ++seg) {
+        const int b = cur.seg_entry / a.row_tiles, rt = cur.seg_entry - b * a.row_tiles;
+        if (a.parents != nullptr && b != last && !make_tree(b)) break;
+        if constexpr (QUANT) {
+          if (!split_q(seg, b, rt)) break;
+        }
       }
     }
   } else {
     // ============================================ softmax ==============================================================
     setmaxnreg_inc<L::kSoftmaxRegs>();
+    if (threadIdx.x < 128) sts64(ml_u32 + threadIdx.x * 8, make_uint2(0xffffffffu, 0u));
     if (threadIdx.x == 0) a.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);  // (its first segment overwrites it)
     const int grp = warp >> 2;
     const int row_lane = (warp & 3) * 32 + lane;
@@ -661,7 +674,31 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     const int r = row_lane % L::kRows;
     const int col0 = part * L::kKeys;
     const uint32_t tmem_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t s_tmem = tmem_lane + grp * 128, o_tmem = tmem_lane + L::kOCol + grp * D;
+    const uint32_t o_tmem = tmem_lane + L::kOCol;
+    const uint32_t m_sh = ml_u32 + row_lane * 8;  // the latest tile of this row and copy, and the maximum after it
+    const uint32_t l_u32 = ml_u32 + 128 * 8;      // sums of the warpgroups, at the end
+    // A lane's maximum after tile `step`, which its counterpart in the other warpgroup has left or will leave there.
+    float m_got = 0.f;
+    auto wait_m = [&](int step) -> bool {
+      uint2 got = lds64(m_sh);
+      if (!__all_sync(0xffffffffu, got.x == static_cast<uint32_t>(step))) {
+        const uint64_t t0 = global_timer_ns();
+        for (uint32_t spins = 1; ; ++spins) {
+          got = lds64(m_sh);
+          if (__all_sync(0xffffffffu, got.x == static_cast<uint32_t>(step))) break;
+          if ((spins & 0xff) == 0) {
+            bool give_up = lds32(SPLASH_KWORD(abort_flag)) != 0;
+            if (!give_up && global_timer_ns() - t0 > kWaitLimitNs) {
+              sts32(SPLASH_KWORD(abort_flag), 0x80000000u | (static_cast<uint32_t>(kCSiteSmxM) << 20) | (static_cast<uint32_t>(step) & 0xfffffu));
+              give_up = true;
+            }
+            if (__any_sync(0xffffffffu, give_up)) return false;
+          }
+        }
+      }
+      m_got = __uint_as_float(got.y);
+      return true;
+    };
     const uint32_t my_scales = scale_u32 + warp * (L::kKeys * 12);
     const int piece_shift = min(a.page_shift, 7);
     const bool tree = a.parents != nullptr;
@@ -670,13 +707,20 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     const float inv_cap = a.soft_cap > 0.f ? 1.f / a.soft_cap : 1.f;
     constexpr float kThreshold = QUANT ? 1.f : 8.f;          // powers of 2 by which the maximum may lag behind
     constexpr float kPScale = QUANT ? 128.f : 1.f;           // 8 bit: P up to 2 * 128 of e4m3's 448
-    uint32_t s_par = 0, sync_par = 0;
+    uint32_t sync_par = 0;
+    int step0 = 0;   // tiles of the CTA in front of the segment
     int seq = 0;     // ring position of the segment's first tile
     int aux0 = 0;    // exponent slot of the segment's first tile
     bool ok = true;
-    uint32_t zero16[16];
+    if constexpr (KG > 1) {
+      // The probabilities of the other copies' keys are zero, once and for all: buffer `grp` is written by this warpgroup.
+      uint32_t zero16[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) zero16[j] = 0;
+      for (int j = 0; j < 16; ++j) zero16[j] = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_st16(tmem_lane + L::kPCol + grp * 64 + c * 16, zero16);
+      tmem_wait_st();
+    }
     int trees = 0, last_b = -1;
     auto arrive = [&](uint32_t bar) {  // of a warp, for what all its lanes have done
       __syncwarp();
@@ -727,9 +771,13 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         if (key < g.hi) asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(id) : "l"(table + (key >> a.page_shift)));
         return id;
       };
-      int page = page_of(grp);
+      const int i0 = (grp ^ step0) & 1;  // the CTA's tiles alternate between the warpgroups, whatever segment they are of
+      int page = page_of(i0);
 
-      for (int i = grp; i < n; i += 2) {
+      for (int i = i0; i < n; i += 2) {
+        const int step = step0 + i, buf = grp;
+        const uint32_t par = (step >> 1) & 1;
+        const uint32_t s_tmem = tmem_lane + buf * 128, p_tmem = tmem_lane + L::kPCol + buf * 64;
         const int key0 = cur.key0(i);
         asm volatile("" : "+r"(page));  // looked at here and not where it was asked for, a tile ago
         const uint32_t good = __ballot_sync(0xffffffffu, page >= 0 && page < a.num_pages);  // pieces that have a page
@@ -741,8 +789,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           const int key = key0 + at;
           return key < g.hi && (key >= g.lo || key < g.sink_hi) && ((good >> (at >> piece_shift)) & 1u);
         };
-        if (!warp_wait(SPLASH_KBAR(s_ready, grp), s_par, ctx, kCSiteSmxS, i)) { ok = false; break; }
-        s_par ^= 1;
+        if (!warp_wait(SPLASH_KBAR(s_ready, buf), par, ctx, kCSiteSmxS, step)) { ok = false; break; }
         tc_fence_after();
         float sv[L::kKeys];
         {
@@ -753,7 +800,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         if constexpr (QUANT) {
           // Scales of this warp's keys in shared memory of its own: 2^ek | ev | 2^ev * 32, while the scores arrive.
           // (The exponents came with the keys, for which the scores waited.)
-          if (i == grp) {
+          if (i == i0) {
             const float q_scale = __uint_as_float(lds32(qscale_u32 + ((seg & 1) * 128 + r) * 4));
             q_mul = q_scale * inv_cap;
             mul = a.soft_cap > 0.f ? unit2 : unit2 * q_scale;
@@ -775,6 +822,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           __syncwarp();
         }
         tmem_wait_ld();
+        tc_fence_before();
+        arrive(SPLASH_KBAR(s_free, buf));  // the scores of tile step + 2 may come
         if constexpr (QUANT) {
 #pragma unroll
           for (int j = 0; j < L::kKeys; j += 4) {
@@ -811,7 +860,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           // Values that no row sees are cleared: their probability is 0, and 0 times what lies there may be NaN.
           const uint32_t clear = __ballot_sync(0xffffffffu, !there(row_lane));
           if (clear) {
-            const int at = seq + (i + 1 < n ? 2 * i + 2 : 2 * n - 1);  // place of V(i) among the loads
+            const int at = seq + i + min(i + 3, n);  // place of V(i) among the loads
             const int slot = at % L::kSlots;
             if (!warp_wait(SPLASH_KBAR(full, slot), (at / L::kSlots) & 1, ctx, kCSiteSmxV, i)) { ok = false; break; }
             // The warp's 32 rows of the tile, 32 pieces of 16 bytes at a time.
@@ -845,6 +894,15 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
         float top = fmaxf(mx0, mx1);
         if constexpr (!QUANT) top *= mul;
+        if (i > 0) {
+          // The maximum that the previous tile settled on; this warpgroup's sum moves there first.
+          if (!wait_m(step - 1)) { ok = false; break; }
+          const float m_prev = m_got;
+          if (m_prev != m_run) {
+            l_run = m_run == -INFINITY ? (l_run == l_run ? 0.f : l_run) : l_run * ex2_approx(m_run - m_prev);
+            m_run = m_prev;
+          }
+        }
         const float m_new = fmaxf(m_run, top);
         const bool moved = m_new - m_run > kThreshold;  // false for NaN (-inf - -inf)
         float alpha = 1.f;
@@ -853,11 +911,14 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           m_run = m_new;
           l_run *= alpha;
         }
+        sts64(m_sh, make_uint2(static_cast<uint32_t>(step), __float_as_uint(m_run)));
+        // P's columns are free once P.V of this warpgroup's previous tile is done.
+        if (step >= 2 && !warp_wait(SPLASH_KBAR(pv_done, buf), ((step - 2) >> 1) & 1, ctx, kCSiteSmxP, step)) { ok = false; break; }
         const float shift = m_run == -INFINITY ? 0.f : -m_run;
         const float2 shift_2 = make_float2(shift, shift);
         float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
-        // P lies over S, 32 keys at a time: 16 columns of 16-bit numbers, or 8 columns of either e4m3 term, the second
-        // term 32 columns behind the first.  It is zero for the keys of the other copies.
+        // P is written 32 keys at a time: 16 columns of 16-bit numbers, or 8 columns of either e4m3 term, the second term 32
+        // columns behind the first.
 #pragma unroll
         for (int c = 0; c < L::kKeys / 32; ++c) {
           if constexpr (QUANT) {
@@ -879,8 +940,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
               p1[j] = e4m3x2(hx.x, hx.y) | (e4m3x2(hy.x, hy.y) << 16);
               p2[j] = e4m3x2(rx.x, rx.y) | (e4m3x2(ry.x, ry.y) << 16);
             }
-            tmem_st8(s_tmem + col0 / 4 + c * 8, p1);
-            tmem_st8(s_tmem + 32 + col0 / 4 + c * 8, p2);
+            tmem_st8(p_tmem + col0 / 4 + c * 8, p1);
+            tmem_st8(p_tmem + 32 + col0 / 4 + c * 8, p2);
           } else {
             uint32_t pk[16];
 #pragma unroll
@@ -890,24 +951,14 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
               if (j & 1) sum_b = add2(sum_b, e); else sum_a = add2(sum_a, e);
               pk[j] = pack2<BF16>(e.x, e.y);
             }
-            tmem_st16(s_tmem + col0 / 2 + c * 16, pk);
-          }
-        }
-        if constexpr (KG > 1) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (c * 32 >= col0 && c * 32 < col0 + L::kKeys) continue;
-            if constexpr (QUANT) {
-              tmem_st8(s_tmem + c * 8, zero16);
-              tmem_st8(s_tmem + 32 + c * 8, zero16);
-            } else {
-              tmem_st16(s_tmem + c * 16, zero16);
-            }
+            tmem_st16(p_tmem + col0 / 2 + c * 16, pk);
           }
         }
         l_run += (sum_a.x + sum_a.y) + (sum_b.x + sum_b.y);
-        // The scores of this tile came after P.V of the warpgroup's previous one: O stands still.
-        if (__builtin_expect(i >= 2 && __any_sync(0xffffffffu, moved), 0)) {
+        if (__builtin_expect(i > 0 && __any_sync(0xffffffffu, moved), 0)) {
+          // O may be touched once P.V of the previous tile is done.
+          if (!warp_wait(SPLASH_KBAR(pv_done, (step - 1) & 1), ((step - 1) >> 1) & 1, ctx, kCSiteSmxO, step)) { ok = false; break; }
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -920,32 +971,39 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
         tmem_wait_st();
         tc_fence_before();
-        arrive(SPLASH_KBAR(p_ready, grp));
+        arrive(SPLASH_KBAR(p_ready, buf));
       }
       if (!ok) break;
 
-      // ---- the parts of a row, added up: two warpgroups, and the copies of the rows ----
-      sts32(ml_u32 + threadIdx.x * 8, __float_as_uint(m_run));
-      sts32(ml_u32 + threadIdx.x * 8 + 4, __float_as_uint(l_run));
-      if (!warp_wait(SPLASH_KBAR(o_done, 0), seg & 1, ctx, kCSiteSmxDone, seg)) { ok = false; break; }
-      tc_fence_after();
+      // ---- the parts of a row, added up: the sums of the warpgroups, and the copies of the rows ----
+      const int last = step0 + n - 1;
+      if (!wait_m(last)) { ok = false; break; }
+      {
+        const float m_fin = m_got;
+        if (m_fin != m_run) {
+          l_run = m_run == -INFINITY ? (l_run == l_run ? 0.f : l_run) : l_run * ex2_approx(m_run - m_fin);
+          m_run = m_fin;
+        }
+      }
+      sts32(l_u32 + threadIdx.x * 4, __float_as_uint(l_run));
       if (!group_sync()) { ok = false; break; }
       float m_tot = -INFINITY, l_tot = 0.f;
 #pragma unroll
-      for (int src = 0; src < 2 * KG; ++src) {
-        const uint32_t at = ml_u32 + ((src / KG) * 128 + (src % KG) * L::kRows + r) * 8;
-        m_tot = fmaxf(m_tot, __uint_as_float(lds32(at)));
-      }
+      for (int src = 0; src < KG; ++src) m_tot = fmaxf(m_tot, __uint_as_float(lds32(ml_u32 + (src * L::kRows + r) * 8 + 4)));
 #pragma unroll
-      for (int src = 0; src < 2 * KG; ++src) {
-        const uint32_t at = ml_u32 + ((src / KG) * 128 + (src % KG) * L::kRows + r) * 8;
-        const float m = __uint_as_float(lds32(at)), l = __uint_as_float(lds32(at + 4));
+      for (int src = 0; src < KG; ++src) {
+        const uint32_t at = (src * L::kRows + r) * 4;
+        const float m = __uint_as_float(lds32(ml_u32 + 2 * at + 4));
+        const float l = __uint_as_float(lds32(l_u32 + at)) + __uint_as_float(lds32(l_u32 + 512 + at));
         if (l != 0.f) l_tot += m == -INFINITY ? l : l * ex2_approx(m - m_tot);
       }
+      const float l_mine = __uint_as_float(lds32(l_u32 + row_lane * 4)) + __uint_as_float(lds32(l_u32 + 512 + row_lane * 4));
+      if (!warp_wait(SPLASH_KBAR(pv_done, last & 1), (last >> 1) & 1, ctx, kCSiteSmxDone, last)) { ok = false; break; }
+      tc_fence_after();
       const bool whole = cur.whole;
       float w = m_run == -INFINITY ? 0.f : ex2_approx(m_run - m_tot);
       w *= 1.f / kPScale;
-      if (l_run != l_run) w = l_run;  // NaN: no maximum may have been met
+      if (l_mine != l_mine) w = l_mine;  // NaN: no maximum may have been met
       if (whole) w *= l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
       const long long out_row0 = static_cast<long long>(b * a.kv_heads + cur.seg_head) * a.rows + rt * L::kRows;
       const long long part0 = static_cast<long long>(2 * blockIdx.x + (seg > 0)) * L::kRows;
@@ -955,24 +1013,24 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         else if (a.lse_out && row_all < a.rows)
           a.lse_out[out_row0 + r] = live && l_tot != 0.f ? (m_tot + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
       }
-      const int col = (threadIdx.x % 8) * 4;  // of a chunk of 32: eight threads add up a row of it, 128 bytes
+      // Each warpgroup has one half of O's columns, 32 at a time: every copy's lanes leave theirs, eight threads add up the 128
+      // bytes of a row.
+      const int col = (threadIdx.x % 8) * 4;
+      const uint32_t my_stage = stage_u32 + grp * (128 * L::kStageStride * 4);
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = grp * (D / 64); c < (grp + 1) * (D / 64); ++c) {
         uint32_t o[32];
-        if (grp < n) {
-          tmem_ld32(o_tmem + c * 32, o);
-          tmem_wait_ld();
-        }
-        if (c == D / 32 - 1) {
+        tmem_ld32(o_tmem + c * 32, o);
+        tmem_wait_ld();
+        if (c == (grp + 1) * (D / 64) - 1) {
           tc_fence_before();
           arrive(SPLASH_KBAR(o_free, 0));
         }
-        const uint32_t dst = stage_u32 + threadIdx.x * (L::kStageStride * 4);
-        const bool any = grp < n && live;
+        const uint32_t dst = my_stage + row_lane * (L::kStageStride * 4);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           uint4 x = make_uint4(0, 0, 0, 0);
-          if (any) {
+          if (live) {
             x.x = __float_as_uint(__uint_as_float(o[k * 4]) * w);
             x.y = __float_as_uint(__uint_as_float(o[k * 4 + 1]) * w);
             x.z = __float_as_uint(__uint_as_float(o[k * 4 + 2]) * w);
@@ -982,13 +1040,12 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
         if (!group_sync()) { ok = false; break; }
 #pragma unroll
-        for (int k = 0; k < L::kRows / 32; ++k) {
-          const int row = k * 32 + threadIdx.x / 8;
+        for (int k = 0; k < L::kRows / 16; ++k) {
+          const int row = k * 16 + (threadIdx.x & 127) / 8;
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int src = 0; src < 2 * KG; ++src) {
-            const int from = (src / KG) * 128 + (src % KG) * L::kRows + row;
-            const uint4 x = lds128(stage_u32 + (from * L::kStageStride + col) * 4);
+          for (int src = 0; src < KG; ++src) {
+            const uint4 x = lds128(my_stage + ((src * L::kRows + row) * L::kStageStride + col) * 4);
             acc.x += __uint_as_float(x.x);
             acc.y += __uint_as_float(x.y);
             acc.z += __uint_as_float(x.z);
@@ -1004,6 +1061,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
         if (!group_sync()) { ok = false; break; }
       }
+      step0 += n;
       seq += 2 * n;
       aux0 += n;
     }
