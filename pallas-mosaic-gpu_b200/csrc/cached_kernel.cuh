@@ -8,15 +8,16 @@
 //   * The tiles of all units stand in one line that is cut into equal shares, one per CTA (one CTA per SM), whatever the
 //     lengths of the sequences are.  A unit that several CTAs share leaves partial results (unnormalised O, maximum and
 //     sum per row, f32) for cached_finish_kernel, which adds them in the order of the keys: the same bits every time.
-//   * One producer warp walks the line ahead of the others, across units: page ids a tile ahead, one TMA box per page.
+//   * Two producer warps, for keys and values, walk the line ahead of the others, across units: page ids two tiles ahead, one
+//     TMA box per page.
 //   * Rows are few, so the 128 rows of an MMA are used otherwise: Q is laid into shared memory 128 / R times, and each
 //     copy's warps take the exponentials of their own part of the tile's keys (P is zero elsewhere); the copies' results
 //     are added like partial ones.  A softmax warp of a one-token call thus works on 32 of 128 keys.
 //   * Two softmax warpgroups take the tiles in turn.  They hand the (lagging) maxima to one another through shared memory,
 //     a tile's right after its comparison and long before its exponentials, and keep partial sums; P has columns of its
-//     own, so the scores of tile t + 2 are computed as soon as those of tile t are in registers: one warp issues the score
-//     products, another P V, and neither waits for what the other waits for.  Tensor memory: S0 S1 P0 P1 O = 128 + 128 + 64 +
-//     64 + head_dim columns.
+//     own, so the scores of tile t + 2 are computed as soon as those of tile t are in registers: the warp that issues the
+//     products looks at what either kind waits for and takes what is ready.  Tensor memory: S0 S1 P0 P1 O = 128 + 128 + 64 + 64
+//     + head_dim columns.
 //
 // 8-bit caches are not widened on the way: e4m3 keys and values are operands of the MMA as they lie in the cache, and
 // the 16-bit Q and the probabilities are split into e4m3 terms instead, which are few:
@@ -37,7 +38,7 @@ namespace splash {
 
 constexpr int kCachedThreads = 384;
 constexpr int kCachedTile = 128;        // keys per tile
-constexpr int kCachedMaxSlots = 12;
+constexpr int kCachedMaxSlots = 6;      // of the K ring, and of the V ring
 constexpr int kCachedAuxSlots = 16;     // exponents of a tile; more than tiles can be on their way (see the producer)
 constexpr int kCachedMaxTree = 128;     // nodes of a drafted tree
 // What a unit costs besides its tiles, in tiles (its start, and the sum of its parts): it stands that much longer in the line.
@@ -175,10 +176,10 @@ struct CachedLayout {
   static constexpr int kQScaleBytes = QUANT ? 2 * 128 * 4 : 0;
   static constexpr int kTreeBytes = kCachedMaxTree * 8 + 2 * kCachedMaxTree * 8 * 4;  // parents, pointers | two trees
   static constexpr int kFixed = 1024 + kQBytes + kStageBytes + kMlBytes + kBarBytes + kAuxBytes + kScaleBytes + kQScaleBytes + kTreeBytes;
-  static constexpr int kSlotsFit = (227 * 1024 - kFixed) / kSlotBytes;
-  static constexpr int kSlots = kSlotsFit < kCachedMaxSlots ? kSlotsFit : kCachedMaxSlots;
-  static_assert(kSlots >= 4, "two tiles have to fit");
-  static constexpr int kSmem = kFixed + kSlots * kSlotBytes;
+  static constexpr int kSlotsFit = (227 * 1024 - kFixed) / (2 * kSlotBytes);
+  static constexpr int kSlots = kSlotsFit < kCachedMaxSlots ? kSlotsFit : kCachedMaxSlots;  // tiles of either ring
+  static_assert(kSlots >= 2, "two tiles have to fit");
+  static constexpr int kSmem = kFixed + 2 * kSlots * kSlotBytes;
   static constexpr int kPCol = 256, kOCol = 384;  // S of the two warpgroups | P of the two | O
   // Registers of the warpgroups: 384 * 168 at launch = 256 * 208 + 128 * 88 = 256 * 184 + 128 * 136.
   static constexpr int kSoftmaxRegs = kKeys == 128 ? 208 : 184;
@@ -186,7 +187,9 @@ struct CachedLayout {
 };
 
 struct CachedBarriers {
-  uint64_t full[kCachedMaxSlots], empty[kCachedMaxSlots];
+  // The keys' ring and the values' are apart: a parity tells a slot's phase only from the one before, so whoever waits for
+  // a slot must have waited for its previous use, and scores and P V go through their tiles at paces of their own.
+  uint64_t k_full[kCachedMaxSlots], k_empty[kCachedMaxSlots], v_full[kCachedMaxSlots], v_empty[kCachedMaxSlots];
   uint64_t s_ready[2], pv_done[2];
   uint64_t s_free[2], p_ready[2];
   uint64_t q_full, q_free, o_free, sync;
@@ -264,13 +267,28 @@ __device__ __forceinline__ uint32_t cached_swz(uint32_t row, uint32_t chunk) {
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.volatile.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+// Whole 64-bit words: tile (low half) and maximum of a row arrive together.
+__device__ __forceinline__ uint64_t lds64(uint32_t addr) {
+  uint64_t v;
+  asm volatile("ld.volatile.shared.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void sts64(uint32_t addr, uint2 v) {
-  asm volatile("st.volatile.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
+__device__ __forceinline__ void sts64(uint32_t addr, uint64_t v) {
+  asm volatile("st.volatile.shared.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+// Whether a barrier's phase is over, without waiting.
+__device__ __forceinline__ bool mbar_probe(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 __device__ __forceinline__ int lds_s8(uint32_t addr) {
   int v;
@@ -289,8 +307,9 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   using L = CachedLayout<D, BF16, QUANT, KG>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t q_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t ring_u32 = q_u32 + L::kQBytes;
-  const uint32_t stage_u32 = ring_u32 + L::kSlots * L::kSlotBytes;
+  const uint32_t k_u32 = q_u32 + L::kQBytes;
+  const uint32_t v_u32 = k_u32 + L::kSlots * L::kSlotBytes;
+  const uint32_t stage_u32 = v_u32 + L::kSlots * L::kSlotBytes;
   const uint32_t ml_u32 = stage_u32 + L::kStageBytes;
   const uint32_t bars_u32 = ml_u32 + L::kMlBytes;
   const uint32_t aux_u32 = bars_u32 + L::kBarBytes;
@@ -330,6 +349,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   } else if (warp == 9) {
     tmem_alloc(SPLASH_KWORD(tmem_base), 512);
     tmem_relinquish();
+  } else if (warp >= 4 && warp < 8) {
+    sts64(ml_u32 + (threadIdx.x - 128) * 8, 0xffffffffull);  // no tile yet
   } else if (warp == 0) {
     const int entries = a.batch * a.row_tiles;
     auto line = [&](int e) -> int {  // what (sequence, row tile) e takes of the line, all kv heads
@@ -385,20 +406,23 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
 
   if (warp >= 8) {
     setmaxnreg_dec<L::kLoadRegs>();
-    if (warp == 8) {
-      // ------------------------------------------ loads --------------------------------------------------------------
-      // Order of the tiles in the ring, for T tiles of a segment: K0 K1 K2 V0 K3 V1 ... K(T-1) V(T-3) V(T-2) V(T-1), which is
-      // about the order in which the MMA warps use them.  A lane has one page of a tile.
-      const int piece_shift = min(a.page_shift, 7), piece = 1 << piece_shift;  // keys per TMA box
+    if (warp == 8 || warp == 11) {
+      // ------------------------------------------ loads: keys (and Q, and exponents), values ----------------------------
+      const bool is_v = warp == 11;
+      const CUtensorMap* tm = is_v ? &tm_v : &tm_k;
+      const uint32_t ring = is_v ? v_u32 : k_u32;
+      const uint32_t full = is_v ? SPLASH_KBAR(v_full, 0) : SPLASH_KBAR(k_full, 0);
+      const uint32_t empty = is_v ? SPLASH_KBAR(v_empty, 0) : SPLASH_KBAR(k_empty, 0);
+      const int piece_shift = min(a.page_shift, 7), piece = 1 << piece_shift;  // keys per TMA box; a lane has one box of a tile
       const int pieces = kCachedTile >> piece_shift;
       int slot = 0;
       uint32_t phase = 0;
-      int seq = 0, aux = 0;
+      int step = 0;
       bool ok = true;
       for (int seg = 0; ok && cur.next(a); ++seg) {
         const CachedGeom& g = cur.g;
         const int b = cur.seg_entry / a.row_tiles, rt = cur.seg_entry - b * a.row_tiles;
-        if constexpr (!QUANT) {
+        if (!QUANT && !is_v) {
           if (seg > 0 && !warp_wait(SPLASH_KBAR(q_free, 0), (seg - 1) & 1, ctx, kCSiteLoadQ, seg)) break;
           if (elect_one()) {
             const int row = (b * a.kv_heads + cur.seg_head) * a.rows + rt * L::kRows;
@@ -411,70 +435,80 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           }
         }
         const int32_t* table = a.page_table + b * a.table_stride;
-        // Row of the cache where this lane's piece of tile i begins, -1: nobody sees it, or no page.
-        auto piece_row = [&](int i) -> int {
-          if (i >= cur.seg_n || lane >= pieces) return -1;
-          const int key = cur.key0(i) + lane * piece;
-          if (key >= g.hi || (key + piece <= g.lo && key >= g.sink_hi)) return -1;
-          const int page = table[key >> a.page_shift];
-          if (page < 0 || page >= a.num_pages) return -1;
-          return ((page * a.kv_heads + cur.seg_head) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
-        };
-        int row = piece_row(0), row_1 = -1, row_2 = -1;  // of tiles i, i - 1, i - 2
-        for (int i = 0; i < cur.seg_n + 2; ++i) {
-          const int row_next = piece_row(i + 1);  // its page id is on the way while this tile is loaded
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {  // K(i), V(i - 2)
-            if (kv == 0 ? i >= cur.seg_n : i < 2) continue;
-            const int at = kv == 0 ? row : row_2;
-            if (seq >= L::kSlots && !warp_wait(SPLASH_KBAR(empty, slot), phase ^ 1, ctx, kCSiteLoadEmpty, seq)) { ok = false; break; }
-            const uint32_t some = __ballot_sync(0xffffffffu, at >= 0);
-            uint32_t bytes = __popc(some) * piece * L::kRowBytes;
-            if (QUANT && kv == 0) bytes += __popc(some) * piece * 2;
-            if (lane == 0) mbar_arrive_expect_tx(SPLASH_KBAR(full, slot), bytes);
-            __syncwarp();
-            if (at >= 0) {
-              const uint32_t dst = ring_u32 + slot * L::kSlotBytes + lane * piece * L::kBoxBytes;
-#pragma unroll
-              for (int c = 0; c < L::kBoxes; ++c)
-                tma_load_2d(dst + c * (kCachedTile * L::kBoxBytes), kv == 0 ? &tm_k : &tm_v, c * L::kBoxElems, at, SPLASH_KBAR(full, slot));
-              if (QUANT && kv == 0) {
-                // Exponents of the tile's keys and values.  Their slot is used again 16 tiles on; this warp is ahead of
-                // P V by the ring (at most 12 loads), and that one follows the softmax.
-                const uint32_t x = aux_u32 + aux * (2 * kCachedTile) + lane * piece;
-                bulk_load_1d(x, a.k_exponent + at, piece, SPLASH_KBAR(full, slot));
-                bulk_load_1d(x + kCachedTile, a.v_exponent + at, piece, SPLASH_KBAR(full, slot));
-              }
-            }
-            if (kv == 0 && ++aux == kCachedAuxSlots) aux = 0;
-            ++seq;
-            if (++slot == L::kSlots) { slot = 0; phase ^= 1; }
+        // This lane's piece of tile i: its page id, -1 where nobody sees it; asked for two tiles ahead of its use, so that
+        // the load never waits for it.
+        auto page_of = [&](int i) -> int {
+          int id = -1;
+          if (i < cur.seg_n && lane < pieces) {
+            const int key = cur.key0(i) + lane * piece;
+            if (key < g.hi && (key + piece > g.lo || key < g.sink_hi))
+              asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(id) : "l"(table + (key >> a.page_shift)));
           }
-          if (!ok) break;
-          row_2 = row_1;
-          row_1 = row;
-          row = row_next;
+          return id;
+        };
+        int page = page_of(0), page_1 = page_of(1);  // of tiles i, i + 1
+        for (int i = 0; i < cur.seg_n; ++i, ++step) {
+          const int page_2 = page_of(i + 2);
+          if (step >= L::kSlots && !warp_wait(empty + 8 * slot, phase ^ 1, ctx, kCSiteLoadEmpty, step)) { ok = false; break; }
+          asm volatile("" : "+r"(page));
+          const bool some = page >= 0 && page < a.num_pages;
+          const uint32_t count = __popc(__ballot_sync(0xffffffffu, some));
+          if (lane == 0) mbar_arrive_expect_tx(full + 8 * slot, count * piece * (L::kRowBytes + (QUANT && !is_v ? 2 : 0)));
+          __syncwarp();
+          if (some) {
+            const int row = ((page * a.kv_heads + cur.seg_head) << a.page_shift) + ((cur.key0(i) + lane * piece) & ((1 << a.page_shift) - 1));
+            const uint32_t dst = ring + slot * L::kSlotBytes + lane * piece * L::kBoxBytes;
+#pragma unroll
+            for (int c = 0; c < L::kBoxes; ++c)
+              tma_load_2d(dst + c * (kCachedTile * L::kBoxBytes), tm, c * L::kBoxElems, row, full + 8 * slot);
+            if (QUANT && !is_v) {
+              // Exponents of the tile's keys and values.  Their slot is used again 16 tiles on; this warp is ahead of the
+              // scores by the ring (at most 6 tiles), and those of the softmax by two.
+              const uint32_t x = aux_u32 + (step % kCachedAuxSlots) * (2 * kCachedTile) + lane * piece;
+              bulk_load_1d(x, a.k_exponent + row, piece, full + 8 * slot);
+              bulk_load_1d(x + kCachedTile, a.v_exponent + row, piece, full + 8 * slot);
+            }
+          }
+          if (++slot == L::kSlots) { slot = 0; phase ^= 1; }
+          page = page_1;
+          page_1 = page_2;
         }
       }
-    } else if (warp == 9 || warp == 10) {
+    } else if (warp == 9) {
       // ------------------------------------------ products -----------------------------------------------------------
       constexpr uint32_t kHi = cached_desc_hi<L::kBoxBytes>();
       constexpr uint32_t kIdescQK = make_idesc(BF16 && !QUANT, 128, kCachedTile, false, false);
       constexpr uint32_t kIdescPV = make_idesc(BF16 && !QUANT, 128, D, false, true);
       constexpr int kStepsPerBox = L::kBoxBytes / 32;  // an MMA takes 32 bytes of K per row
-      int step0 = 0, seq = 0;  // tiles of the CTA in front of the segment, and their loads
-      bool ok = true;
-      for (int seg = 0; ok && cur.next(a); ++seg) {
-        const int n = cur.seg_n;
-        if (warp == 9) {
-          if (!warp_wait(SPLASH_KBAR(q_full, 0), seg & 1, ctx, kCSiteMmaQ, seg)) break;
-          for (int i = 0; i < n; ++i) {
-            const int step = step0 + i, buf = step & 1;
-            const int at = seq + i + max(i - 2, 0), slot = at % L::kSlots;  // place of K(i) among the loads
-            if (!warp_wait(SPLASH_KBAR(full, slot), (at / L::kSlots) & 1, ctx, kCSiteMmaFull, step) ||
-                (step >= 2 && !warp_wait(SPLASH_KBAR(s_free, buf), ((step - 2) >> 1) & 1, ctx, kCSiteMmaS, step))) { ok = false; break; }
+      // Two walks along the share, over tiles: the scores' and P V's.  `step`: tiles of the CTA so far, buffers by its lowest
+      // bit and parities by the next, ring slots by its remainder.
+      struct Walk {
+        CachedCursor cur;
+        int seg, i, step;
+        bool on;
+        __device__ __forceinline__ void advance(const CachedArgs& a) {
+          ++step;
+          if (++i == cur.seg_n) {
+            i = 0;
+            ++seg;
+            on = cur.next(a);
+          }
+        }
+      };
+      const bool any = cur.next(a);
+      Walk qk{cur, 0, 0, 0, any}, pv = qk;
+      uint32_t spins = 0;
+      uint64_t t0 = 0;
+      while (qk.on || pv.on) {
+        bool issued = false;
+        if (qk.on) {
+          const int buf = qk.step & 1, slot = qk.step % L::kSlots;
+          const bool ready = mbar_probe(SPLASH_KBAR(k_full, slot), (qk.step / L::kSlots) & 1) &&
+                             (qk.step < 2 || mbar_probe(SPLASH_KBAR(s_free, buf), ((qk.step - 2) >> 1) & 1)) &&
+                             (qk.i > 0 || mbar_probe(SPLASH_KBAR(q_full, 0), qk.seg & 1));
+          if (__all_sync(0xffffffffu, ready)) {
             tc_fence_after();
-            const uint32_t b_lo = desc_lo(ring_u32 + slot * L::kSlotBytes, 16);
+            const uint32_t b_lo = desc_lo(k_u32 + slot * L::kSlotBytes, 16);
 #pragma unroll
             for (int t = 0; t < L::kTerms; ++t) {
               const uint32_t a_lo = desc_lo(q_u32 + t * L::kQTerm, 16);
@@ -486,36 +520,51 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
               }
             }
             umma_commit_w(SPLASH_KBAR(s_ready, buf));
-            umma_commit_w(SPLASH_KBAR(empty, slot));
+            umma_commit_w(SPLASH_KBAR(k_empty, slot));
+            if (qk.i + 1 == qk.cur.seg_n) umma_commit_w(SPLASH_KBAR(q_free, 0));
+            qk.advance(a);
+            issued = true;
           }
-          if (ok) umma_commit_w(SPLASH_KBAR(q_free, 0));
-        } else {
-          // O may be written again once the previous segment's has been read.
-          if (seg > 0 && !warp_wait(SPLASH_KBAR(o_free, 0), (seg - 1) & 1, ctx, kCSiteMmaO, seg)) break;
-          for (int i = 0; i < n; ++i) {
-            const int step = step0 + i, buf = step & 1;
-            const int at = seq + i + min(i + 3, n), slot = at % L::kSlots;  // place of V(i)
-            if (!warp_wait(SPLASH_KBAR(full, slot), (at / L::kSlots) & 1, ctx, kCSiteMmaFull, step) ||
-                !warp_wait(SPLASH_KBAR(p_ready, buf), (step >> 1) & 1, ctx, kCSiteMmaP, step)) { ok = false; break; }
+        }
+        if (pv.on) {
+          const int buf = pv.step & 1, slot = pv.step % L::kSlots;
+          const bool ready = mbar_probe(SPLASH_KBAR(p_ready, buf), (pv.step >> 1) & 1) &&
+                             mbar_probe(SPLASH_KBAR(v_full, slot), (pv.step / L::kSlots) & 1) &&
+                             // O may be written again once the previous segment's has been read.
+                             (pv.i > 0 || pv.seg == 0 || mbar_probe(SPLASH_KBAR(o_free, 0), (pv.seg - 1) & 1));
+          if (__all_sync(0xffffffffu, ready)) {
             tc_fence_after();
-            const uint32_t b_lo = desc_lo(ring_u32 + slot * L::kSlotBytes, kCachedTile * L::kBoxBytes);
+            const uint32_t b_lo = desc_lo(v_u32 + slot * L::kSlotBytes, kCachedTile * L::kBoxBytes);
             const uint32_t p_tmem = tmem + L::kPCol + buf * 64;
             constexpr int kKeysPerMma = QUANT ? 32 : 16;
             // P is 8 columns an MMA; 8 bit: its second term follows in columns 32 .. 63, on the same values.
 #pragma unroll
             for (int kk = 0; kk < (QUANT ? 2 : 1) * kCachedTile / kKeysPerMma; ++kk) {
               const uint32_t off = ((kk * kKeysPerMma) % kCachedTile * L::kBoxBytes) >> 4;
-              if constexpr (QUANT) umma8_ts2_w(tmem + L::kOCol, p_tmem + kk * 8, b_lo + off, kHi, kIdescPV, i > 0 || kk > 0);
-              else umma_ts2_w(tmem + L::kOCol, p_tmem + kk * 8, b_lo + off, kHi, kIdescPV, i > 0 || kk > 0);
+              if constexpr (QUANT) umma8_ts2_w(tmem + L::kOCol, p_tmem + kk * 8, b_lo + off, kHi, kIdescPV, pv.i > 0 || kk > 0);
+              else umma_ts2_w(tmem + L::kOCol, p_tmem + kk * 8, b_lo + off, kHi, kIdescPV, pv.i > 0 || kk > 0);
             }
-            umma_commit_w(SPLASH_KBAR(empty, slot));
+            umma_commit_w(SPLASH_KBAR(v_empty, slot));
             umma_commit_w(SPLASH_KBAR(pv_done, buf));
+            pv.advance(a);
+            issued = true;
           }
         }
-        step0 += n;
-        seq += 2 * n;
+        // Bounded, as every wait: about a second without anything to issue.
+        if (issued) {
+          spins = 0;
+        } else if ((++spins & 0xff) == 0) {
+          const uint64_t now = global_timer_ns();
+          if (spins == 0x100) t0 = now;
+          bool give_up = lds32(SPLASH_KWORD(abort_flag)) != 0;
+          if (!give_up && now - t0 > kWaitLimitNs) {
+            sts32(SPLASH_KWORD(abort_flag), 0x80000000u | (static_cast<uint32_t>(kCSiteMmaFull) << 20) | (static_cast<uint32_t>(pv.step) & 0xfffffu));
+            give_up = true;
+          }
+          if (__any_sync(0xffffffffu, give_up)) break;
+        }
       }
-    } else if (warp == 11 && (QUANT || a.parents != nullptr)) {
+    } else if (warp == 10 && (QUANT || a.parents != nullptr)) {
       // ------------------------------ drafted trees, and Q as e4m3 terms, ahead of their use ------------------------------
       int trees = 0, last = -1;
       // Which nodes each node sees -- itself and its ancestors -- by doubling: what a node sees is what it and the node
@@ -666,7 +715,6 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   } else {
     // ============================================ softmax ==============================================================
     setmaxnreg_inc<L::kSoftmaxRegs>();
-    if (threadIdx.x < 128) sts64(ml_u32 + threadIdx.x * 8, make_uint2(0xffffffffu, 0u));
     if (threadIdx.x == 0) a.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);  // (its first segment overwrites it)
     const int grp = warp >> 2;
     const int row_lane = (warp & 3) * 32 + lane;
@@ -680,12 +728,12 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     // A lane's maximum after tile `step`, which its counterpart in the other warpgroup has left or will leave there.
     float m_got = 0.f;
     auto wait_m = [&](int step) -> bool {
-      uint2 got = lds64(m_sh);
-      if (!__all_sync(0xffffffffu, got.x == static_cast<uint32_t>(step))) {
+      uint64_t got = lds64(m_sh);
+      if (!__all_sync(0xffffffffu, static_cast<uint32_t>(got) == static_cast<uint32_t>(step))) {
         const uint64_t t0 = global_timer_ns();
         for (uint32_t spins = 1; ; ++spins) {
           got = lds64(m_sh);
-          if (__all_sync(0xffffffffu, got.x == static_cast<uint32_t>(step))) break;
+          if (__all_sync(0xffffffffu, static_cast<uint32_t>(got) == static_cast<uint32_t>(step))) break;
           if ((spins & 0xff) == 0) {
             bool give_up = lds32(SPLASH_KWORD(abort_flag)) != 0;
             if (!give_up && global_timer_ns() - t0 > kWaitLimitNs) {
@@ -696,7 +744,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           }
         }
       }
-      m_got = __uint_as_float(got.y);
+      m_got = __uint_as_float(static_cast<uint32_t>(got >> 32));
       return true;
     };
     const uint32_t my_scales = scale_u32 + warp * (L::kKeys * 12);
@@ -709,8 +757,6 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     constexpr float kPScale = QUANT ? 128.f : 1.f;           // 8 bit: P up to 2 * 128 of e4m3's 448
     uint32_t sync_par = 0;
     int step0 = 0;   // tiles of the CTA in front of the segment
-    int seq = 0;     // ring position of the segment's first tile
-    int aux0 = 0;    // exponent slot of the segment's first tile
     bool ok = true;
     if constexpr (KG > 1) {
       // The probabilities of the other copies' keys are zero, once and for all: buffer `grp` is written by this warpgroup.
@@ -805,7 +851,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             q_mul = q_scale * inv_cap;
             mul = a.soft_cap > 0.f ? unit2 : unit2 * q_scale;
           }
-          const uint32_t x = aux_u32 + ((aux0 + i) % kCachedAuxSlots) * (2 * kCachedTile) + col0;
+          const uint32_t x = aux_u32 + (step % kCachedAuxSlots) * (2 * kCachedTile) + col0;
           __syncwarp();
 #pragma unroll
           for (int c = 0; c < L::kKeys / 32; ++c) {
@@ -860,12 +906,13 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           // Values that no row sees are cleared: their probability is 0, and 0 times what lies there may be NaN.
           const uint32_t clear = __ballot_sync(0xffffffffu, !there(row_lane));
           if (clear) {
-            const int at = seq + i + min(i + 3, n);  // place of V(i) among the loads
-            const int slot = at % L::kSlots;
-            if (!warp_wait(SPLASH_KBAR(full, slot), (at / L::kSlots) & 1, ctx, kCSiteSmxV, i)) { ok = false; break; }
+            // (P V of tile step - 2 is over: so is the previous use of the slot, without which its parity says nothing.)
+            const int slot = step % L::kSlots;
+            if ((step >= 2 && !warp_wait(SPLASH_KBAR(pv_done, buf), ((step - 2) >> 1) & 1, ctx, kCSiteSmxP, step)) ||
+                !warp_wait(SPLASH_KBAR(v_full, slot), (step / L::kSlots) & 1, ctx, kCSiteSmxV, step)) { ok = false; break; }
             // The warp's 32 rows of the tile, 32 pieces of 16 bytes at a time.
             constexpr int kChunks = L::kBoxBytes / 16, kAtOnce = 32 / kChunks;
-            const uint32_t dst = ring_u32 + slot * L::kSlotBytes + (warp & 3) * 32 * L::kBoxBytes + (lane % kChunks) * 16;
+            const uint32_t dst = v_u32 + slot * L::kSlotBytes + (warp & 3) * 32 * L::kBoxBytes + (lane % kChunks) * 16;
 #pragma unroll 1
             for (int k = lane / kChunks; k < 32; k += kAtOnce)
               if ((clear >> k) & 1u)
@@ -911,7 +958,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           m_run = m_new;
           l_run *= alpha;
         }
-        sts64(m_sh, make_uint2(static_cast<uint32_t>(step), __float_as_uint(m_run)));
+        sts64(m_sh, static_cast<uint64_t>(__float_as_uint(m_run)) << 32 | static_cast<uint32_t>(step));
         // P's columns are free once P.V of this warpgroup's previous tile is done.
         if (step >= 2 && !warp_wait(SPLASH_KBAR(pv_done, buf), ((step - 2) >> 1) & 1, ctx, kCSiteSmxP, step)) { ok = false; break; }
         const float shift = m_run == -INFINITY ? 0.f : -m_run;
@@ -1062,8 +1109,6 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         if (!group_sync()) { ok = false; break; }
       }
       step0 += n;
-      seq += 2 * n;
-      aux0 += n;
     }
     // Units whose rows see no key stand nowhere in the line: zeros.
     for (int e = blockIdx.x; ok && e < a.batch * a.row_tiles; e += gridDim.x) {
