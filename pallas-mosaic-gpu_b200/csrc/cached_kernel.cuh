@@ -24,9 +24,9 @@
 //   * q * 2^-eq = q1 + q2 (+ q3 for f16), each term what the ones before leave; S sums their products.  bf16 has 8 bits,
 //     a term 4: nothing is lost but below 2^-18 of the row's largest number.
 //   * 2^ek of a key scales its column of S; 2^ev of a value scales its column of P, and the running maximum is one of
-//     s + ev and lags behind by a factor of 2 at most, so that the scaled probabilities end between 128 and 256.
-//   * P = p1 + p2 with p1, p2 e4m3: 8 bits as a bf16 P has, down to 2^-10 of the row's largest scaled probability; below
-//     that the steps stay at 2^-17 of it.
+//     s + ev and lags behind by a factor of 8 at most, so that the scaled probabilities end between 32 and 256.
+//   * P = p1 + p2 with p1, p2 e4m3: 8 bits as a bf16 P has, down to 2^-7 of the row's largest scaled probability; below
+//     that the steps stay at 2^-14 of it or less.
 #pragma once
 
 #include <stddef.h>
@@ -753,8 +753,10 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     const float unit = a.soft_cap > 0.f ? a.soft_cap : 1.f;
     const float unit2 = unit * kCachedLog2e;
     const float inv_cap = a.soft_cap > 0.f ? 1.f / a.soft_cap : 1.f;
-    constexpr float kThreshold = QUANT ? 1.f : 8.f;          // powers of 2 by which the maximum may lag behind
-    constexpr float kPScale = QUANT ? 128.f : 1.f;           // 8 bit: P up to 2 * 128 of e4m3's 448
+    // Powers of 2 by which the maximum may lag behind before O is rescaled, which takes about a tile's time.  8 bit: with a
+    // lag of 2^1 every third tile rescales (32 x 64 heads, 2000 to 32768 keys: 272 us), with 2^3 hardly one.
+    constexpr float kThreshold = QUANT ? 3.f : 8.f;
+    constexpr float kPScale = QUANT ? 32.f : 1.f;            // 8 bit: P up to 2^3 * 32 of e4m3's 448
     uint32_t sync_par = 0;
     int step0 = 0;   // tiles of the CTA in front of the segment
     bool ok = true;

@@ -2,7 +2,7 @@
 
 Bars, per number of the result, with p the softmax weights and A = sum_j p_j |v_j|:
   * P is rounded once (16 bits: half a step h, bf16 2^-8, f16 2^-11; 8-bit caches: two terms of e4m3, 2^-4 * 2^-4, and below
-    their range half a step of the subnormals, 2^-10 where the largest 2^ev p is 128 or more, times the codes of the values),
+    their range half a step of the subnormals, 2^-10 where the largest 2^ev p is 32 or more, times the codes of the values),
     the result once (h);
   * the scores are off by dS = 2^-19 sum|q k| + 2^-10 |s| under a soft-cap (tanh.approx) and, 8 bit, 2^-17 max|q| sum|k| (the
     e4m3 terms of q), which moves p by at most 2 dS relative to itself for dS < 0.1; 2^-12 A covers 32-bit sums and ex2.approx.
@@ -69,7 +69,7 @@ def _want(q, k, v, codes, exps, seen, cap):
   low = torch.zeros_like(a)
   if codes is not None:
     top = (p * exps[:, None]).amax(-1, keepdim=True)
-    low = 2.0 ** -17 * top * (seen.double() @ torch.where(seen.any(1)[..., None], codes, 0.0))
+    low = 2.0 ** -15 * top * (seen.double() @ torch.where(seen.any(1)[..., None], codes, 0.0))
   return (x.view(h, n, -1) for x in (out, a, low)), lse.view(h, n), ds.view(h, n), any_seen.view(h, n)
 
 
