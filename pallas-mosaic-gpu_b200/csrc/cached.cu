@@ -1,6 +1,6 @@
 // Entry points of the attention over a paged cache, and its second pass.
 #include "cached_dispatch.h"
-#include "cached_kernel.cuh"
+#include "cached_common.cuh"
 #include "host_common.cuh"
 
 namespace splash {
@@ -97,17 +97,18 @@ static int check_cached(const SplashCachedParams* p) {
   if (capacity >= (1ll << 30)) return fail(SPLASH_INVALID_ARGUMENT, "a page table may hold at most 2^30 tokens");
   if (rows >= (1ll << 30) || static_cast<int64_t>(p->batch) * p->kv_heads * rows >= limit)
     return fail(SPLASH_INVALID_ARGUMENT, "batch * heads * new tokens must fit in 31 bits");
-  const int64_t units = (rows + 31) / 32 * p->batch * p->kv_heads;
+  const int64_t units = (rows + 7) / 8 * p->batch * p->kv_heads;
   if (units * (capacity / kCachedTile + 2 + kCachedUnitCost) >= limit)
     return fail(SPLASH_INVALID_ARGUMENT, "batch * kv heads * tiles of rows * tiles of keys must fit in 31 bits");
   return SPLASH_OK;
 }
 
-// Rows per tile: as few as hold the call's, since the other copies of few rows share the softmax (see the kernel).
+// Rows per tile: as few as hold the call's.  Up to 16 take the kernel whose MMA rows are keys (cached_few_kernel.cuh), the
+// others the one with copies of the rows.
 static CachedPlan cached_plan(const SplashCachedParams& p) {
   CachedPlan plan;
   const int64_t rows = static_cast<int64_t>(p.heads / p.kv_heads) * p.n;
-  plan.row_cap = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  plan.row_cap = rows <= 8 && p.quantized ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   plan.row_tiles = static_cast<int>((rows + plan.row_cap - 1) / plan.row_cap);
   const int64_t entries = static_cast<int64_t>(p.batch) * plan.row_tiles;
   const int64_t capacity = static_cast<int64_t>(p.table_width) * p.page_size;

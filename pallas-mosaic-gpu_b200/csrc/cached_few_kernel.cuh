@@ -1,0 +1,621 @@
+// Attention over a paged cache for few rows: up to 16 new tokens x heads of a kv head, as in token-by-token decoding.
+//
+// cached_kernel.cuh spends an MMA's 128 rows on copies of the few rows there are, and its products then take as long as an
+// 8-bit tile's transfer.  Here the keys are the 128 rows instead:
+//   S^T = K Q^T       [128 keys x rows]        A = K as it lies in the cache, B = Q, 16 to 48 columns
+//   O^T += V^T P^T    [head_dim x rows]        A = V^T (V read M-major), B = P^T, which a key's thread writes as 16 or 32 bytes
+// An MMA costs its 4 KB of A, 32 cycles: 256 a tile of either type, where the copies cost 1024.  A thread has one key and all
+// rows: the scales of an 8-bit key and value are two numbers of its own, and no exponential is computed twice.
+//
+// The rows' maxima lie across the threads now.  They are not looked for: a thread compares its scores with the lagging maxima
+// (registers, the same in every thread of a warpgroup), and only if one of the warpgroup's threads is above by 2^lag do the
+// four warps reduce, agree on new maxima and rescale their warpgroup's O.  The two warpgroups take the tiles in turn, each
+// with maxima, sums and O of its own, joined at the end of a segment.
+//
+// 8 bit: Q is 2 (bf16) or 3 (f16) e4m3 terms side by side in B, whose columns of S are added; P is two terms, p1 + p2 / 16,
+// side by side as well, whose columns of O are added with that factor.
+#pragma once
+
+#include "cached_common.cuh"
+
+namespace splash {
+
+template <int D, bool BF16, bool QUANT, int R>
+struct CachedFewLayout {
+  static constexpr int kRows = R;
+  static constexpr int kTerms = QUANT ? (BF16 ? 2 : 3) : 1;
+  static constexpr int kSCols = (kTerms * R + 15) / 16 * 16;  // N of the scores: a multiple of 16
+  static constexpr int kOCols = (QUANT ? 2 : 1) * R;          // N of P V
+  static_assert(kOCols % 16 == 0, "");
+  static constexpr int kItem = QUANT ? 1 : 2;
+  static constexpr int kRowBytes = D * kItem;
+  static constexpr int kBoxBytes = kRowBytes < 128 ? kRowBytes : 128;
+  static constexpr int kBoxes = kRowBytes / kBoxBytes;
+  static constexpr int kBoxElems = kBoxBytes / kItem;
+  static constexpr int kSlotBytes = kCachedTile * kRowBytes;
+  static constexpr int kQBox = kSCols * kBoxBytes;            // rows of all terms, one box of their numbers
+  static constexpr int kQBytes = kBoxes * kQBox;
+  // P^T of a warpgroup: core matrices of 8 keys x 16 bytes, keys one after the other, 16 bytes of rows beside one another
+  // 2 KB apart.
+  static constexpr int kPBlocks = kOCols * kItem / 16;
+  static constexpr int kPBlock = kCachedTile * 16;
+  static constexpr int kPBytes = kPBlocks * kPBlock;
+  static constexpr int kBarBytes = 512;
+  static constexpr int kAuxBytes = QUANT ? kCachedAuxSlots * 2 * kCachedTile : 0;
+  static constexpr int kQScaleBytes = QUANT ? 2 * R * 4 : 0;
+  static constexpr int kVoteBytes = 2 * 2 * 16;               // by warpgroup and parity of its tiles: a word per warp
+  static constexpr int kMaxBytes = 8 * R * 4;                 // per warp: maxima of its keys
+  static constexpr int kSumBytes = 2 * (8 + 2) * R * 4;       // by parity of the segment: sums per warp, maxima per warpgroup
+  static constexpr int kRowInfoBytes = 8 * R * 16;            // per warp: what each row sees
+  static constexpr int kTreeBytes = kCachedMaxTree * 8 + 2 * kCachedMaxTree * 8 * 4;
+  static constexpr int kFixed = 1024 + (kQBytes + 1023) / 1024 * 1024 + 2 * kPBytes + kBarBytes + kAuxBytes + kQScaleBytes + kVoteBytes +
+                                kMaxBytes + kSumBytes + kRowInfoBytes + kTreeBytes;
+  static constexpr int kSlotsFit = (227 * 1024 - kFixed) / (2 * kSlotBytes);
+  static constexpr int kSlots = kSlotsFit < kCachedMaxSlots ? kSlotsFit : kCachedMaxSlots;
+  static constexpr int kSmem = kFixed + 2 * kSlots * kSlotBytes;
+  // Tensor memory: four buffers of scores, O of the two warpgroups.
+  static constexpr int kOCol = 4 * kSCols;
+  static constexpr int kTmemCols = 256;
+  static_assert(kOCol + 2 * kOCols <= kTmemCols, "");
+  static constexpr int kSoftmaxRegs = 184, kLoadRegs = 136;   // 384 * 168 = 256 * 184 + 128 * 136
+};
+
+// N columns of a lane.
+template <int N>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t addr, uint32_t* r) {
+  if constexpr (N == 16) tmem_ld16(addr, r);
+  else if constexpr (N == 32) tmem_ld32(addr, r);
+  else { tmem_ld32(addr, r); tmem_ld16(addr + 32, r + 32); }
+}
+
+template <int D, bool BF16, bool QUANT, int R>
+__global__ void __launch_bounds__(kCachedThreads, 1)
+cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v, const CachedArgs a) {
+  using L = CachedFewLayout<D, BF16, QUANT, R>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t q_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t k_u32 = q_u32 + (L::kQBytes + 1023) / 1024 * 1024;
+  const uint32_t v_u32 = k_u32 + L::kSlots * L::kSlotBytes;
+  const uint32_t p_u32 = v_u32 + L::kSlots * L::kSlotBytes;
+  const uint32_t bars_u32 = p_u32 + 2 * L::kPBytes;
+  const uint32_t aux_u32 = bars_u32 + L::kBarBytes;
+  const uint32_t vote_u32 = aux_u32 + L::kAuxBytes;
+  const uint32_t qscale_u32 = vote_u32 + L::kVoteBytes;
+  const uint32_t max_u32 = qscale_u32 + L::kQScaleBytes;
+  const uint32_t sum_u32 = max_u32 + L::kMaxBytes;
+  const uint32_t info_u32 = sum_u32 + L::kSumBytes;
+  const uint32_t parents_u32 = info_u32 + L::kRowInfoBytes;
+  const uint32_t trees_u32 = parents_u32 + 2 * kCachedMaxTree * 4;
+
+  const int warp = uniform_warp_index();
+  const int lane = threadIdx.x & 31;
+  const WaitCtx ctx{SPLASH_KWORD(abort_flag)};
+
+  if (warp == 8) {
+    cached_init_barriers(bars_u32, lane);
+    if (lane == 0) {
+      launch_dependents();
+      sts32(SPLASH_KWORD(abort_flag), 0);
+      sts32(SPLASH_KWORD(dead), a.status[0] != 0);
+      prefetch_tensormap(&tm_k);
+      prefetch_tensormap(&tm_v);
+      if (!QUANT) prefetch_tensormap(&tm_q);
+    }
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  } else if (warp == 9) {
+    tmem_alloc(SPLASH_KWORD(tmem_base), L::kTmemCols);
+    tmem_relinquish();
+  } else if (warp == 10) {
+    // No votes yet; and zeros in rows of Q that no term fills (the scores' columns are a multiple of 16).
+    if (lane < L::kVoteBytes / 4) sts32(vote_u32 + lane * 4, 0xffffffffu);
+    for (int i = lane; i < L::kQBytes / 16; i += 32) sts128(q_u32 + i * 16, make_uint4(0, 0, 0, 0));
+    fence_proxy_async_smem();
+  } else if (warp == 0) {
+    cached_find_share(a, bars_u32, lane);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = lds32(SPLASH_KWORD(tmem_base));
+  if (lds32(SPLASH_KWORD(dead))) {
+    if (warp == 9) {
+      __syncwarp();
+      tmem_dealloc(tmem, L::kTmemCols);
+    }
+    return;
+  }
+  CachedCursor cur;
+  cur.start(a, lds32(SPLASH_KWORD(first_entry)), lds32(SPLASH_KWORD(first_head)), lds32(SPLASH_KWORD(first_offset)),
+            lds32(SPLASH_KWORD(share)));
+
+  if (warp >= 8) {
+    setmaxnreg_dec<L::kLoadRegs>();
+    if (warp == 8 || warp == 11) {
+      // ------------------------------------------ loads: keys (and Q, and exponents), values ----------------------------
+      const bool is_v = warp == 11;
+      cached_load<L, QUANT>(a, cur, bars_u32, is_v ? v_u32 : k_u32, aux_u32, is_v ? &tm_v : &tm_k, is_v, lane, ctx, [&](int b, int rt, int head) {
+        if (elect_one()) {
+          const int row = (b * a.kv_heads + head) * a.rows + rt * R;
+          mbar_arrive_expect_tx(SPLASH_KBAR(q_full, 0), L::kQBytes);
+#pragma unroll
+          for (int c = 0; c < L::kBoxes; ++c) tma_load_2d(q_u32 + c * L::kQBox, &tm_q, c * L::kBoxElems, row, SPLASH_KBAR(q_full, 0));
+        }
+      });
+    } else if (warp == 9) {
+      // ------------------------------------------ products -----------------------------------------------------------
+      constexpr uint32_t kHi = cached_desc_hi<L::kBoxBytes>();
+      constexpr uint32_t kPHi = desc_hi_plain(L::kPBlock);  // M/N-major without swizzle: blocks of 16 bytes, 2 KB apart
+      constexpr uint32_t kIdescS = make_idesc(BF16 && !QUANT, 128, L::kSCols, false, false);
+      constexpr uint32_t kIdescO = make_idesc(BF16 && !QUANT, 128, L::kOCols, true, true);
+      constexpr int kStepsPerBox = L::kBoxBytes / 32;  // an MMA takes 32 bytes of a key's numbers, or 16 / 32 keys
+      constexpr int kKeysPerMma = QUANT ? 32 : 16;
+      // V^T has 128 rows in two boxes, in one (e4m3), or at head_dim 64 one box of 64 rows twice, whose second half is not read.
+      constexpr uint32_t kVBox = L::kBoxes > 1 ? kCachedTile * L::kBoxBytes : 0;
+      struct Walk {
+        CachedCursor cur;
+        int seg, i, step;
+        bool on;
+        __device__ __forceinline__ void advance(const CachedArgs& a) {
+          ++step;
+          if (++i == cur.seg_n) {
+            i = 0;
+            ++seg;
+            on = cur.next(a);
+          }
+        }
+      };
+      const bool any = cur.next(a);
+      Walk qk{cur, 0, 0, 0, any}, pv = qk;
+      uint32_t spins = 0;
+      uint64_t t0 = 0;
+      while (qk.on || pv.on) {
+        bool issued = false;
+        if (pv.on) {
+          const int grp = pv.step & 1, slot = pv.step % L::kSlots;
+          const bool ready = mbar_probe(SPLASH_KBAR(p_ready, grp), (pv.step >> 1) & 1) &&
+                             mbar_probe(SPLASH_KBAR(v_full, slot), (pv.step / L::kSlots) & 1) &&
+                             // O may be written again once the previous segment's has been read.
+                             (pv.i > 0 || pv.seg == 0 || mbar_probe(SPLASH_KBAR(o_free, 0), (pv.seg - 1) & 1));
+          if (__all_sync(0xffffffffu, ready)) {
+            tc_fence_after();
+            const uint32_t a_lo = desc_lo(v_u32 + slot * L::kSlotBytes, kVBox);
+            const uint32_t b_lo = desc_lo_plain(p_u32 + grp * L::kPBytes, 128);
+            const uint32_t o_tmem = tmem + L::kOCol + grp * L::kOCols;
+#pragma unroll
+            for (int kk = 0; kk < kCachedTile / kKeysPerMma; ++kk) {
+              const uint32_t ao = (kk * kKeysPerMma * L::kBoxBytes) >> 4, bo = (kk * kKeysPerMma * 16) >> 4;
+              if constexpr (QUANT) umma8_ss2_w(o_tmem, a_lo + ao, kHi, b_lo + bo, kPHi, kIdescO, pv.i > 1 || kk > 0);
+              else umma_ss2_w(o_tmem, a_lo + ao, kHi, b_lo + bo, kPHi, kIdescO, pv.i > 1 || kk > 0);
+            }
+            umma_commit_w(SPLASH_KBAR(v_empty, slot));
+            umma_commit_w(SPLASH_KBAR(pv_done, grp));
+            pv.advance(a);
+            issued = true;
+          }
+        }
+        if (qk.on) {
+          const int buf = qk.step & 3, slot = qk.step % L::kSlots;
+          const bool ready = mbar_probe(SPLASH_KBAR(k_full, slot), (qk.step / L::kSlots) & 1) &&
+                             (qk.step < 4 || mbar_probe(SPLASH_KBAR(s_free, buf), ((qk.step - 4) >> 2) & 1)) &&
+                             (qk.i > 0 || mbar_probe(SPLASH_KBAR(q_full, 0), qk.seg & 1));
+          if (__all_sync(0xffffffffu, ready)) {
+            tc_fence_after();
+            const uint32_t a_lo = desc_lo(k_u32 + slot * L::kSlotBytes, 16), b_lo = desc_lo(q_u32, 16);
+#pragma unroll
+            for (int kk = 0; kk < L::kRowBytes / 32; ++kk) {
+              const uint32_t ao = ((kk / kStepsPerBox) * (kCachedTile * L::kBoxBytes) + (kk % kStepsPerBox) * 32) >> 4;
+              const uint32_t bo = ((kk / kStepsPerBox) * L::kQBox + (kk % kStepsPerBox) * 32) >> 4;
+              if constexpr (QUANT) umma8_ss2_w(tmem + buf * L::kSCols, a_lo + ao, kHi, b_lo + bo, kHi, kIdescS, kk > 0);
+              else umma_ss2_w(tmem + buf * L::kSCols, a_lo + ao, kHi, b_lo + bo, kHi, kIdescS, kk > 0);
+            }
+            umma_commit_w(SPLASH_KBAR(s_ready, buf));
+            umma_commit_w(SPLASH_KBAR(k_empty, slot));
+            if (qk.i + 1 == qk.cur.seg_n) umma_commit_w(SPLASH_KBAR(q_free, 0));
+            qk.advance(a);
+            issued = true;
+          }
+        }
+        // Bounded, as every wait: about a second without anything to issue.
+        if (issued) {
+          spins = 0;
+        } else if ((++spins & 0xff) == 0) {
+          const uint64_t now = global_timer_ns();
+          if (spins == 0x100) t0 = now;
+          bool give_up = lds32(SPLASH_KWORD(abort_flag)) != 0;
+          if (!give_up && now - t0 > kWaitLimitNs) {
+            sts32(SPLASH_KWORD(abort_flag), 0x80000000u | (static_cast<uint32_t>(kCSiteMmaFull) << 20) | (static_cast<uint32_t>(pv.step) & 0xfffffu));
+            give_up = true;
+          }
+          if (__any_sync(0xffffffffu, give_up)) break;
+        }
+      }
+    } else if (warp == 10 && (QUANT || a.parents != nullptr)) {
+      // ------------------------------ drafted trees, and Q as e4m3 terms, ahead of their use ------------------------------
+      int trees = 0, last = -1;
+      for (int seg = 0; cur.next(a); ++seg) {
+        const int b = cur.seg_entry / a.row_tiles, rt = cur.seg_entry - b * a.row_tiles;
+        if (a.parents != nullptr && b != last) {
+          last = b;
+          if (!cached_make_tree(a, b, cur.g.before, trees++, bars_u32, parents_u32, lane, ctx)) break;
+        }
+        if constexpr (QUANT) {
+          auto store = [&](int t, int r, uint32_t byte, uint32_t codes) {
+            sts_bytes<D / 32>(q_u32 + cached_swz<L::kBoxBytes>(t * R + r, byte >> 4) + (byte & 15u), codes);
+          };
+          if (!cached_split_q<D, BF16, L::kTerms, R>(a, seg, b, rt, cur.seg_head, bars_u32, qscale_u32, lane, ctx, store)) break;
+        }
+      }
+    }
+  } else {
+    // ============================================ softmax ==============================================================
+    setmaxnreg_inc<L::kSoftmaxRegs>();
+    if (threadIdx.x == 0) a.cuts[blockIdx.x] = make_int4(-1, 0, 0, 0);  // (its first segment overwrites it)
+    const int grp = warp >> 2, quarter = warp & 3;
+    const int key_lane = quarter * 32 + lane;   // key of a tile; row of O^T
+    const uint32_t tmem_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t o_tmem = tmem_lane + L::kOCol;
+    const uint32_t p_row = p_u32 + grp * L::kPBytes + key_lane * 16;
+    const uint32_t my_info = info_u32 + warp * (R * 16);
+    const int piece_shift = min(a.page_shift, 7);
+    const bool tree = a.parents != nullptr;
+    const bool capped = a.soft_cap > 0.f;
+    const float unit2 = (capped ? a.soft_cap : 1.f) * kCachedLog2e;
+    const float inv_cap = capped ? 1.f / a.soft_cap : 1.f;
+    // Powers of 2 by which the maximum may lag behind; 8 bit: P up to 2^3 * 32 of e4m3's 448.
+    constexpr float kThreshold = QUANT ? 3.f : 8.f;
+    constexpr float kPScale = QUANT ? 32.f : 1.f;
+    uint32_t sync_par = 0;
+    int step0 = 0;           // tiles of the CTA in front of the segment
+    int trees = 0, last_b = -1;
+    bool ok = true;
+    auto arrive = [&](uint32_t bar) {  // of a warp, for what all its lanes have done
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    auto group_sync = [&]() -> bool {
+      arrive(SPLASH_KBAR(sync, 0));
+      const bool fine = warp_wait(SPLASH_KBAR(sync, 0), sync_par, ctx, kCSiteSmxSync, 0);
+      sync_par ^= 1;
+      return fine;
+    };
+    // The four warps of a warpgroup on one question, asked once a tile and once more where the answer was yes: a word
+    // (ballot number, answer) per warp, of two sets in turn -- a warp is at most one ballot ahead of the slowest.
+    uint32_t ballots = 0;
+    auto vote = [&](bool yes, bool& any) -> bool {
+      const uint32_t set = vote_u32 + (grp * 2 + (ballots & 1)) * 16;
+      const uint32_t want = ballots & 0x7fffffffu;
+      ++ballots;
+      __syncwarp();
+      if (lane == 0) sts32(set + quarter * 4, want << 1 | (yes ? 1u : 0u));
+      uint64_t t0 = 0;
+      for (uint32_t spins = 0;; ++spins) {
+        uint64_t lo = lds64(set), hi = lds64(set + 8);
+        const uint32_t w0 = static_cast<uint32_t>(lo), w1 = static_cast<uint32_t>(lo >> 32), w2 = static_cast<uint32_t>(hi), w3 = static_cast<uint32_t>(hi >> 32);
+        const bool all = (w0 >> 1) == want && (w1 >> 1) == want && (w2 >> 1) == want && (w3 >> 1) == want;
+        if (__all_sync(0xffffffffu, all)) {
+          any = (w0 | w1 | w2 | w3) & 1u;
+          return true;
+        }
+        if ((spins & 0xff) == 0xff) {
+          const uint64_t now = global_timer_ns();
+          if (t0 == 0) t0 = now;
+          bool give_up = lds32(SPLASH_KWORD(abort_flag)) != 0;
+          if (!give_up && now - t0 > kWaitLimitNs) {
+            sts32(SPLASH_KWORD(abort_flag), 0x80000000u | (static_cast<uint32_t>(kCSiteSmxM) << 20));
+            give_up = true;
+          }
+          if (__any_sync(0xffffffffu, give_up)) return false;
+        }
+      }
+    };
+
+    for (int seg = 0; ok && cur.next(a); ++seg) {
+      const CachedGeom& g = cur.g;
+      const int n = cur.seg_n;
+      const int b = cur.seg_entry / a.row_tiles, rt = cur.seg_entry - b * a.row_tiles;
+      if (tree && b != last_b) {
+        if (last_b >= 0) arrive(SPLASH_KBAR(tree_free, (trees - 1) & 1));
+        last_b = b;
+        if (!warp_wait(SPLASH_KBAR(tree_full, trees & 1), (trees >> 1) & 1, ctx, kCSiteSmxTree, seg)) { ok = false; break; }
+        ++trees;
+      }
+      // What each row sees, a lane per row: keys [lo, hi) and [0, sink), and the words of its node in a tree.
+      __syncwarp();
+      uint32_t live = 0;  // bit r: row r is a new token's
+      {
+        const int row_all = rt * R + lane;
+        const int node = row_all % a.n;
+        const bool alive = lane < R && row_all < a.rows && node < g.count;
+        uint32_t above = 0;
+        int depth = node;
+        if (tree) {
+          above = trees_u32 + (((trees - 1) & 1) * kCachedMaxTree + node) * 32;
+          depth = static_cast<int>(lds32(above + 28));
+        }
+        const int position = g.before + depth;
+        const int v_hi = !alive ? 0 : (tree ? g.before : position + 1);
+        const int v_lo = a.window < 0 ? 0 : max(0, position - a.window);
+        const int v_sink = a.window < 0 ? 0 : min(a.sinks, v_hi);
+        if (lane < R)
+          sts128(my_info + lane * 16, make_uint4(v_lo, v_hi, v_sink, alive ? above : 0u));
+        live = __ballot_sync(0xffffffffu, alive);
+      }
+      __syncwarp();
+      const int seen_by_all = g.before + (tree ? 0 : g.i0 + 1);  // keys in front of this are behind no row
+      const int all_from = a.window < 0 ? 0 : g.before + g.i1 - 1 - a.window;
+      const int32_t* table = a.page_table + b * a.table_stride;
+      const int pages = kCachedTile >> piece_shift;
+      auto page_of = [&](int i) -> int {  // lane p: page id of piece p of tile i (anything for pieces nobody sees)
+        if (i >= n || lane >= pages) return 0;
+        const int key = cur.key0(i) + (lane << piece_shift);
+        int id = 0;  // (asked for here, whatever the compiler thinks of its use a tile later)
+        if (key < g.hi) asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(id) : "l"(table + (key >> a.page_shift)));
+        return id;
+      };
+      float m[R], l[R], mul[R];  // maxima (powers of 2; the same in every thread), this key's sums, score to powers of 2
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        mul[r] = (live >> r) & 1u ? unit2 : 0.f;  // rows that are none never call for new maxima
+      }
+      const int i0 = (grp ^ step0) & 1;  // the CTA's tiles alternate between the warpgroups, whatever segment they are of
+      int page = page_of(i0);
+
+      for (int i = i0; i < n; i += 2) {
+        const int step = step0 + i, buf = step & 3;
+        const int key0 = cur.key0(i), key = key0 + key_lane;
+        asm volatile("" : "+r"(page));  // looked at here and not where it was asked for, a tile ago
+        const uint32_t good = __ballot_sync(0xffffffffu, page >= 0 && page < a.num_pages);  // pieces that have a page
+        page = page_of(i + 2);
+        const bool plain = key0 + kCachedTile <= seen_by_all && (key0 >= all_from || key0 + kCachedTile <= g.sink_hi) &&
+                           good == 0xffffffffu;
+        // Whether this thread's key is there for some row; others may hold anything, and nothing was loaded for some.
+        const bool there = key < g.hi && (key >= g.lo || key < g.sink_hi) && ((good >> (key_lane >> piece_shift)) & 1u);
+        if (!warp_wait(SPLASH_KBAR(s_ready, buf), (step >> 2) & 1, ctx, kCSiteSmxS, step)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t raw[L::kSCols];
+        tmem_ld_cols<L::kSCols>(tmem_lane + buf * L::kSCols, raw);
+        float k_scale = 1.f, v_exp = 0.f, v_scale = kPScale;
+        if constexpr (QUANT) {
+          // The key's own scales.  (The exponents came with the keys, for which the scores waited.)
+          if (i == i0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              const float q_scale = __uint_as_float(lds32(qscale_u32 + ((seg & 1) * R + r) * 4));
+              mul[r] *= capped ? 1.f : q_scale;
+            }
+          }
+          if (there) {
+            const uint32_t x = aux_u32 + (step % kCachedAuxSlots) * (2 * kCachedTile) + key_lane;
+            const int ek = lds_s8(x), ev = lds_s8(x + kCachedTile);
+            k_scale = exponent_scale(ek);
+            v_exp = static_cast<float>(ev);
+            v_scale = exponent_scale(ev) * kPScale;
+          }
+        }
+        tmem_wait_ld();
+        tc_fence_before();
+        arrive(SPLASH_KBAR(s_free, buf));  // the scores of tile step + 4 may come
+        float x[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          x[r] = __uint_as_float(raw[r]);
+          if constexpr (QUANT) {
+#pragma unroll
+            for (int t = 1; t < L::kTerms; ++t) x[r] += __uint_as_float(raw[t * R + r]);
+            x[r] *= k_scale;
+          }
+        }
+        if (__builtin_expect(capped, 0)) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            float to_cap = inv_cap;
+            if constexpr (QUANT) to_cap *= __uint_as_float(lds32(qscale_u32 + ((seg & 1) * R + r) * 4));
+            x[r] = tanh_approx(x[r] * to_cap);
+          }
+        }
+        if (__builtin_expect(!plain, 0)) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const uint4 info = lds128(my_info + r * 16);
+            bool seen = (key >= static_cast<int>(info.x) && key < static_cast<int>(info.y)) || key < static_cast<int>(info.z);
+            const int d = key - g.before;
+            if (info.w != 0 && d >= 0 && d < kCachedMaxTree) seen = seen || ((lds32(info.w + (1 + (d >> 5)) * 4) >> (d & 31)) & 1u);
+            if (!seen || !there) x[r] = -INFINITY;
+          }
+          // Values that no row sees are cleared: their probability is 0, and 0 times what lies there may be NaN.
+          const uint32_t clear = __ballot_sync(0xffffffffu, !there);
+          if (clear) {
+            // (P V of tile step - 2 is over: so is the previous use of the slot, without which its parity says nothing.)
+            const int slot = step % L::kSlots;
+            if ((step >= 2 && !warp_wait(SPLASH_KBAR(pv_done, grp), ((step - 2) >> 1) & 1, ctx, kCSiteSmxP, step)) ||
+                !warp_wait(SPLASH_KBAR(v_full, slot), (step / L::kSlots) & 1, ctx, kCSiteSmxV, step)) { ok = false; break; }
+            // The warp's 32 rows of the tile, 32 pieces of 16 bytes at a time.
+            constexpr int kChunks = L::kBoxBytes / 16, kAtOnce = 32 / kChunks;
+            const uint32_t dst = v_u32 + slot * L::kSlotBytes + quarter * 32 * L::kBoxBytes + (lane % kChunks) * 16;
+#pragma unroll 1
+            for (int k = lane / kChunks; k < 32; k += kAtOnce)
+              if ((clear >> k) & 1u)
+#pragma unroll
+                for (int c = 0; c < L::kBoxes; ++c)
+                  sts128(dst + c * (kCachedTile * L::kBoxBytes) + k * L::kBoxBytes, make_uint4(0, 0, 0, 0));
+          }
+        }
+        // ---- does a score stand above the maxima by more than they may lag? ----
+        bool above = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) above = above || fmaf(x[r], mul[r], v_exp) > m[r] + kThreshold;  // (-inf + lag is -inf)
+        bool move;
+        if (!vote(__any_sync(0xffffffffu, above), move)) { ok = false; break; }
+        if (__builtin_expect(move, 0)) {
+          // New maxima where they are above by that much: of the warp by exchange, of the warpgroup through shared memory.
+          const uint32_t mine = max_u32 + warp * (R * 4);
+          float top[R];
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            top[r] = fmaf(x[r], mul[r], v_exp);
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], d));
+            if (lane == 0) sts32(mine + r * 4, __float_as_uint(top[r]));
+          }
+          bool unused;
+          __threadfence_block();
+          if (!vote(false, unused)) { ok = false; break; }
+          __threadfence_block();
+          float alpha[R];
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            float t = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) t = fmaxf(t, __uint_as_float(lds32(max_u32 + ((grp * 4 + w) * R + r) * 4)));
+            alpha[r] = 1.f;
+            if (t > m[r] + kThreshold) {
+              alpha[r] = ex2_approx(m[r] - t);  // 0 when m was -inf
+              m[r] = t;
+              l[r] *= alpha[r];
+            }
+          }
+          if (i >= 2) {
+            // O may be touched once P V of this warpgroup's previous tile is done.
+            if (!warp_wait(SPLASH_KBAR(pv_done, grp), ((step - 2) >> 1) & 1, ctx, kCSiteSmxO, step)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t o[L::kOCols];
+            tmem_ld_cols<L::kOCols>(o_tmem + grp * L::kOCols, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < L::kOCols; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha[c % R]);
+            if constexpr (L::kOCols == 16) tmem_st16(o_tmem + grp * L::kOCols, o);
+            else tmem_st32(o_tmem + grp * L::kOCols, o);
+            tmem_wait_st();
+          }
+        }
+        // ---- P ----
+        uint32_t pk[L::kOCols * L::kItem / 4];
+#pragma unroll
+        for (int r = 0; r < R; r += 4) {
+          float p[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float shift = m[r + k] == -INFINITY ? 0.f : -m[r + k];
+            const float e = ex2_approx(fmaf(x[r + k], mul[r + k], shift));
+            l[r + k] += e;
+            p[k] = QUANT ? e * v_scale : e;
+          }
+          if constexpr (QUANT) {
+            // The first term is P rounded to four bits, in integer arithmetic: its code need not be read back.  The second
+            // is what is left, times 16.
+            const float2 a0 = make_float2(p[0], p[1]), a1 = make_float2(p[2], p[3]);
+            const float2 h0 = four_bits(a0), h1 = four_bits(a1);
+            const float2 r0 = mul2(sub2(a0, h0), make_float2(16.f, 16.f)), r1 = mul2(sub2(a1, h1), make_float2(16.f, 16.f));
+            pk[r / 4] = e4m3x2(h0.x, h0.y) | (e4m3x2(h1.x, h1.y) << 16);
+            pk[R / 4 + r / 4] = e4m3x2(r0.x, r0.y) | (e4m3x2(r1.x, r1.y) << 16);
+          } else {
+            pk[r / 2] = pack2<BF16>(p[0], p[1]);
+            pk[r / 2 + 1] = pack2<BF16>(p[2], p[3]);
+          }
+        }
+        // P's room is free once P V of this warpgroup's previous tile is done.
+        if (step >= 2 && !warp_wait(SPLASH_KBAR(pv_done, grp), ((step - 2) >> 1) & 1, ctx, kCSiteSmxP, step)) { ok = false; break; }
+#pragma unroll
+        for (int c = 0; c < L::kPBlocks; ++c)
+          sts128(p_row + c * L::kPBlock, make_uint4(pk[c * 4], pk[c * 4 + 1], pk[c * 4 + 2], pk[c * 4 + 3]));
+        fence_proxy_async_smem();
+        tc_fence_before();
+        arrive(SPLASH_KBAR(p_ready, grp));
+      }
+      if (!ok) break;
+
+      // ---- the parts of a row, added up: the sums of the keys, the two warpgroups ----
+      const uint32_t sums = sum_u32 + (seg & 1) * (10 * R * 4), maxima = sums + 8 * R * 4;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float s = l[r];
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
+        if (lane == 0) sts32(sums + (warp * R + r) * 4, __float_as_uint(s));
+        if (lane == 0 && quarter == 0) sts32(maxima + (grp * R + r) * 4, __float_as_uint(m[r]));
+      }
+      if (!group_sync()) { ok = false; break; }
+      // (Both warpgroups are past their tiles, so the barrier's phase before the last tile's is over.)
+      const int last = step0 + n - 1;
+      if (!warp_wait(SPLASH_KBAR(pv_done, last & 1), (last >> 1) & 1, ctx, kCSiteSmxDone, last)) { ok = false; break; }
+      tc_fence_after();
+      const bool whole = cur.whole;
+      const bool has[2] = {n > 1 || !(step0 & 1), n > 1 || (step0 & 1)};  // which warpgroups had a tile
+      uint32_t o0[L::kOCols], o1[L::kOCols];
+      if (has[0]) tmem_ld_cols<L::kOCols>(o_tmem, o0);
+      if (has[1]) tmem_ld_cols<L::kOCols>(o_tmem + L::kOCols, o1);
+      tmem_wait_ld();
+      tc_fence_before();
+      arrive(SPLASH_KBAR(o_free, 0));
+      const long long out_row0 = static_cast<long long>(b * a.kv_heads + cur.seg_head) * a.rows + rt * R;
+      const long long part0 = static_cast<long long>(2 * blockIdx.x + (seg > 0)) * R;
+      if (seg == 0 && threadIdx.x == 0) a.cuts[blockIdx.x] = make_int4(cur.seg_entry, cur.seg_head, cur.seg_tile, g.tiles);
+      // Warpgroup g writes its half of the rows, a thread one number of each.
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if ((r >= R / 2) != (grp == 1) || rt * R + r >= a.rows) continue;
+        const float m0 = __uint_as_float(lds32(maxima + r * 4)), m1 = __uint_as_float(lds32(maxima + (R + r) * 4));
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          l0 += __uint_as_float(lds32(sums + (w * R + r) * 4));
+          l1 += __uint_as_float(lds32(sums + ((4 + w) * R + r) * 4));
+        }
+        const float m_tot = fmaxf(m0, m1);
+        // A warpgroup that met no key has nothing to add, but its sum if that is NaN.
+        float w0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - m_tot), w1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - m_tot);
+        const float l_tot = (l0 != 0.f ? (m0 == -INFINITY ? l0 : l0 * w0) : 0.f) + (l1 != 0.f ? (m1 == -INFINITY ? l1 : l1 * w1) : 0.f);
+        const bool is_live = (live >> r) & 1u;
+        float value = 0.f;
+        if (is_live) {
+          if (has[0]) {
+            float o = __uint_as_float(o0[r]);
+            if constexpr (QUANT) o = fmaf(__uint_as_float(o0[R + r]), 1.f / 16, o);
+            value = o * w0;
+          }
+          if (has[1]) {
+            float o = __uint_as_float(o1[r]);
+            if constexpr (QUANT) o = fmaf(__uint_as_float(o1[R + r]), 1.f / 16, o);
+            value = fmaf(o, w1, value);
+          }
+          value *= 1.f / kPScale;
+          if (l_tot != l_tot) value = l_tot;
+          else if (whole) value *= l_tot > 0.f ? 1.f / l_tot : 0.f;
+        }
+        if (!whole) {
+          if (key_lane < D) a.part_o[(part0 + r) * D + key_lane] = value;
+          if (key_lane == 0) a.part_ml[part0 + r] = make_float2(m_tot, l_tot);
+        } else {
+          if (key_lane < D)
+            static_cast<uint16_t*>(a.out)[(out_row0 + r) * D + key_lane] = static_cast<uint16_t>(pack2<BF16>(value, 0.f));
+          if (key_lane == 0 && a.lse_out)
+            a.lse_out[out_row0 + r] = is_live && l_tot != 0.f ? (m_tot + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
+        }
+      }
+      step0 += n;
+    }
+    // Units whose rows see no key stand nowhere in the line: zeros.
+    if (ok) cached_fill_unseen<D>(a, static_cast<int>(threadIdx.x));
+  }
+
+  // ---- teardown: every thread of every role ends up here ----
+  tc_fence_before();
+  __syncthreads();
+  if (const uint32_t gave_up = lds32(SPLASH_KWORD(abort_flag))) {
+    if (threadIdx.x == 0) report_abort(a.status, gave_up, a.status_host);
+    // Copies still in flight land before the shared memory goes to another CTA.
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000) {}
+  }
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, L::kTmemCols);
+  }
+}
+
+}  // namespace splash
