@@ -103,12 +103,12 @@ static int check_cached(const SplashCachedParams* p) {
   return SPLASH_OK;
 }
 
-// Rows per tile: as few as hold the call's.  Up to 16 take the kernel whose MMA rows are keys (cached_few_kernel.cuh), the
-// others the one with copies of the rows.
+// Rows per tile: as few as hold the call's.  Up to 8 rows over an 8-bit cache take the kernel whose MMA rows are keys
+// (cached_few_kernel.cuh; measured there), the others the one with copies of the rows.
 static CachedPlan cached_plan(const SplashCachedParams& p) {
   CachedPlan plan;
   const int64_t rows = static_cast<int64_t>(p.heads / p.kv_heads) * p.n;
-  plan.row_cap = rows <= 8 && p.quantized ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  plan.row_cap = rows <= 8 && p.quantized ? 8 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   plan.row_tiles = static_cast<int>((rows + plan.row_cap - 1) / plan.row_cap);
   const int64_t entries = static_cast<int64_t>(p.batch) * plan.row_tiles;
   const int64_t capacity = static_cast<int64_t>(p.table_width) * p.page_size;

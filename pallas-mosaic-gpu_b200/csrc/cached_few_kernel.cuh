@@ -1,48 +1,46 @@
-// Attention over a paged cache for few rows: up to 16 new tokens x heads of a kv head, as in token-by-token decoding.
+// Attention over an 8-bit paged cache for few rows: up to 8 new tokens x heads of a kv head, as in token-by-token decoding.
 //
-// cached_kernel.cuh spends an MMA's 128 rows on copies of the few rows there are, and its products then take as long as an
-// 8-bit tile's transfer.  Here the keys are the 128 rows instead:
-//   S^T = K Q^T       [128 keys x rows]        A = K as it lies in the cache, B = Q, 16 to 48 columns
-//   O^T += V^T P^T    [head_dim x rows]        A = V^T (V read M-major), B = P^T, which a key's thread writes as 16 or 32 bytes
-// An MMA costs its 4 KB of A, 32 cycles: 256 a tile of either type, where the copies cost 1024.  A thread has one key and all
-// rows: the scales of an 8-bit key and value are two numbers of its own, and no exponential is computed twice.
+// cached_kernel.cuh spends an MMA's 128 rows on copies of the few rows there are, and its products then take about as long as
+// an 8-bit tile's transfer (32 sequences of 2000 to 32768 keys, 64 / 8 heads: 278 us; here 196).  Here the keys are the 128
+// rows instead:
+//   S^T = K Q^T       [128 keys x rows]        A = K as it lies in the cache, B = Q, 16 or 24 columns
+//   O^T += V^T P^T    [head_dim x rows]        A = V^T (V read M-major), B = P^T, which a key's thread writes as 16 bytes
+// An MMA costs its 4 KB of A, 32 cycles: 256 a tile, where the copies cost 1024.  A thread has one key and all rows: the
+// scales of the key and its value are two numbers of its own, and no exponential is computed twice.
 //
 // The rows' maxima lie across the threads now.  They are not looked for: a thread compares its scores with the lagging maxima
 // (registers, the same in every thread of a warpgroup), and only if one of the warpgroup's threads is above by 2^lag do the
 // four warps reduce, agree on new maxima and rescale their warpgroup's O.  The two warpgroups take the tiles in turn, each
 // with maxima, sums and O of its own, joined at the end of a segment.
 //
-// 8 bit: Q is 2 (bf16) or 3 (f16) e4m3 terms side by side in B, whose columns of S are added; P is two terms, p1 + p2 / 16,
-// side by side as well, whose columns of O are added with that factor.
+// Q is 2 (bf16) or 3 (f16) e4m3 terms side by side in B, whose columns of S are added; P is two terms, p1 + p2 / 16, side by
+// side as well, whose columns of O are added with that factor.
+//
+// Not here: 16-bit caches, whose tiles take twice as long to arrive while the copies' products take no longer than here (192
+// us there, 203 here for 16 sequences of 4000 to 32768 keys, 32 / 8 heads); and 9 to 16 rows, whose state does not fit a
+// thread's registers (64 sequences of 300 to 32768 keys, windows of 4096, 16 rows: 123 us there, 204 here).
 #pragma once
 
 #include "cached_common.cuh"
 
 namespace splash {
 
-template <int D, bool BF16, bool QUANT, int R>
+constexpr int kCachedFewRows = 8;
+
+template <int D, bool BF16>
 struct CachedFewLayout {
-  static constexpr int kRows = R;
-  static constexpr int kTerms = QUANT ? (BF16 ? 2 : 3) : 1;
+  static constexpr int R = kCachedFewRows;
+  static constexpr int kTerms = BF16 ? 2 : 3;
   static constexpr int kSCols = (kTerms * R + 15) / 16 * 16;  // N of the scores: a multiple of 16
-  static constexpr int kOCols = (QUANT ? 2 : 1) * R;          // N of P V
-  static_assert(kOCols % 16 == 0, "");
-  static constexpr int kItem = QUANT ? 1 : 2;
-  static constexpr int kRowBytes = D * kItem;
-  static constexpr int kBoxBytes = kRowBytes < 128 ? kRowBytes : 128;
-  static constexpr int kBoxes = kRowBytes / kBoxBytes;
-  static constexpr int kBoxElems = kBoxBytes / kItem;
+  static constexpr int kOCols = 2 * R;                        // N of P V
+  static_assert(kOCols == 16, "a key's probabilities are one row of a core matrix");
+  static constexpr int kItem = 1, kRowBytes = D, kBoxBytes = D, kBoxes = 1, kBoxElems = D;  // a key: one box of 64 or 128 bytes
   static constexpr int kSlotBytes = kCachedTile * kRowBytes;
-  static constexpr int kQBox = kSCols * kBoxBytes;            // rows of all terms, one box of their numbers
-  static constexpr int kQBytes = kBoxes * kQBox;
-  // P^T of a warpgroup: core matrices of 8 keys x 16 bytes, keys one after the other, 16 bytes of rows beside one another
-  // 2 KB apart.
-  static constexpr int kPBlocks = kOCols * kItem / 16;
-  static constexpr int kPBlock = kCachedTile * 16;
-  static constexpr int kPBytes = kPBlocks * kPBlock;
+  static constexpr int kQBytes = kSCols * D;
+  static constexpr int kPBytes = kCachedTile * kOCols;        // P^T: core matrices of 8 keys x 16 bytes, one after the other
   static constexpr int kBarBytes = 512;
-  static constexpr int kAuxBytes = QUANT ? kCachedAuxSlots * 2 * kCachedTile : 0;
-  static constexpr int kQScaleBytes = QUANT ? 2 * R * 4 : 0;
+  static constexpr int kAuxBytes = kCachedAuxSlots * 2 * kCachedTile;
+  static constexpr int kQScaleBytes = 2 * R * 4;
   static constexpr int kVoteBytes = 2 * 2 * 16;               // by warpgroup and parity of its tiles: a word per warp
   static constexpr int kMaxBytes = 8 * R * 4;                 // per warp: maxima of its keys
   static constexpr int kSumBytes = 2 * (8 + 2) * R * 4;       // by parity of the segment: sums per warp, maxima per warpgroup
@@ -60,19 +58,11 @@ struct CachedFewLayout {
   static constexpr int kSoftmaxRegs = 184, kLoadRegs = 136;   // 384 * 168 = 256 * 184 + 128 * 136
 };
 
-// N columns of a lane.
-template <int N>
-__device__ __forceinline__ void tmem_ld_cols(uint32_t addr, uint32_t* r) {
-  if constexpr (N == 16) tmem_ld16(addr, r);
-  else if constexpr (N == 32) tmem_ld32(addr, r);
-  else { tmem_ld32(addr, r); tmem_ld16(addr + 32, r + 32); }
-}
-
-template <int D, bool BF16, bool QUANT, int R>
+template <int D, bool BF16>
 __global__ void __launch_bounds__(kCachedThreads, 1)
-cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                  const __grid_constant__ CUtensorMap tm_v, const CachedArgs a) {
-  using L = CachedFewLayout<D, BF16, QUANT, R>;
+cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const CachedArgs a) {
+  using L = CachedFewLayout<D, BF16>;
+  constexpr int R = L::R;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t q_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t k_u32 = q_u32 + (L::kQBytes + 1023) / 1024 * 1024;
@@ -100,7 +90,6 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       sts32(SPLASH_KWORD(dead), a.status[0] != 0);
       prefetch_tensormap(&tm_k);
       prefetch_tensormap(&tm_v);
-      if (!QUANT) prefetch_tensormap(&tm_q);
     }
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -133,26 +122,17 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   if (warp >= 8) {
     setmaxnreg_dec<L::kLoadRegs>();
     if (warp == 8 || warp == 11) {
-      // ------------------------------------------ loads: keys (and Q, and exponents), values ----------------------------
+      // ------------------------------------------ loads: keys (and exponents), values -----------------------------------
       const bool is_v = warp == 11;
-      cached_load<L, QUANT>(a, cur, bars_u32, is_v ? v_u32 : k_u32, aux_u32, is_v ? &tm_v : &tm_k, is_v, lane, ctx, [&](int b, int rt, int head) {
-        if (elect_one()) {
-          const int row = (b * a.kv_heads + head) * a.rows + rt * R;
-          mbar_arrive_expect_tx(SPLASH_KBAR(q_full, 0), L::kQBytes);
-#pragma unroll
-          for (int c = 0; c < L::kBoxes; ++c) tma_load_2d(q_u32 + c * L::kQBox, &tm_q, c * L::kBoxElems, row, SPLASH_KBAR(q_full, 0));
-        }
-      });
+      cached_load<L, true>(a, cur, bars_u32, is_v ? v_u32 : k_u32, aux_u32, is_v ? &tm_v : &tm_k, is_v, lane, ctx, [](int, int, int) {});
     } else if (warp == 9) {
       // ------------------------------------------ products -----------------------------------------------------------
       constexpr uint32_t kHi = cached_desc_hi<L::kBoxBytes>();
-      constexpr uint32_t kPHi = desc_hi_plain(L::kPBlock);  // M/N-major without swizzle: blocks of 16 bytes, 2 KB apart
-      constexpr uint32_t kIdescS = make_idesc(BF16 && !QUANT, 128, L::kSCols, false, false);
-      constexpr uint32_t kIdescO = make_idesc(BF16 && !QUANT, 128, L::kOCols, true, true);
-      constexpr int kStepsPerBox = L::kBoxBytes / 32;  // an MMA takes 32 bytes of a key's numbers, or 16 / 32 keys
-      constexpr int kKeysPerMma = QUANT ? 32 : 16;
-      // V^T has 128 rows in two boxes, in one (e4m3), or at head_dim 64 one box of 64 rows twice, whose second half is not read.
-      constexpr uint32_t kVBox = L::kBoxes > 1 ? kCachedTile * L::kBoxBytes : 0;
+      constexpr uint32_t kPHi = desc_hi_plain(L::kPBytes);  // N-major without swizzle; the one block of 16 rows has no next
+      constexpr uint32_t kIdescS = make_idesc(false, 128, L::kSCols, false, false);
+      constexpr uint32_t kIdescO = make_idesc(false, 128, L::kOCols, true, true);
+      // An MMA takes 32 of a key's numbers, or 32 keys.  V^T has 128 rows; at head_dim 64 they are the 64 of its box twice, whose
+      // second half is not read (distance 0 from one box to the next).
       struct Walk {
         CachedCursor cur;
         int seg, i, step;
@@ -180,15 +160,12 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                              (pv.i > 0 || pv.seg == 0 || mbar_probe(SPLASH_KBAR(o_free, 0), (pv.seg - 1) & 1));
           if (__all_sync(0xffffffffu, ready)) {
             tc_fence_after();
-            const uint32_t a_lo = desc_lo(v_u32 + slot * L::kSlotBytes, kVBox);
+            const uint32_t a_lo = desc_lo(v_u32 + slot * L::kSlotBytes, 0);
             const uint32_t b_lo = desc_lo_plain(p_u32 + grp * L::kPBytes, 128);
             const uint32_t o_tmem = tmem + L::kOCol + grp * L::kOCols;
 #pragma unroll
-            for (int kk = 0; kk < kCachedTile / kKeysPerMma; ++kk) {
-              const uint32_t ao = (kk * kKeysPerMma * L::kBoxBytes) >> 4, bo = (kk * kKeysPerMma * 16) >> 4;
-              if constexpr (QUANT) umma8_ss2_w(o_tmem, a_lo + ao, kHi, b_lo + bo, kPHi, kIdescO, pv.i > 1 || kk > 0);
-              else umma_ss2_w(o_tmem, a_lo + ao, kHi, b_lo + bo, kPHi, kIdescO, pv.i > 1 || kk > 0);
-            }
+            for (int kk = 0; kk < kCachedTile / 32; ++kk)
+              umma8_ss2_w(o_tmem, a_lo + ((kk * 32 * D) >> 4), kHi, b_lo + ((kk * 32 * 16) >> 4), kPHi, kIdescO, pv.i > 1 || kk > 0);
             umma_commit_w(SPLASH_KBAR(v_empty, slot));
             umma_commit_w(SPLASH_KBAR(pv_done, grp));
             pv.advance(a);
@@ -204,12 +181,8 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             tc_fence_after();
             const uint32_t a_lo = desc_lo(k_u32 + slot * L::kSlotBytes, 16), b_lo = desc_lo(q_u32, 16);
 #pragma unroll
-            for (int kk = 0; kk < L::kRowBytes / 32; ++kk) {
-              const uint32_t ao = ((kk / kStepsPerBox) * (kCachedTile * L::kBoxBytes) + (kk % kStepsPerBox) * 32) >> 4;
-              const uint32_t bo = ((kk / kStepsPerBox) * L::kQBox + (kk % kStepsPerBox) * 32) >> 4;
-              if constexpr (QUANT) umma8_ss2_w(tmem + buf * L::kSCols, a_lo + ao, kHi, b_lo + bo, kHi, kIdescS, kk > 0);
-              else umma_ss2_w(tmem + buf * L::kSCols, a_lo + ao, kHi, b_lo + bo, kHi, kIdescS, kk > 0);
-            }
+            for (int kk = 0; kk < D / 32; ++kk)
+              umma8_ss2_w(tmem + buf * L::kSCols, a_lo + kk * 2, kHi, b_lo + kk * 2, kHi, kIdescS, kk > 0);
             umma_commit_w(SPLASH_KBAR(s_ready, buf));
             umma_commit_w(SPLASH_KBAR(k_empty, slot));
             if (qk.i + 1 == qk.cur.seg_n) umma_commit_w(SPLASH_KBAR(q_free, 0));
@@ -231,7 +204,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           if (__any_sync(0xffffffffu, give_up)) break;
         }
       }
-    } else if (warp == 10 && (QUANT || a.parents != nullptr)) {
+    } else if (warp == 10) {
       // ------------------------------ drafted trees, and Q as e4m3 terms, ahead of their use ------------------------------
       int trees = 0, last = -1;
       for (int seg = 0; cur.next(a); ++seg) {
@@ -240,12 +213,10 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           last = b;
           if (!cached_make_tree(a, b, cur.g.before, trees++, bars_u32, parents_u32, lane, ctx)) break;
         }
-        if constexpr (QUANT) {
-          auto store = [&](int t, int r, uint32_t byte, uint32_t codes) {
-            sts_bytes<D / 32>(q_u32 + cached_swz<L::kBoxBytes>(t * R + r, byte >> 4) + (byte & 15u), codes);
-          };
-          if (!cached_split_q<D, BF16, L::kTerms, R>(a, seg, b, rt, cur.seg_head, bars_u32, qscale_u32, lane, ctx, store)) break;
-        }
+        auto store = [&](int t, int r, uint32_t byte, uint32_t codes) {
+          sts_bytes<D / 32>(q_u32 + cached_swz<L::kBoxBytes>(t * R + r, byte >> 4) + (byte & 15u), codes);
+        };
+        if (!cached_split_q<D, BF16, L::kTerms, R>(a, seg, b, rt, cur.seg_head, bars_u32, qscale_u32, lane, ctx, store)) break;
       }
     }
   } else {
@@ -261,11 +232,10 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int piece_shift = min(a.page_shift, 7);
     const bool tree = a.parents != nullptr;
     const bool capped = a.soft_cap > 0.f;
-    const float unit2 = (capped ? a.soft_cap : 1.f) * kCachedLog2e;
-    const float inv_cap = capped ? 1.f / a.soft_cap : 1.f;
-    // Powers of 2 by which the maximum may lag behind; 8 bit: P up to 2^3 * 32 of e4m3's 448.
-    constexpr float kThreshold = QUANT ? 3.f : 8.f;
-    constexpr float kPScale = QUANT ? 32.f : 1.f;
+    // What takes a score to powers of 2, or to the argument of the soft-cap and from there to powers of 2.
+    const float pre = capped ? 1.f / a.soft_cap : kCachedLog2e, post = a.soft_cap * kCachedLog2e;
+    constexpr float kThreshold = 3.f;  // powers of 2 by which the maxima may lag behind
+    constexpr float kPScale = 32.f;    // P up to 2^3 * 32 of e4m3's 448
     uint32_t sync_par = 0;
     int step0 = 0;           // tiles of the CTA in front of the segment
     int trees = 0, last_b = -1;
@@ -354,12 +324,12 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (key < g.hi) asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(id) : "l"(table + (key >> a.page_shift)));
         return id;
       };
-      float m[R], l[R], mul[R];  // maxima (powers of 2; the same in every thread), this key's sums, score to powers of 2
+      float m[R], l[R], mul[R];  // maxima of s + ev (powers of 2; the same in every thread), this key's sums, factor of a row
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         m[r] = -INFINITY;
         l[r] = 0.f;
-        mul[r] = (live >> r) & 1u ? unit2 : 0.f;  // rows that are none never call for new maxima
+        mul[r] = 0.f;
       }
       const int i0 = (grp ^ step0) & 1;  // the CTA's tiles alternate between the warpgroups, whatever segment they are of
       int page = page_of(i0);
@@ -377,45 +347,36 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (!warp_wait(SPLASH_KBAR(s_ready, buf), (step >> 2) & 1, ctx, kCSiteSmxS, step)) { ok = false; break; }
         tc_fence_after();
         uint32_t raw[L::kSCols];
-        tmem_ld_cols<L::kSCols>(tmem_lane + buf * L::kSCols, raw);
+        tmem_ld16(tmem_lane + buf * L::kSCols, raw);
+        if constexpr (L::kSCols == 32) tmem_ld16(tmem_lane + buf * L::kSCols + 16, raw + 16);
         float k_scale = 1.f, v_exp = 0.f, v_scale = kPScale;
-        if constexpr (QUANT) {
-          // The key's own scales.  (The exponents came with the keys, for which the scores waited.)
-          if (i == i0) {
+        // The key's own scales, and once the rows'.  (The exponents came with the keys, for which the scores waited.)
+        if (i == i0) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-              const float q_scale = __uint_as_float(lds32(qscale_u32 + ((seg & 1) * R + r) * 4));
-              mul[r] *= capped ? 1.f : q_scale;
-            }
-          }
-          if (there) {
-            const uint32_t x = aux_u32 + (step % kCachedAuxSlots) * (2 * kCachedTile) + key_lane;
-            const int ek = lds_s8(x), ev = lds_s8(x + kCachedTile);
-            k_scale = exponent_scale(ek);
-            v_exp = static_cast<float>(ev);
-            v_scale = exponent_scale(ev) * kPScale;
-          }
+          for (int r = 0; r < R; ++r)  // rows that are none have factor 0 and never call for new maxima
+            if ((live >> r) & 1u) mul[r] = pre * __uint_as_float(lds32(qscale_u32 + ((seg & 1) * R + r) * 4));
+        }
+        if (there) {
+          const uint32_t at = aux_u32 + (step % kCachedAuxSlots) * (2 * kCachedTile) + key_lane;
+          const int ek = lds_s8(at), ev = lds_s8(at + kCachedTile);
+          k_scale = exponent_scale(ek);
+          v_exp = static_cast<float>(ev);
+          v_scale = exponent_scale(ev) * kPScale;
         }
         tmem_wait_ld();
         tc_fence_before();
         arrive(SPLASH_KBAR(s_free, buf));  // the scores of tile step + 4 may come
-        float x[R];
+        float x[R];  // scores in powers of 2
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           x[r] = __uint_as_float(raw[r]);
-          if constexpr (QUANT) {
 #pragma unroll
-            for (int t = 1; t < L::kTerms; ++t) x[r] += __uint_as_float(raw[t * R + r]);
-            x[r] *= k_scale;
-          }
+          for (int t = 1; t < L::kTerms; ++t) x[r] += __uint_as_float(raw[t * R + r]);
+          x[r] *= k_scale * mul[r];
         }
         if (__builtin_expect(capped, 0)) {
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            float to_cap = inv_cap;
-            if constexpr (QUANT) to_cap *= __uint_as_float(lds32(qscale_u32 + ((seg & 1) * R + r) * 4));
-            x[r] = tanh_approx(x[r] * to_cap);
-          }
+          for (int r = 0; r < R; ++r) x[r] = tanh_approx(x[r]) * post;
         }
         if (__builtin_expect(!plain, 0)) {
 #pragma unroll
@@ -447,24 +408,26 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         // ---- does a score stand above the maxima by more than they may lag? ----
         bool above = false;
 #pragma unroll
-        for (int r = 0; r < R; ++r) above = above || fmaf(x[r], mul[r], v_exp) > m[r] + kThreshold;  // (-inf + lag is -inf)
+        for (int r = 0; r < R; ++r) above = above || x[r] + v_exp > m[r] + kThreshold;  // (-inf + lag is -inf)
         bool move;
         if (!vote(__any_sync(0xffffffffu, above), move)) { ok = false; break; }
         if (__builtin_expect(move, 0)) {
           // New maxima where they are above by that much: of the warp by exchange, of the warpgroup through shared memory.
           const uint32_t mine = max_u32 + warp * (R * 4);
-          float top[R];
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            top[r] = fmaf(x[r], mul[r], v_exp);
-#pragma unroll
-            for (int d = 16; d > 0; d /= 2) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], d));
-            if (lane == 0) sts32(mine + r * 4, __float_as_uint(top[r]));
+            // Floats that order like integers, for the one instruction that takes a maximum over a warp.
+            const int bits = __float_as_int(x[r] + v_exp);
+            const int top = __reduce_max_sync(0xffffffffu, bits ^ ((bits >> 31) & 0x7fffffff));
+            if (lane == 0) sts32(mine + r * 4, static_cast<uint32_t>(top ^ ((top >> 31) & 0x7fffffff)));
           }
           bool unused;
           __threadfence_block();
           if (!vote(false, unused)) { ok = false; break; }
           __threadfence_block();
+          // O may be touched once P V of this warpgroup's previous tile is done.
+          if (i >= 2 && !warp_wait(SPLASH_KBAR(pv_done, grp), ((step - 2) >> 1) & 1, ctx, kCSiteSmxO, step)) { ok = false; break; }
+          tc_fence_after();
           float alpha[R];
 #pragma unroll
           for (int r = 0; r < R; ++r) {
@@ -479,49 +442,38 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
           }
           if (i >= 2) {
-            // O may be touched once P V of this warpgroup's previous tile is done.
-            if (!warp_wait(SPLASH_KBAR(pv_done, grp), ((step - 2) >> 1) & 1, ctx, kCSiteSmxO, step)) { ok = false; break; }
-            tc_fence_after();
             uint32_t o[L::kOCols];
-            tmem_ld_cols<L::kOCols>(o_tmem + grp * L::kOCols, o);
+            tmem_ld16(o_tmem + grp * L::kOCols, o);
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < L::kOCols; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha[c % R]);
-            if constexpr (L::kOCols == 16) tmem_st16(o_tmem + grp * L::kOCols, o);
-            else tmem_st32(o_tmem + grp * L::kOCols, o);
+            tmem_st16(o_tmem + grp * L::kOCols, o);
             tmem_wait_st();
           }
         }
         // ---- P ----
-        uint32_t pk[L::kOCols * L::kItem / 4];
+        uint32_t pk[L::kOCols / 4];
 #pragma unroll
         for (int r = 0; r < R; r += 4) {
           float p[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const float shift = m[r + k] == -INFINITY ? 0.f : -m[r + k];
-            const float e = ex2_approx(fmaf(x[r + k], mul[r + k], shift));
+            const float e = ex2_approx(x[r + k] + shift);
             l[r + k] += e;
-            p[k] = QUANT ? e * v_scale : e;
+            p[k] = e * v_scale;
           }
-          if constexpr (QUANT) {
-            // The first term is P rounded to four bits, in integer arithmetic: its code need not be read back.  The second
-            // is what is left, times 16.
-            const float2 a0 = make_float2(p[0], p[1]), a1 = make_float2(p[2], p[3]);
-            const float2 h0 = four_bits(a0), h1 = four_bits(a1);
-            const float2 r0 = mul2(sub2(a0, h0), make_float2(16.f, 16.f)), r1 = mul2(sub2(a1, h1), make_float2(16.f, 16.f));
-            pk[r / 4] = e4m3x2(h0.x, h0.y) | (e4m3x2(h1.x, h1.y) << 16);
-            pk[R / 4 + r / 4] = e4m3x2(r0.x, r0.y) | (e4m3x2(r1.x, r1.y) << 16);
-          } else {
-            pk[r / 2] = pack2<BF16>(p[0], p[1]);
-            pk[r / 2 + 1] = pack2<BF16>(p[2], p[3]);
-          }
+          // The first term is P rounded to four bits, in integer arithmetic: its code need not be read back.  The second is
+          // what is left, times 16.
+          const float2 a0 = make_float2(p[0], p[1]), a1 = make_float2(p[2], p[3]);
+          const float2 h0 = four_bits(a0), h1 = four_bits(a1);
+          const float2 r0 = mul2(sub2(a0, h0), make_float2(16.f, 16.f)), r1 = mul2(sub2(a1, h1), make_float2(16.f, 16.f));
+          pk[r / 4] = e4m3x2(h0.x, h0.y) | (e4m3x2(h1.x, h1.y) << 16);
+          pk[R / 4 + r / 4] = e4m3x2(r0.x, r0.y) | (e4m3x2(r1.x, r1.y) << 16);
         }
         // P's room is free once P V of this warpgroup's previous tile is done.
         if (step >= 2 && !warp_wait(SPLASH_KBAR(pv_done, grp), ((step - 2) >> 1) & 1, ctx, kCSiteSmxP, step)) { ok = false; break; }
-#pragma unroll
-        for (int c = 0; c < L::kPBlocks; ++c)
-          sts128(p_row + c * L::kPBlock, make_uint4(pk[c * 4], pk[c * 4 + 1], pk[c * 4 + 2], pk[c * 4 + 3]));
+        sts128(p_row, make_uint4(pk[0], pk[1], pk[2], pk[3]));
         fence_proxy_async_smem();
         tc_fence_before();
         arrive(SPLASH_KBAR(p_ready, grp));
@@ -530,13 +482,24 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
       // ---- the parts of a row, added up: the sums of the keys, the two warpgroups ----
       const uint32_t sums = sum_u32 + (seg & 1) * (10 * R * 4), maxima = sums + 8 * R * 4;
+      {
+        // Sums over the warp's keys: the lanes halve the rows between them until each has one, lane / (32 / R).
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float s = l[r];
+        for (int s = 1; s < R; s *= 2) {
+          const bool upper = lane & (16 / s);
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-        if (lane == 0) sts32(sums + (warp * R + r) * 4, __float_as_uint(s));
-        if (lane == 0 && quarter == 0) sts32(maxima + (grp * R + r) * 4, __float_as_uint(m[r]));
+          for (int k = 0; k < R / 2 / s; ++k) {
+            const float low = l[k], high = l[k + R / 2 / s];
+            l[k] = (upper ? high : low) + __shfl_xor_sync(0xffffffffu, upper ? low : high, 16 / s);
+          }
+        }
+#pragma unroll
+        for (int d = 16 / R; d > 0; d /= 2) l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
+        if ((lane & (32 / R - 1)) == 0) sts32(sums + (warp * R + lane / (32 / R)) * 4, __float_as_uint(l[0]));
+      }
+      if (quarter == 0 && lane == 0) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) sts32(maxima + (grp * R + r) * 4, __float_as_uint(m[r]));
       }
       if (!group_sync()) { ok = false; break; }
       // (Both warpgroups are past their tiles, so the barrier's phase before the last tile's is over.)
@@ -546,18 +509,18 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const bool whole = cur.whole;
       const bool has[2] = {n > 1 || !(step0 & 1), n > 1 || (step0 & 1)};  // which warpgroups had a tile
       uint32_t o0[L::kOCols], o1[L::kOCols];
-      if (has[0]) tmem_ld_cols<L::kOCols>(o_tmem, o0);
-      if (has[1]) tmem_ld_cols<L::kOCols>(o_tmem + L::kOCols, o1);
+      if (has[0]) tmem_ld16(o_tmem, o0);
+      if (has[1]) tmem_ld16(o_tmem + L::kOCols, o1);
       tmem_wait_ld();
       tc_fence_before();
       arrive(SPLASH_KBAR(o_free, 0));
       const long long out_row0 = static_cast<long long>(b * a.kv_heads + cur.seg_head) * a.rows + rt * R;
       const long long part0 = static_cast<long long>(2 * blockIdx.x + (seg > 0)) * R;
       if (seg == 0 && threadIdx.x == 0) a.cuts[blockIdx.x] = make_int4(cur.seg_entry, cur.seg_head, cur.seg_tile, g.tiles);
-      // Warpgroup g writes its half of the rows, a thread one number of each.
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if ((r >= R / 2) != (grp == 1) || rt * R + r >= a.rows) continue;
+      // Lane r: what the warpgroups' numbers of row r count for.
+      float m_tot, l_tot, w0, w1;
+      {
+        const int r = lane % R;
         const float m0 = __uint_as_float(lds32(maxima + r * 4)), m1 = __uint_as_float(lds32(maxima + (R + r) * 4));
         float l0 = 0.f, l1 = 0.f;
 #pragma unroll
@@ -565,36 +528,34 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           l0 += __uint_as_float(lds32(sums + (w * R + r) * 4));
           l1 += __uint_as_float(lds32(sums + ((4 + w) * R + r) * 4));
         }
-        const float m_tot = fmaxf(m0, m1);
+        m_tot = fmaxf(m0, m1);
         // A warpgroup that met no key has nothing to add, but its sum if that is NaN.
-        float w0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - m_tot), w1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - m_tot);
-        const float l_tot = (l0 != 0.f ? (m0 == -INFINITY ? l0 : l0 * w0) : 0.f) + (l1 != 0.f ? (m1 == -INFINITY ? l1 : l1 * w1) : 0.f);
-        const bool is_live = (live >> r) & 1u;
+        w0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - m_tot);
+        w1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - m_tot);
+        l_tot = (l0 != 0.f ? (m0 == -INFINITY ? l0 : l0 * w0) : 0.f) + (l1 != 0.f ? (m1 == -INFINITY ? l1 : l1 * w1) : 0.f);
+        const float scale = l_tot != l_tot ? l_tot : (whole ? (l_tot > 0.f ? 1.f / l_tot : 0.f) : 1.f) / kPScale;
+        w0 *= scale;
+        w1 *= scale;
+        if (l_tot != l_tot) w0 = w1 = l_tot;
+      }
+      // Warpgroup g writes its half of the rows, a thread one number of each.
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float w0_r = __shfl_sync(0xffffffffu, w0, r), w1_r = __shfl_sync(0xffffffffu, w1, r);
+        if ((r >= R / 2) != (grp == 1) || rt * R + r >= a.rows) continue;
         float value = 0.f;
-        if (is_live) {
-          if (has[0]) {
-            float o = __uint_as_float(o0[r]);
-            if constexpr (QUANT) o = fmaf(__uint_as_float(o0[R + r]), 1.f / 16, o);
-            value = o * w0;
-          }
-          if (has[1]) {
-            float o = __uint_as_float(o1[r]);
-            if constexpr (QUANT) o = fmaf(__uint_as_float(o1[R + r]), 1.f / 16, o);
-            value = fmaf(o, w1, value);
-          }
-          value *= 1.f / kPScale;
-          if (l_tot != l_tot) value = l_tot;
-          else if (whole) value *= l_tot > 0.f ? 1.f / l_tot : 0.f;
+        if ((live >> r) & 1u) {
+          if (has[0]) value = fmaf(__uint_as_float(o0[R + r]), 1.f / 16, __uint_as_float(o0[r])) * w0_r;
+          if (has[1]) value = fmaf(fmaf(__uint_as_float(o1[R + r]), 1.f / 16, __uint_as_float(o1[r])), w1_r, value);
         }
-        if (!whole) {
-          if (key_lane < D) a.part_o[(part0 + r) * D + key_lane] = value;
-          if (key_lane == 0) a.part_ml[part0 + r] = make_float2(m_tot, l_tot);
-        } else {
-          if (key_lane < D)
-            static_cast<uint16_t*>(a.out)[(out_row0 + r) * D + key_lane] = static_cast<uint16_t>(pack2<BF16>(value, 0.f));
-          if (key_lane == 0 && a.lse_out)
-            a.lse_out[out_row0 + r] = is_live && l_tot != 0.f ? (m_tot + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
-        }
+        if (key_lane >= D) continue;
+        if (!whole) a.part_o[(part0 + r) * D + key_lane] = value;
+        else static_cast<uint16_t*>(a.out)[(out_row0 + r) * D + key_lane] = static_cast<uint16_t>(pack2<BF16>(value, 0.f));
+      }
+      if (warp == 0 && lane < R && rt * R + lane < a.rows) {
+        if (!whole) a.part_ml[part0 + lane] = make_float2(m_tot, l_tot);
+        else if (a.lse_out)
+          a.lse_out[out_row0 + lane] = ((live >> lane) & 1u) && l_tot != 0.f ? (m_tot + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
       }
       step0 += n;
     }
