@@ -109,6 +109,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   tc_fence_after();
   const uint32_t tmem = lds32(SPLASH_KWORD(tmem_base));
   if (lds32(SPLASH_KWORD(dead))) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) repeat_abort(a.status, a.status_host);
     if (warp == 9) {
       __syncwarp();
       tmem_dealloc(tmem, L::kTmemCols);

@@ -114,6 +114,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem = lds32(SPLASH_KWORD(tmem_base));
   if (lds32(SPLASH_KWORD(dead))) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) repeat_abort(a.status, a.status_host);
     if (warp == 9) {
       __syncwarp();
       tmem_dealloc(tmem, 512);

@@ -149,6 +149,17 @@ __device__ __forceinline__ void report_abort(int* status, uint32_t word, volatil
   __threadfence();
 }
 
+// A kernel that returns at entry because an earlier one gave up: one thread of the grid tells the host, which the earlier one
+// may not have been able to (null then).
+__device__ __forceinline__ void repeat_abort(const int* status, volatile int* host) {
+  if (!host) return;
+  host[1] = status[1];
+  host[2] = status[2];
+  host[3] = status[3];
+  __threadfence_system();
+  host[0] = status[0];
+}
+
 // Whole-warp wait with a warp-uniform verdict, for warps that go on to execute
 // .sync.aligned instructions (tcgen05.ld/st): either every lane continues or none.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const WaitCtx& ctx, int site, int step) {

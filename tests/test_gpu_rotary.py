@@ -163,3 +163,20 @@ def test_gpu_rotary_refusals():
                      ((q, k, p.cpu()), ValueError), ((q, k[:1], p), ValueError), ((q[:, :0], k, p), ValueError)):
     with pytest.raises(error):
       plan(*bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pairing", ["half", "adjacent"])
+def test_gpu_rotary_gradient_is_the_transpose(pairing):
+  """The rotation is linear: differences along unit vectors are its matrix, whose transpose the gradient applies.  Either is one
+  product per number here, rounded once."""
+  d = 64
+  plan = sa.make_rotary(d, (8, 24), pairing=pairing, q_scale=0.37)
+  eye = torch.eye(d, device=DEV, dtype=torch.bfloat16).view(1, 1, d, d)
+  positions = torch.tensor([[17], [900]], device=DEV, dtype=torch.int32).expand(2, d)  # one place for all
+  zero = torch.zeros_like(eye)
+  forward = plan(eye, None, positions).double() - plan(zero, None, positions).double()
+  leaf = zero.clone().requires_grad_(True)
+  backward, = torch.autograd.grad(plan(leaf, None, positions), leaf, eye)
+  off = (backward[0, 0].double() - forward[0, 0].T).abs()
+  assert (off <= 2 * 2.0 ** -8 * forward[0, 0].T.abs() + 2.0 ** -20).all()

@@ -59,3 +59,22 @@ def test_masks_with_other_sinks_differ():
   np.testing.assert_array_equal(info.mask_descriptors[:, 3], [0, 4])
   with pytest.raises(ValueError, match="num_sinks"):
     sa.LocalMask((256, 256), (64, 0), num_sinks=-1)
+
+
+def test_formula_of_the_gradients_against_differences():
+  """The formula that the kernels' gradients are held against, windows and sinks included, shared heads too."""
+  import torch
+  from oracle import dense_attention
+  h, kvh, s, d = 4, 2, 12, 8
+  mask = np.asarray(sa.LocalMask((s, s), (3, 0), 0, num_sinks=2)[:, :])[None]
+  g = torch.Generator().manual_seed(0)
+  q, k, v, do = (torch.randn(1, x, s, d, generator=g, dtype=torch.float64) for x in (h, kvh, kvh, h))
+  grads = dense_attention.attention_backward(mask, q, k, v, do, None)
+  loss = lambda *x: float((dense_attention.attention_forward(mask, *x, None)[0] * do.numpy()).sum())
+  for i, grad in enumerate(grads):
+    u = torch.randn((q, k, v)[i].shape, generator=g, dtype=torch.float64)
+    step = 2.0 ** -6
+    at = lambda t: loss(*(x + t * u if j == i else x for j, x in enumerate((q, k, v))))
+    slope = (8 * (at(step) - at(-step)) - (at(2 * step) - at(-2 * step))) / (12 * step)
+    # 32-bit sums: 2^-24 of about 400 terms of size 1, over the step; the difference itself is off by step^4 f^(5) / 30.
+    assert abs(slope - float((torch.as_tensor(grad) * u).sum())) < 400 * 2.0 ** -24 * 12 / step + step ** 4 * 400
