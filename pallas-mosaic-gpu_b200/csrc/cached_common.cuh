@@ -13,9 +13,11 @@ constexpr int kCachedThreads = 384;
 constexpr int kCachedTile = 128;        // keys per tile
 constexpr int kCachedMaxSlots = 6;      // of the K ring, and of the V ring
 constexpr int kCachedAuxSlots = 16;     // exponents of a tile; more than tiles can be on their way (see the producer)
+// Lengths of segments on their way from the warp that loads the keys to P V, which is at most 14 tiles behind: the ring, and
+// the scores that the softmax lets be ahead of P V (it writes no P before that of its previous tile was used).
+constexpr int kCachedSegRing = 16;
 constexpr int kCachedMaxTree = 128;     // nodes of a drafted tree
-// What a unit costs besides its tiles, in tiles (its start, and the sum of its parts): it stands that much longer in the line.
-constexpr int kCachedUnitCost = 2;
+constexpr int kCachedMostUnitCost = 8;  // (see cached_plan)
 constexpr float kCachedLog2e = 1.4426950408889634f;
 constexpr float kCachedLn2 = 0.6931471805599453f;
 
@@ -36,6 +38,7 @@ struct CachedArgs {
   float2* part_ml;    // [2 * CTAs, R]: maximum (powers of 2) and sum
   int64_t table_stride, parents_stride;
   int32_t batch, heads, kv_heads, n, rows, row_tiles, row_cap;  // rows = heads / kv_heads * n
+  int32_t unit_cost;  // what a unit costs besides its tiles, in tiles: it stands that much longer in the line
   int32_t num_pages, page_shift, table_width;  // pages of 2^page_shift tokens
   int32_t window, sinks;  // window < 0: none
   float mask_value, soft_cap;
@@ -99,10 +102,10 @@ struct CachedCursor {
           g = cached_geom(a, entry);
         } while (g.tiles == 0);
       }
-      const int from = max(offset - kCachedUnitCost, 0), to = min(offset + left - kCachedUnitCost, g.tiles);
+      const int from = max(offset - a.unit_cost, 0), to = min(offset + left - a.unit_cost, g.tiles);
       seg_entry = entry;
       seg_head = head;
-      left -= g.tiles + kCachedUnitCost - offset;
+      left -= g.tiles + a.unit_cost - offset;
       offset = 0;
       ++head;
       if (to > from) {
@@ -136,6 +139,7 @@ struct CachedBarriers {
   uint64_t tree_full[2], tree_free[2];
   uint32_t tmem_base, abort_flag, dead;
   int32_t first_entry, first_head, first_offset, share;
+  int32_t seg_n[kCachedSegRing];
 };
 static_assert(sizeof(CachedBarriers) <= 512, "");
 
@@ -246,6 +250,27 @@ __device__ __forceinline__ int lds_s8(uint32_t addr) {
   (bars_u32 + static_cast<uint32_t>(offsetof(CachedBarriers, field)) + 8u * static_cast<uint32_t>(idx))
 #define SPLASH_KWORD(field) (bars_u32 + static_cast<uint32_t>(offsetof(CachedBarriers, field)))
 
+// A walk of the warp that issues the products, over the CTA's tiles; there are two, the scores' and P V's.  `step`: tiles so far,
+// which give buffers, ring slots and parities.  The segments' lengths come from the warp that loads the keys, which is ahead (a
+// cursor of its own would cost registers that this warp does not have).
+struct CachedWalk {
+  int seg = 0, i = 0, step = 0, n = 0;
+  __device__ __forceinline__ void at_tile(uint32_t bars_u32) {  // once the tile's keys have come
+    if (i == 0) n = static_cast<int>(lds32(SPLASH_KWORD(seg_n) + (seg % kCachedSegRing) * 4));
+  }
+  __device__ __forceinline__ void advance() {
+    ++step;
+    if (++i == n) {
+      i = 0;
+      ++seg;
+    }
+  }
+};
+__device__ __forceinline__ int cached_share_tiles(const CachedArgs& a, CachedCursor cur) {
+  int tiles = 0;
+  while (cur.next(a)) tiles += cur.seg_n;
+  return tiles;
+}
 
 // ---- what the warps of both kernels have in common ------------------------------------------------------------------
 // One warp: barriers.  The softmax warps arrive once each: 32 arrivals of a warp would be taken one after the other.
@@ -267,7 +292,7 @@ __device__ __forceinline__ void cached_find_share(const CachedArgs& a, uint32_t 
   auto line = [&](int e) -> int {  // what (sequence, row tile) e takes of the line, all kv heads
     if (e >= entries) return 0;
     const int tiles = cached_geom(a, e).tiles;
-    return tiles > 0 ? (tiles + kCachedUnitCost) * a.kv_heads : 0;
+    return tiles > 0 ? (tiles + a.unit_cost) * a.kv_heads : 0;
   };
   int total = 0;
   for (int e0 = 0; e0 < entries; e0 += 32) total += __reduce_add_sync(0xffffffffu, line(e0 + lane));
@@ -336,6 +361,7 @@ __device__ __forceinline__ void cached_load(const CachedArgs& a, CachedCursor cu
       if (seg > 0 && !warp_wait(SPLASH_KBAR(q_free, 0), (seg - 1) & 1, ctx, kCSiteLoadQ, seg)) return;
       load_q(b, rt, cur.seg_head);
     }
+    if (!is_v && lane == 0) sts32(SPLASH_KWORD(seg_n) + (seg % kCachedSegRing) * 4, static_cast<uint32_t>(cur.seg_n));
     const int32_t* table = a.page_table + b * a.table_stride;
     // This lane's piece of tile i: its page id, -1 where nobody sees it; asked for two tiles ahead of its use, so that
     // the load never waits for it.
@@ -389,6 +415,7 @@ __device__ __forceinline__ bool cached_make_tree(const CachedArgs& a, int b, int
   if (trees >= 2 && !warp_wait(SPLASH_KBAR(tree_free, buf), ((trees >> 1) & 1) ^ 1, ctx, kCSiteTree, trees)) return false;
   const uint32_t tree = trees_u32 + buf * (kCachedMaxTree * 32);
   constexpr int kPer = kCachedMaxTree / 32;
+  static_assert(kPer == 4, "");
   uint32_t bits[kPer][4];
   int up[kPer];
 #pragma unroll
@@ -404,7 +431,7 @@ __device__ __forceinline__ bool cached_make_tree(const CachedArgs& a, int b, int
     for (int w = 0; w < 8; ++w) sts32(tree + (i * 8 + w) * 4, w >= 1 && w <= 4 ? bits[j][w - 1] : 0u);
   }
   __syncwarp();
-  for (int steps = 1; steps < a.n; steps *= 2) {
+  while (__any_sync(0xffffffffu, (up[0] & up[1] & up[2] & up[3]) >= 0)) {  // (-1 in all: every chain is at its end)
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       if (up[j] < 0) continue;

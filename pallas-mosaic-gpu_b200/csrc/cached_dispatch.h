@@ -9,9 +9,9 @@ namespace splash {
 
 struct CachedArgs;
 
-// How a call is cut: rows per tile, tiles of rows per (sequence, kv head), CTAs, and where the workspace's parts begin.
+// How a call is cut: rows per tile, tiles of rows per (sequence, kv head), CTAs, cost of a unit in tiles, and where the workspace's parts begin.
 struct CachedPlan {
-  int row_cap, row_tiles, ctas;
+  int row_cap, row_tiles, ctas, unit_cost;
   int64_t part_o, part_ml, bytes;
 };
 

@@ -134,26 +134,13 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       constexpr uint32_t kIdescO = make_idesc(false, 128, L::kOCols, true, true);
       // An MMA takes 32 of a key's numbers, or 32 keys.  V^T has 128 rows; at head_dim 64 they are the 64 of its box twice, whose
       // second half is not read (distance 0 from one box to the next).
-      struct Walk {
-        CachedCursor cur;
-        int seg, i, step;
-        bool on;
-        __device__ __forceinline__ void advance(const CachedArgs& a) {
-          ++step;
-          if (++i == cur.seg_n) {
-            i = 0;
-            ++seg;
-            on = cur.next(a);
-          }
-        }
-      };
-      const bool any = cur.next(a);
-      Walk qk{cur, 0, 0, 0, any}, pv = qk;
+      const int tiles = cached_share_tiles(a, cur);
+      CachedWalk qk, pv;
       uint32_t spins = 0;
       uint64_t t0 = 0;
-      while (qk.on || pv.on) {
+      while (pv.step < tiles) {
         bool issued = false;
-        if (pv.on) {
+        {
           const int grp = pv.step & 1, slot = pv.step % L::kSlots;
           const bool ready = mbar_probe(SPLASH_KBAR(p_ready, grp), (pv.step >> 1) & 1) &&
                              mbar_probe(SPLASH_KBAR(v_full, slot), (pv.step / L::kSlots) & 1) &&
@@ -161,6 +148,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
                              (pv.i > 0 || pv.seg == 0 || mbar_probe(SPLASH_KBAR(o_free, 0), (pv.seg - 1) & 1));
           if (__all_sync(0xffffffffu, ready)) {
             tc_fence_after();
+            pv.at_tile(bars_u32);
             const uint32_t a_lo = desc_lo(v_u32 + slot * L::kSlotBytes, 0);
             const uint32_t b_lo = desc_lo_plain(p_u32 + grp * L::kPBytes, 128);
             const uint32_t o_tmem = tmem + L::kOCol + grp * L::kOCols;
@@ -169,25 +157,26 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               umma8_ss2_w(o_tmem, a_lo + ((kk * 32 * D) >> 4), kHi, b_lo + ((kk * 32 * 16) >> 4), kPHi, kIdescO, pv.i > 1 || kk > 0);
             umma_commit_w(SPLASH_KBAR(v_empty, slot));
             umma_commit_w(SPLASH_KBAR(pv_done, grp));
-            pv.advance(a);
+            pv.advance();
             issued = true;
           }
         }
-        if (qk.on) {
+        if (qk.step < tiles) {
           const int buf = qk.step & 3, slot = qk.step % L::kSlots;
           const bool ready = mbar_probe(SPLASH_KBAR(k_full, slot), (qk.step / L::kSlots) & 1) &&
                              (qk.step < 4 || mbar_probe(SPLASH_KBAR(s_free, buf), ((qk.step - 4) >> 2) & 1)) &&
                              (qk.i > 0 || mbar_probe(SPLASH_KBAR(q_full, 0), qk.seg & 1));
           if (__all_sync(0xffffffffu, ready)) {
             tc_fence_after();
+            qk.at_tile(bars_u32);
             const uint32_t a_lo = desc_lo(k_u32 + slot * L::kSlotBytes, 16), b_lo = desc_lo(q_u32, 16);
 #pragma unroll
             for (int kk = 0; kk < D / 32; ++kk)
               umma8_ss2_w(tmem + buf * L::kSCols, a_lo + kk * 2, kHi, b_lo + kk * 2, kHi, kIdescS, kk > 0);
             umma_commit_w(SPLASH_KBAR(s_ready, buf));
             umma_commit_w(SPLASH_KBAR(k_empty, slot));
-            if (qk.i + 1 == qk.cur.seg_n) umma_commit_w(SPLASH_KBAR(q_free, 0));
-            qk.advance(a);
+            if (qk.i + 1 == qk.n) umma_commit_w(SPLASH_KBAR(q_free, 0));
+            qk.advance();
             issued = true;
           }
         }

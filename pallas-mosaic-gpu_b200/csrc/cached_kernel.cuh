@@ -49,7 +49,7 @@ struct CachedLayout {
   static constexpr int kStageStride = 36;                  // words per row of the staging area (32 used)
   static constexpr int kStageBytes = 256 * kStageStride * 4;
   // Behind the staging area: maxima and sums, barriers, then (8 bit) exponents, scales, row scales, and the tree.
-  static constexpr int kMlBytes = 128 * 8 + 256 * 4;
+  static constexpr int kMlBytes = 128 * 8 + 2 * 256 * 4;
   static constexpr int kBarBytes = 512;
   static constexpr int kAuxBytes = QUANT ? kCachedAuxSlots * 2 * kCachedTile : 0;
   static constexpr int kScaleBytes = QUANT ? 8 * kKeys * 12 : 0;  // per warp: three numbers for each of its keys
@@ -147,34 +147,20 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       constexpr uint32_t kIdescQK = make_idesc(BF16 && !QUANT, 128, kCachedTile, false, false);
       constexpr uint32_t kIdescPV = make_idesc(BF16 && !QUANT, 128, D, false, true);
       constexpr int kStepsPerBox = L::kBoxBytes / 32;  // an MMA takes 32 bytes of K per row
-      // Two walks along the share, over tiles: the scores' and P V's.  `step`: tiles of the CTA so far, buffers by its lowest
-      // bit and parities by the next, ring slots by its remainder.
-      struct Walk {
-        CachedCursor cur;
-        int seg, i, step;
-        bool on;
-        __device__ __forceinline__ void advance(const CachedArgs& a) {
-          ++step;
-          if (++i == cur.seg_n) {
-            i = 0;
-            ++seg;
-            on = cur.next(a);
-          }
-        }
-      };
-      const bool any = cur.next(a);
-      Walk qk{cur, 0, 0, 0, any}, pv = qk;
+      const int tiles = cached_share_tiles(a, cur);
+      CachedWalk qk, pv;
       uint32_t spins = 0;
       uint64_t t0 = 0;
-      while (qk.on || pv.on) {
+      while (pv.step < tiles) {
         bool issued = false;
-        if (qk.on) {
+        if (qk.step < tiles) {
           const int buf = qk.step & 1, slot = qk.step % L::kSlots;
           const bool ready = mbar_probe(SPLASH_KBAR(k_full, slot), (qk.step / L::kSlots) & 1) &&
                              (qk.step < 2 || mbar_probe(SPLASH_KBAR(s_free, buf), ((qk.step - 2) >> 1) & 1)) &&
                              (qk.i > 0 || mbar_probe(SPLASH_KBAR(q_full, 0), qk.seg & 1));
           if (__all_sync(0xffffffffu, ready)) {
             tc_fence_after();
+            qk.at_tile(bars_u32);
             const uint32_t b_lo = desc_lo(k_u32 + slot * L::kSlotBytes, 16);
 #pragma unroll
             for (int t = 0; t < L::kTerms; ++t) {
@@ -188,12 +174,12 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             }
             umma_commit_w(SPLASH_KBAR(s_ready, buf));
             umma_commit_w(SPLASH_KBAR(k_empty, slot));
-            if (qk.i + 1 == qk.cur.seg_n) umma_commit_w(SPLASH_KBAR(q_free, 0));
-            qk.advance(a);
+            if (qk.i + 1 == qk.n) umma_commit_w(SPLASH_KBAR(q_free, 0));
+            qk.advance();
             issued = true;
           }
         }
-        if (pv.on) {
+        {
           const int buf = pv.step & 1, slot = pv.step % L::kSlots;
           const bool ready = mbar_probe(SPLASH_KBAR(p_ready, buf), (pv.step >> 1) & 1) &&
                              mbar_probe(SPLASH_KBAR(v_full, slot), (pv.step / L::kSlots) & 1) &&
@@ -201,6 +187,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
                              (pv.i > 0 || pv.seg == 0 || mbar_probe(SPLASH_KBAR(o_free, 0), (pv.seg - 1) & 1));
           if (__all_sync(0xffffffffu, ready)) {
             tc_fence_after();
+            pv.at_tile(bars_u32);
             const uint32_t b_lo = desc_lo(v_u32 + slot * L::kSlotBytes, kCachedTile * L::kBoxBytes);
             const uint32_t p_tmem = tmem + L::kPCol + buf * 64;
             constexpr int kKeysPerMma = QUANT ? 32 : 16;
@@ -213,7 +200,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             }
             umma_commit_w(SPLASH_KBAR(v_empty, slot));
             umma_commit_w(SPLASH_KBAR(pv_done, buf));
-            pv.advance(a);
+            pv.advance();
             issued = true;
           }
         }
@@ -262,7 +249,6 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     const uint32_t tmem_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t o_tmem = tmem_lane + L::kOCol;
     const uint32_t m_sh = ml_u32 + row_lane * 8;  // the latest tile of this row and copy, and the maximum after it
-    const uint32_t l_u32 = ml_u32 + 128 * 8;      // sums of the warpgroups, at the end
     // A lane's maximum after tile `step`, which its counterpart in the other warpgroup has left or will leave there.
     float m_got = 0.f;
     auto wait_m = [&](int step) -> bool {
@@ -308,6 +294,12 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       tmem_wait_st();
     }
     int trees = 0, last_b = -1;
+    bool tree_seen = false;
+    auto see_tree = [&](int seg) -> bool {  // of the trees so far, the last
+      const bool fine = tree_seen || warp_wait(SPLASH_KBAR(tree_full, (trees - 1) & 1), ((trees - 1) >> 1) & 1, ctx, kCSiteSmxTree, seg);
+      tree_seen = true;
+      return fine;
+    };
     auto arrive = [&](uint32_t bar) {  // of a warp, for what all its lanes have done
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
@@ -330,13 +322,21 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       uint32_t above = 0;  // the words of this row's node
       if (tree) {
         if (b != last_b) {
-          if (last_b >= 0) arrive(SPLASH_KBAR(tree_free, (trees - 1) & 1));
+          // (Also waited for if nobody looked at it: the barrier's parity tells a tree only from the one before.)
+          if (last_b >= 0) {
+            if (!see_tree(seg)) { ok = false; break; }
+            arrive(SPLASH_KBAR(tree_free, (trees - 1) & 1));
+          }
           last_b = b;
-          if (!warp_wait(SPLASH_KBAR(tree_full, trees & 1), (trees >> 1) & 1, ctx, kCSiteSmxTree, seg)) { ok = false; break; }
           ++trees;
+          tree_seen = false;
         }
         above = trees_u32 + (((trees - 1) & 1) * kCachedMaxTree + node) * 32;
-        depth = static_cast<int>(lds32(above + 28));
+        // Positions are only looked at for a window; without one the tree is, once its tiles come.
+        if (a.window >= 0) {
+          if (!see_tree(seg)) { ok = false; break; }
+          depth = static_cast<int>(lds32(above + 28));
+        }
       }
       // Keys of the context (tree) or of context and run that this row sees: [v_lo, v_hi) and [0, v_sink).
       const int position = g.before + depth;
@@ -424,6 +424,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           for (int j = 0; j < L::kKeys; ++j) sv[j] = tanh_approx(sv[j] * q_mul);
         }
         if (__builtin_expect(!plain, 0)) {
+          if (tree && !see_tree(seg)) { ok = false; break; }
 #pragma unroll
           for (int c = 0; c < L::kKeys / 32; ++c) {
             const int at = col0 + c * 32, kb = key0 + at;
@@ -572,15 +573,21 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           m_run = m_fin;
         }
       }
+      // Sums of the warpgroups, by parity of the segment: a warp that still reads them has not freed O, without which the next
+      // but one cannot end.
+      const uint32_t l_u32 = ml_u32 + 128 * 8 + (seg & 1) * (256 * 4);
       sts32(l_u32 + threadIdx.x * 4, __float_as_uint(l_run));
       if (!group_sync()) { ok = false; break; }
-      float m_tot = -INFINITY, l_tot = 0.f;
+      // (Maxima of other copies in shared memory: their next tile comes after the barriers of this epilogue.)
+      float m_tot = m_run, l_tot = 0.f;
+      if constexpr (KG > 1) {
 #pragma unroll
-      for (int src = 0; src < KG; ++src) m_tot = fmaxf(m_tot, __uint_as_float(lds32(ml_u32 + (src * L::kRows + r) * 8 + 4)));
+        for (int src = 0; src < KG; ++src) m_tot = fmaxf(m_tot, __uint_as_float(lds32(ml_u32 + (src * L::kRows + r) * 8 + 4)));
+      }
 #pragma unroll
       for (int src = 0; src < KG; ++src) {
         const uint32_t at = (src * L::kRows + r) * 4;
-        const float m = __uint_as_float(lds32(ml_u32 + 2 * at + 4));
+        const float m = KG > 1 ? __uint_as_float(lds32(ml_u32 + 2 * at + 4)) : m_run;
         const float l = __uint_as_float(lds32(l_u32 + at)) + __uint_as_float(lds32(l_u32 + 512 + at));
         if (l != 0.f) l_tot += m == -INFINITY ? l : l * ex2_approx(m - m_tot);
       }
@@ -601,7 +608,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           a.lse_out[out_row0 + r] = live && l_tot != 0.f ? (m_tot + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
       }
       // Each warpgroup has one half of O's columns, 32 at a time: every copy's lanes leave theirs, eight threads add up the 128
-      // bytes of a row.
+      // bytes of a row.  Rows without copies stay within their warp, which waits for no other.
       const int col = (threadIdx.x % 8) * 4;
       const uint32_t my_stage = stage_u32 + grp * (128 * L::kStageStride * 4);
 #pragma unroll 1
@@ -625,10 +632,14 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           }
           sts128(dst + k * 16, x);
         }
-        if (!group_sync()) { ok = false; break; }
+        if constexpr (KG > 1) {
+          if (!group_sync()) { ok = false; break; }
+        } else {
+          __syncwarp();
+        }
 #pragma unroll
-        for (int k = 0; k < L::kRows / 16; ++k) {
-          const int row = k * 16 + (threadIdx.x & 127) / 8;
+        for (int k = 0; k < 8 / KG; ++k) {
+          const int row = KG > 1 ? k * 16 + (threadIdx.x & 127) / 8 : (warp & 3) * 32 + k * 4 + lane / 8;
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int src = 0; src < KG; ++src) {
@@ -646,7 +657,11 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
                 make_uint2(pack2<BF16>(acc.x, acc.y), pack2<BF16>(acc.z, acc.w));
           }
         }
-        if (!group_sync()) { ok = false; break; }
+        if constexpr (KG > 1) {
+          if (!group_sync()) { ok = false; break; }
+        } else {
+          __syncwarp();
+        }
       }
       step0 += n;
     }
