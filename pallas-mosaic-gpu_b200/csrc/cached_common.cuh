@@ -240,6 +240,11 @@ __device__ __forceinline__ void sts_bytes(uint32_t addr, uint32_t v) {
   if constexpr (N == 4) sts32(addr, v);
   else asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(static_cast<uint16_t>(v)) : "memory");
 }
+// Numbers of four bits and below 2^13, to the steps of e4m3's subnormals where they are among those: what e4m3 holds of them.
+__device__ __forceinline__ float2 e4m3_steps(float2 x) {
+  const float2 c = make_float2(0x1.8p14f, 0x1.8p14f);  // its last bit is 2^-9
+  return sub2(add2(x, c), c);
+}
 __device__ __forceinline__ int lds_s8(uint32_t addr) {
   int v;
   asm volatile("ld.shared.s8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");

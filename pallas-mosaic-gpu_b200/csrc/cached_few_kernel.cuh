@@ -4,7 +4,7 @@
 // an 8-bit tile's transfer (32 sequences of 2000 to 32768 keys, 64 / 8 heads: 278 us; here 196).  Here the keys are the 128
 // rows instead:
 //   S^T = K Q^T       [128 keys x rows]        A = K as it lies in the cache, B = Q, 16 or 24 columns
-//   O^T += V^T P^T    [head_dim x rows]        A = V^T (V read M-major), B = P^T, which a key's thread writes as 16 bytes
+//   O^T += V^T P^T    [head_dim x rows]        A = V^T (V read M-major), B = P^T, which a key's thread writes as 16 bytes (f16: 32)
 // An MMA costs its 4 KB of A, 32 cycles: 256 a tile, where the copies cost 1024.  A thread has one key and all rows: the
 // scales of the key and its value are two numbers of its own, and no exponential is computed twice.
 //
@@ -13,8 +13,8 @@
 // four warps reduce, agree on new maxima and rescale their warpgroup's O.  The two warpgroups take the tiles in turn, each
 // with maxima, sums and O of its own, joined at the end of a segment.
 //
-// Q is 2 (bf16) or 3 (f16) e4m3 terms side by side in B, whose columns of S are added; P is two terms, p1 + p2 / 16, side by
-// side as well, whose columns of O are added with that factor.
+// Q is 2 (bf16) or 3 (f16) e4m3 terms side by side in B, whose columns of S are added; P is as many, p1 + p2 / 16 + p3 / 256,
+// side by side as well, whose columns of O are added with those factors.
 //
 // Not here: 16-bit caches, whose tiles take twice as long to arrive while the copies' products take no longer than here (192
 // us there, 203 here for 16 sequences of 4000 to 32768 keys, 32 / 8 heads); and 9 to 16 rows, whose state does not fit a
@@ -32,12 +32,14 @@ struct CachedFewLayout {
   static constexpr int R = kCachedFewRows;
   static constexpr int kTerms = BF16 ? 2 : 3;
   static constexpr int kSCols = (kTerms * R + 15) / 16 * 16;  // N of the scores: a multiple of 16
-  static constexpr int kOCols = 2 * R;                        // N of P V
-  static_assert(kOCols == 16, "a key's probabilities are one row of a core matrix");
+  static constexpr int kPTerms = BF16 ? 2 : 3;
+  static constexpr int kOCols = (kPTerms * R + 15) / 16 * 16;  // N of P V
   static constexpr int kItem = 1, kRowBytes = D, kBoxBytes = D, kBoxes = 1, kBoxElems = D;  // a key: one box of 64 or 128 bytes
   static constexpr int kSlotBytes = kCachedTile * kRowBytes;
   static constexpr int kQBytes = kSCols * D;
-  static constexpr int kPBytes = kCachedTile * kOCols;        // P^T: core matrices of 8 keys x 16 bytes, one after the other
+  // P^T: core matrices of 8 keys x 16 bytes one after the other, and 2 KB on the next 16 columns.
+  static constexpr int kPBlock = kCachedTile * 16;
+  static constexpr int kPBytes = kCachedTile * kOCols;
   static constexpr int kBarBytes = 512;
   static constexpr int kAuxBytes = kCachedAuxSlots * 2 * kCachedTile;
   static constexpr int kQScaleBytes = 2 * R * 4;
@@ -129,7 +131,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     } else if (warp == 9) {
       // ------------------------------------------ products -----------------------------------------------------------
       constexpr uint32_t kHi = cached_desc_hi<L::kBoxBytes>();
-      constexpr uint32_t kPHi = desc_hi_plain(L::kPBytes);  // N-major without swizzle; the one block of 16 rows has no next
+      constexpr uint32_t kPHi = desc_hi_plain(L::kPBlock);  // N-major without swizzle
       constexpr uint32_t kIdescS = make_idesc(false, 128, L::kSCols, false, false);
       constexpr uint32_t kIdescO = make_idesc(false, 128, L::kOCols, true, true);
       // An MMA takes 32 of a key's numbers, or 32 keys.  V^T has 128 rows; at head_dim 64 they are the 64 of its box twice, whose
@@ -433,16 +435,18 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           }
           if (i >= 2) {
             uint32_t o[L::kOCols];
-            tmem_ld16(o_tmem + grp * L::kOCols, o);
+#pragma unroll
+            for (int c = 0; c < L::kOCols; c += 16) tmem_ld16(o_tmem + grp * L::kOCols + c, o + c);
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < L::kOCols; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha[c % R]);
-            tmem_st16(o_tmem + grp * L::kOCols, o);
+#pragma unroll
+            for (int c = 0; c < L::kOCols; c += 16) tmem_st16(o_tmem + grp * L::kOCols + c, o + c);
             tmem_wait_st();
           }
         }
         // ---- P ----
-        uint32_t pk[L::kOCols / 4];
+        uint32_t pk[L::kOCols / 4] = {};
 #pragma unroll
         for (int r = 0; r < R; r += 4) {
           float p[4];
@@ -453,17 +457,26 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             l[r + k] += e;
             p[k] = e * v_scale;
           }
-          // The first term is P rounded to four bits, in integer arithmetic: its code need not be read back.  The second is
-          // what is left, times 16.
+          // The first term is P rounded to four bits, in integer arithmetic: its code need not be read back.  The next is what
+          // is left, times 16, and f16's third what that leaves, times 16 once more.
           const float2 a0 = make_float2(p[0], p[1]), a1 = make_float2(p[2], p[3]);
           const float2 h0 = four_bits(a0), h1 = four_bits(a1);
           const float2 r0 = mul2(sub2(a0, h0), make_float2(16.f, 16.f)), r1 = mul2(sub2(a1, h1), make_float2(16.f, 16.f));
           pk[r / 4] = e4m3x2(h0.x, h0.y) | (e4m3x2(h1.x, h1.y) << 16);
-          pk[R / 4 + r / 4] = e4m3x2(r0.x, r0.y) | (e4m3x2(r1.x, r1.y) << 16);
+          if constexpr (L::kPTerms == 2) {
+            pk[R / 4 + r / 4] = e4m3x2(r0.x, r0.y) | (e4m3x2(r1.x, r1.y) << 16);
+          } else {
+            const float2 g0 = e4m3_steps(four_bits(r0)), g1 = e4m3_steps(four_bits(r1));
+            const float2 t0 = mul2(sub2(r0, g0), make_float2(16.f, 16.f)), t1 = mul2(sub2(r1, g1), make_float2(16.f, 16.f));
+            pk[R / 4 + r / 4] = e4m3x2(g0.x, g0.y) | (e4m3x2(g1.x, g1.y) << 16);
+            pk[R / 2 + r / 4] = e4m3x2(t0.x, t0.y) | (e4m3x2(t1.x, t1.y) << 16);
+          }
         }
         // P's room is free once P V of this warpgroup's previous tile is done.
         if (step >= 2 && !warp_wait(SPLASH_KBAR(pv_done, grp), ((step - 2) >> 1) & 1, ctx, kCSiteSmxP, step)) { ok = false; break; }
-        sts128(p_row, make_uint4(pk[0], pk[1], pk[2], pk[3]));
+#pragma unroll
+        for (int c = 0; c < L::kOCols / 16; ++c)
+          sts128(p_row + c * L::kPBlock, make_uint4(pk[c * 4], pk[c * 4 + 1], pk[c * 4 + 2], pk[c * 4 + 3]));
         fence_proxy_async_smem();
         tc_fence_before();
         arrive(SPLASH_KBAR(p_ready, grp));
@@ -499,8 +512,11 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       const bool whole = cur.whole;
       const bool has[2] = {n > 1 || !(step0 & 1), n > 1 || (step0 & 1)};  // which warpgroups had a tile
       uint32_t o0[L::kOCols], o1[L::kOCols];
-      if (has[0]) tmem_ld16(o_tmem, o0);
-      if (has[1]) tmem_ld16(o_tmem + L::kOCols, o1);
+#pragma unroll
+      for (int c = 0; c < L::kOCols; c += 16) {
+        if (has[0]) tmem_ld16(o_tmem + c, o0 + c);
+        if (has[1]) tmem_ld16(o_tmem + L::kOCols + c, o1 + c);
+      }
       tmem_wait_ld();
       tc_fence_before();
       arrive(SPLASH_KBAR(o_free, 0));
@@ -535,8 +551,14 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if ((r >= R / 2) != (grp == 1) || rt * R + r >= a.rows) continue;
         float value = 0.f;
         if ((live >> r) & 1u) {
-          if (has[0]) value = fmaf(__uint_as_float(o0[R + r]), 1.f / 16, __uint_as_float(o0[r])) * w0_r;
-          if (has[1]) value = fmaf(fmaf(__uint_as_float(o1[R + r]), 1.f / 16, __uint_as_float(o1[r])), w1_r, value);
+          auto all_terms = [&](const uint32_t* o) {
+            float x = __uint_as_float(o[(L::kPTerms - 1) * R + r]);
+#pragma unroll
+            for (int t = L::kPTerms - 2; t >= 0; --t) x = fmaf(x, 1.f / 16, __uint_as_float(o[t * R + r]));
+            return x;
+          };
+          if (has[0]) value = all_terms(o0) * w0_r;
+          if (has[1]) value = fmaf(all_terms(o1), w1_r, value);
         }
         if (key_lane >= D) continue;
         if (!whole) a.part_o[(part0 + r) * D + key_lane] = value;

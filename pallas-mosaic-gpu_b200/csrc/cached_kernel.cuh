@@ -26,7 +26,9 @@
 //   * 2^ek of a key scales its column of S; 2^ev of a value scales its column of P, and the running maximum is one of
 //     s + ev and lags behind by a factor of 8 at most, so that the scaled probabilities end between 32 and 256.
 //   * P = p1 + p2 with p1, p2 e4m3: 8 bits as a bf16 P has, down to 2^-7 of the row's largest scaled probability; below
-//     that the steps stay at 2^-14 of it or less.
+//     that the steps stay at 2^-14 of it or less.  f16 takes a third term (two lose it 3 bits: 6e-4 of a result's size
+//     against 2e-4), for which tensor memory has no columns left: it lies where the tile's scores did, and the scores of tile
+//     t + 2 wait for P V of tile t (16 rows, 32 sequences of 8192 keys, 8 kv heads, head_dim 128: 169 us, bf16 124).
 #pragma once
 
 #include "cached_common.cuh"
@@ -43,7 +45,8 @@ struct CachedLayout {
   static constexpr int kBoxes = kRowBytes / kBoxBytes;
   static constexpr int kBoxElems = kBoxBytes / kItem;
   static constexpr int kSlotBytes = kCachedTile * kRowBytes;
-  static constexpr int kTerms = QUANT ? (BF16 ? 2 : 3) : 1;
+  static constexpr int kTerms = QUANT ? (BF16 ? 2 : 3) : 1;  // of Q, and of P
+  static constexpr bool kThird = kTerms == 3;
   static constexpr int kQTerm = 128 * kRowBytes;
   static constexpr int kQBytes = kTerms * kQTerm;
   static constexpr int kStageStride = 36;                  // words per row of the staging area (32 used)
@@ -157,6 +160,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           const int buf = qk.step & 1, slot = qk.step % L::kSlots;
           const bool ready = mbar_probe(SPLASH_KBAR(k_full, slot), (qk.step / L::kSlots) & 1) &&
                              (qk.step < 2 || mbar_probe(SPLASH_KBAR(s_free, buf), ((qk.step - 2) >> 1) & 1)) &&
+                             (!L::kThird || qk.step < 2 || mbar_probe(SPLASH_KBAR(pv_done, buf), ((qk.step - 2) >> 1) & 1)) &&
                              (qk.i > 0 || mbar_probe(SPLASH_KBAR(q_full, 0), qk.seg & 1));
           if (__all_sync(0xffffffffu, ready)) {
             tc_fence_after();
@@ -191,12 +195,14 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             const uint32_t b_lo = desc_lo(v_u32 + slot * L::kSlotBytes, kCachedTile * L::kBoxBytes);
             const uint32_t p_tmem = tmem + L::kPCol + buf * 64;
             constexpr int kKeysPerMma = QUANT ? 32 : 16;
-            // P is 8 columns an MMA; 8 bit: its second term follows in columns 32 .. 63, on the same values.
+            // P is 8 columns an MMA; 8 bit: its second term follows in columns 32 .. 63, the third where the scores were, on the
+            // same values.
 #pragma unroll
-            for (int kk = 0; kk < (QUANT ? 2 : 1) * kCachedTile / kKeysPerMma; ++kk) {
+            for (int kk = 0; kk < L::kTerms * kCachedTile / kKeysPerMma; ++kk) {
               const uint32_t off = ((kk * kKeysPerMma) % kCachedTile * L::kBoxBytes) >> 4;
-              if constexpr (QUANT) umma8_ts2_w(tmem + L::kOCol, p_tmem + kk * 8, b_lo + off, kHi, kIdescPV, pv.i > 0 || kk > 0);
-              else umma_ts2_w(tmem + L::kOCol, p_tmem + kk * 8, b_lo + off, kHi, kIdescPV, pv.i > 0 || kk > 0);
+              const uint32_t p_at = kk < 8 ? p_tmem + kk * 8 : tmem + buf * 128 + (kk - 8) * 8;
+              if constexpr (QUANT) umma8_ts2_w(tmem + L::kOCol, p_at, b_lo + off, kHi, kIdescPV, pv.i > 0 || kk > 0);
+              else umma_ts2_w(tmem + L::kOCol, p_at, b_lo + off, kHi, kIdescPV, pv.i > 0 || kk > 0);
             }
             umma_commit_w(SPLASH_KBAR(v_empty, slot));
             umma_commit_w(SPLASH_KBAR(pv_done, buf));
@@ -510,7 +516,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
 #pragma unroll
         for (int c = 0; c < L::kKeys / 32; ++c) {
           if constexpr (QUANT) {
-            uint32_t p1[8], p2[8];
+            uint32_t p1[8], p2[8], p3[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const int at = c * 32 + j * 4;
@@ -526,10 +532,27 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
               const float2 hx = four_bits(px), hy = four_bits(py);
               const float2 rx = sub2(px, hx), ry = sub2(py, hy);
               p1[j] = e4m3x2(hx.x, hx.y) | (e4m3x2(hy.x, hy.y) << 16);
-              p2[j] = e4m3x2(rx.x, rx.y) | (e4m3x2(ry.x, ry.y) << 16);
+              if constexpr (!L::kThird) {
+                p2[j] = e4m3x2(rx.x, rx.y) | (e4m3x2(ry.x, ry.y) << 16);
+              } else {
+                const float2 gx = e4m3_steps(four_bits(rx)), gy = e4m3_steps(four_bits(ry));
+                const float2 tx = sub2(rx, gx), ty = sub2(ry, gy);
+                p2[j] = e4m3x2(gx.x, gx.y) | (e4m3x2(gy.x, gy.y) << 16);
+                p3[j] = e4m3x2(tx.x, tx.y) | (e4m3x2(ty.x, ty.y) << 16);
+              }
             }
             tmem_st8(p_tmem + col0 / 4 + c * 8, p1);
             tmem_st8(p_tmem + 32 + col0 / 4 + c * 8, p2);
+            if constexpr (L::kThird) {
+              // (The other copies' keys are scores here, and not zeros from the start.)
+#pragma unroll
+              for (int other = 0; other < KG; ++other) {
+                uint32_t x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = other == part ? p3[j] : 0u;
+                tmem_st8(s_tmem + other * (L::kKeys / 4) + c * 8, x);
+              }
+            }
           } else {
             uint32_t pk[16];
 #pragma unroll

@@ -1,9 +1,9 @@
 """Attention over the paged cache against the definition in 64 bits.
 
 Bars, per number of the result, with p the softmax weights and A = sum_j p_j |v_j|:
-  * P is rounded once (16 bits: half a step h, bf16 2^-8, f16 2^-11; 8-bit caches: two terms of e4m3, 2^-4 * 2^-4, and below
-    their range half a step of the subnormals, 2^-10 where the largest 2^ev p is 32 or more, times the codes of the values),
-    the result once (h);
+  * P is rounded once (16 bits: half a step h, bf16 2^-8, f16 2^-11; 8-bit caches: two terms of e4m3, 2^-4 * 2^-4, or for f16
+    three, and below their range half a step of the subnormals, 2^-10 where the largest 2^ev p is 32 or more, times the codes
+    of the values), the result once (h);
   * the scores are off by dS = 2^-19 sum|q k| + 2^-10 |s| under a soft-cap (tanh.approx) and, 8 bit, 2^-17 max|q| sum|k| (the
     e4m3 terms of q), which moves p by at most 2 dS relative to itself for dS < 0.1; 2^-12 A covers 32-bit sums and ex2.approx.
   logsumexp: dS + 2^-19 (1 + |lse|)."""
@@ -116,7 +116,7 @@ def _check(b, h, kvh, n, d, dtype, quantized, page, lengths, *, counts=None, par
   assert torch.equal(out, again)
   kk, vv = cache.read(table, lens, longest, dtype=dtype)
   half = torch.finfo(dtype).eps / 2
-  p_half = 2.0 ** -8 if quantized else half
+  p_half = (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -12) if quantized else half
   for i in range(b):
     length = lengths[i]
     if length == 0:
