@@ -263,7 +263,7 @@ static_assert(sizeof(WideBarriers) <= WideLayout<128>::kBarBytes, "barrier block
 // with a ring, 357 us here.)
 // SHARED: the columns of a few keys that nearly every query sees (sinks beside a window) would each be the work of one
 // CTA, many times as long as the others'; they are cut into a.parts shares of their steps, whose dK and dV bwd_parts_kernel
-// adds up (window 1024, 4 sinks, 8/2 heads, seq 8192, D = 128: 540 -> 92 us).  Compiled apart.
+// adds up (window 1024, 4 sinks, 8/2 heads, seq 8192, D = 128: 540 -> 99 us).  Compiled apart.
 template <int HEAD_DIM, bool PLAIN, bool BF16, bool SHARED>
 __global__ void __launch_bounds__(WideLayout<HEAD_DIM>::kThreads, 1)
 splash_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,

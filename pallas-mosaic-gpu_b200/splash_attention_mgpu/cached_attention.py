@@ -48,7 +48,7 @@ class CachedAttentionKernel:
 
     q: [B, heads, n, head_dim], or [heads, n, head_dim] for one sequence; pre-scaled
     page_table: int32 [B, pages per sequence]
-    lengths: int32 [B], tokens of each sequence in the cache, the new ones included
+    lengths: int32 [B], tokens of each sequence in the cache, the new ones included (at most what its pages hold)
     counts: int32 [B], new tokens of each sequence, its first rows of q (None: n); the rows behind them give zeros
     parents: int32 [n] or [B, n], the new tokens as a tree: token i follows token parents[i] < i, or (-1) the last token in
       front of the new ones.  It sees those, its ancestors and itself, and its position is one behind its parent's.
