@@ -135,7 +135,7 @@ struct CachedBarriers {
   uint64_t k_full[kCachedMaxSlots], k_empty[kCachedMaxSlots], v_full[kCachedMaxSlots], v_empty[kCachedMaxSlots];
   uint64_t s_ready[4], pv_done[2];
   uint64_t s_free[4], p_ready[2];
-  uint64_t q_full, q_free, o_free, sync;
+  uint64_t q_full[2], q_free[2], o_free, sync;  // (one of either in use where Q has one buffer)
   uint64_t tree_full[2], tree_free[2];
   uint32_t tmem_base, abort_flag, dead;
   int32_t first_entry, first_head, first_offset, share;
@@ -484,17 +484,20 @@ __device__ __forceinline__ bool cached_make_tree(const CachedArgs& a, int b, int
   return true;
 }
 
-// One warp: the rows of a segment as TERMS e4m3 terms each, handed to `store`, and their scales.
-template <int D, bool BF16, int TERMS, int R, typename Store>
+// One warp: the rows of a segment as TERMS e4m3 terms each, handed to `store`, into one of BUFFERS in turn, and their scales into
+// one of SLOTS.  Scales stay longer than the rows: the scores of a segment's last tile free its rows, and the softmax may be that
+// tile and as many more behind as there are buffers of scores, each of another segment.
+template <int D, bool BF16, int TERMS, int R, int BUFFERS, int SLOTS, typename Store>
 __device__ __forceinline__ bool cached_split_q(const CachedArgs& a, int seg, int b, int rt, int head, uint32_t bars_u32, uint32_t qscale_u32,
                                                int lane, const WaitCtx& ctx, Store store) {
   constexpr int kPer = D / 32;  // neighbouring numbers per lane
-  if (seg > 0 && !warp_wait(SPLASH_KBAR(q_free, 0), (seg - 1) & 1, ctx, kCSiteConvQ, seg)) return false;
+  const int buffer = seg % BUFFERS, use = seg / BUFFERS;
+  if (use > 0 && !warp_wait(SPLASH_KBAR(q_free, buffer), (use - 1) & 1, ctx, kCSiteConvQ, seg)) return false;
   const long long row0 = static_cast<long long>(b * a.kv_heads + head) * a.rows + rt * R;
   const int rows = min(R, a.rows - rt * R);
   constexpr int kBatch = 8;  // rows whose loads are in flight together
   for (int r0 = 0; r0 < R; r0 += kBatch) {
-    if (seg > 1 && a.row_tiles == 1 && r0 >= rows) break;  // zeros, as the first two segments have left them
+    if (seg >= SLOTS && a.row_tiles == 1 && r0 >= rows) break;  // zeros, as the first segments have left them
     uint32_t w[kBatch][kPer / 2];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
@@ -527,7 +530,7 @@ __device__ __forceinline__ bool cached_split_q(const CachedArgs& a, int seg, int
         x[2 * i + 1] = f.y * down;
       }
       if (lane == 0)
-        sts32(qscale_u32 + ((seg & 1) * R + r) * 4, bad ? 0x7fc00000u : static_cast<uint32_t>(e + 127) << 23);
+        sts32(qscale_u32 + (seg % SLOTS * R + r) * 4, bad ? 0x7fc00000u : static_cast<uint32_t>(e + 127) << 23);
 #pragma unroll
       for (int t = 0; t < TERMS; ++t) {
         uint32_t code[kPer / 2];
@@ -545,7 +548,7 @@ __device__ __forceinline__ bool cached_split_q(const CachedArgs& a, int seg, int
   }
   fence_proxy_async_smem();
   __syncwarp();
-  if (lane == 0) mbar_arrive(SPLASH_KBAR(q_full, 0));
+  if (lane == 0) mbar_arrive(SPLASH_KBAR(q_full, buffer));
   return true;
 }
 

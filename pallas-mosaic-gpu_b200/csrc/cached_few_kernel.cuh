@@ -1,10 +1,10 @@
-// Attention over an 8-bit paged cache for few rows: up to 8 new tokens x heads of a kv head, as in token-by-token decoding.
+// Attention over an 8-bit paged cache for few rows: up to 8 or 16 new tokens x heads of a kv head, as in token-by-token decoding.
 //
 // cached_kernel.cuh spends an MMA's 128 rows on copies of the few rows there are, and its products then take about as long as
 // an 8-bit tile's transfer (32 sequences of 2000 to 32768 keys, 64 / 8 heads: 278 us; here 196).  Here the keys are the 128
 // rows instead:
-//   S^T = K Q^T       [128 keys x rows]        A = K as it lies in the cache, B = Q, 16 or 24 columns
-//   O^T += V^T P^T    [head_dim x rows]        A = V^T (V read M-major), B = P^T, which a key's thread writes as 16 bytes (f16: 32)
+//   S^T = K Q^T       [128 keys x rows]        A = K as it lies in the cache, B = Q, 16 to 48 columns
+//   O^T += V^T P^T    [head_dim x rows]        A = V^T (V read M-major), B = P^T, which a key's thread writes as 16 to 48 bytes
 // An MMA costs its 4 KB of A, 32 cycles: 256 a tile, where the copies cost 1024.  A thread has one key and all rows: the
 // scales of the key and its value are two numbers of its own, and no exponential is computed twice.
 //
@@ -16,58 +16,58 @@
 // Q is 2 (bf16) or 3 (f16) e4m3 terms side by side in B, whose columns of S are added; P is as many, p1 + p2 / 16 + p3 / 256,
 // side by side as well, whose columns of O are added with those factors.
 //
+// Maxima and factors of the rows are in shared memory between the tiles: with them in registers 16 rows need more than a thread
+// has, and what is spilled comes back from L2, as shared memory leaves the L1 cache next to nothing (173 us instead of 105).
+//
 // Not here: 16-bit caches, whose tiles take twice as long to arrive while the copies' products take no longer than here (192
-// us there, 203 here for 16 sequences of 4000 to 32768 keys, 32 / 8 heads); and 9 to 16 rows, whose state does not fit a
-// thread's registers (64 sequences of 300 to 32768 keys, windows of 4096, 16 rows: 123 us there, 204 here).
+// us there, 203 here for 16 sequences of 4000 to 32768 keys, 32 / 8 heads).
 #pragma once
 
 #include "cached_common.cuh"
 
 namespace splash {
 
-constexpr int kCachedFewRows = 8;
-
-template <int D, bool BF16>
+template <int D, bool BF16, int R>
 struct CachedFewLayout {
-  static constexpr int R = kCachedFewRows;
   static constexpr int kTerms = BF16 ? 2 : 3;
   static constexpr int kSCols = (kTerms * R + 15) / 16 * 16;  // N of the scores: a multiple of 16
   static constexpr int kPTerms = BF16 ? 2 : 3;
   static constexpr int kOCols = (kPTerms * R + 15) / 16 * 16;  // N of P V
   static constexpr int kItem = 1, kRowBytes = D, kBoxBytes = D, kBoxes = 1, kBoxElems = D;  // a key: one box of 64 or 128 bytes
   static constexpr int kSlotBytes = kCachedTile * kRowBytes;
-  static constexpr int kQBytes = kSCols * D;
+  static constexpr int kQBytes = (kSCols * D + 1023) / 1024 * 1024;  // of one of two buffers
   // P^T: core matrices of 8 keys x 16 bytes one after the other, and 2 KB on the next 16 columns.
   static constexpr int kPBlock = kCachedTile * 16;
   static constexpr int kPBytes = kCachedTile * kOCols;
   static constexpr int kBarBytes = 512;
   static constexpr int kAuxBytes = kCachedAuxSlots * 2 * kCachedTile;
-  static constexpr int kQScaleBytes = 2 * R * 4;
+  static constexpr int kQScaleSlots = 8;                      // (four buffers of scores: see cached_split_q)
+  static constexpr int kQScaleBytes = kQScaleSlots * R * 4;
   static constexpr int kVoteBytes = 2 * 2 * 16;               // by warpgroup and parity of its tiles: a word per warp
   static constexpr int kMaxBytes = 8 * R * 4;                 // per warp: maxima of its keys
+  static constexpr int kStateBytes = 8 * R * 8;                // per warp: maxima, and the rows' factors
   static constexpr int kSumBytes = 2 * (8 + 2) * R * 4;       // by parity of the segment: sums per warp, maxima per warpgroup
   static constexpr int kRowInfoBytes = 8 * R * 16;            // per warp: what each row sees
   static constexpr int kTreeBytes = kCachedMaxTree * 8 + 2 * kCachedMaxTree * 8 * 4;
-  static constexpr int kFixed = 1024 + (kQBytes + 1023) / 1024 * 1024 + 2 * kPBytes + kBarBytes + kAuxBytes + kQScaleBytes + kVoteBytes +
-                                kMaxBytes + kSumBytes + kRowInfoBytes + kTreeBytes;
+  static constexpr int kFixed = 1024 + 2 * kQBytes + 2 * kPBytes + kBarBytes + kAuxBytes + kQScaleBytes + kVoteBytes +
+                                kMaxBytes + kStateBytes + kSumBytes + kRowInfoBytes + kTreeBytes;
   static constexpr int kSlotsFit = (227 * 1024 - kFixed) / (2 * kSlotBytes);
   static constexpr int kSlots = kSlotsFit < kCachedMaxSlots ? kSlotsFit : kCachedMaxSlots;
   static constexpr int kSmem = kFixed + 2 * kSlots * kSlotBytes;
   // Tensor memory: four buffers of scores, O of the two warpgroups.
   static constexpr int kOCol = 4 * kSCols;
-  static constexpr int kTmemCols = 256;
+  static constexpr int kTmemCols = kOCol + 2 * kOCols > 256 ? 512 : 256;
   static_assert(kOCol + 2 * kOCols <= kTmemCols, "");
   static constexpr int kSoftmaxRegs = 184, kLoadRegs = 136;   // 384 * 168 = 256 * 184 + 128 * 136
 };
 
-template <int D, bool BF16>
+template <int D, bool BF16, int R>
 __global__ void __launch_bounds__(kCachedThreads, 1)
 cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const CachedArgs a) {
-  using L = CachedFewLayout<D, BF16>;
-  constexpr int R = L::R;
+  using L = CachedFewLayout<D, BF16, R>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t q_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t k_u32 = q_u32 + (L::kQBytes + 1023) / 1024 * 1024;
+  const uint32_t k_u32 = q_u32 + 2 * L::kQBytes;
   const uint32_t v_u32 = k_u32 + L::kSlots * L::kSlotBytes;
   const uint32_t p_u32 = v_u32 + L::kSlots * L::kSlotBytes;
   const uint32_t bars_u32 = p_u32 + 2 * L::kPBytes;
@@ -75,7 +75,8 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   const uint32_t vote_u32 = aux_u32 + L::kAuxBytes;
   const uint32_t qscale_u32 = vote_u32 + L::kVoteBytes;
   const uint32_t max_u32 = qscale_u32 + L::kQScaleBytes;
-  const uint32_t sum_u32 = max_u32 + L::kMaxBytes;
+  const uint32_t state_u32 = max_u32 + L::kMaxBytes;
+  const uint32_t sum_u32 = state_u32 + L::kStateBytes;
   const uint32_t info_u32 = sum_u32 + L::kSumBytes;
   const uint32_t parents_u32 = info_u32 + L::kRowInfoBytes;
   const uint32_t trees_u32 = parents_u32 + 2 * kCachedMaxTree * 4;
@@ -101,7 +102,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   } else if (warp == 10) {
     // No votes yet; and zeros in rows of Q that no term fills (the scores' columns are a multiple of 16).
     if (lane < L::kVoteBytes / 4) sts32(vote_u32 + lane * 4, 0xffffffffu);
-    for (int i = lane; i < L::kQBytes / 16; i += 32) sts128(q_u32 + i * 16, make_uint4(0, 0, 0, 0));
+    for (int i = lane; i < 2 * L::kQBytes / 16; i += 32) sts128(q_u32 + i * 16, make_uint4(0, 0, 0, 0));
     fence_proxy_async_smem();
   } else if (warp == 0) {
     cached_find_share(a, bars_u32, lane);
@@ -167,17 +168,17 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           const int buf = qk.step & 3, slot = qk.step % L::kSlots;
           const bool ready = mbar_probe(SPLASH_KBAR(k_full, slot), (qk.step / L::kSlots) & 1) &&
                              (qk.step < 4 || mbar_probe(SPLASH_KBAR(s_free, buf), ((qk.step - 4) >> 2) & 1)) &&
-                             (qk.i > 0 || mbar_probe(SPLASH_KBAR(q_full, 0), qk.seg & 1));
+                             (qk.i > 0 || mbar_probe(SPLASH_KBAR(q_full, qk.seg & 1), (qk.seg >> 1) & 1));
           if (__all_sync(0xffffffffu, ready)) {
             tc_fence_after();
             qk.at_tile(bars_u32);
-            const uint32_t a_lo = desc_lo(k_u32 + slot * L::kSlotBytes, 16), b_lo = desc_lo(q_u32, 16);
+            const uint32_t a_lo = desc_lo(k_u32 + slot * L::kSlotBytes, 16), b_lo = desc_lo(q_u32 + (qk.seg & 1) * L::kQBytes, 16);
 #pragma unroll
             for (int kk = 0; kk < D / 32; ++kk)
               umma8_ss2_w(tmem + buf * L::kSCols, a_lo + kk * 2, kHi, b_lo + kk * 2, kHi, kIdescS, kk > 0);
             umma_commit_w(SPLASH_KBAR(s_ready, buf));
             umma_commit_w(SPLASH_KBAR(k_empty, slot));
-            if (qk.i + 1 == qk.n) umma_commit_w(SPLASH_KBAR(q_free, 0));
+            if (qk.i + 1 == qk.n) umma_commit_w(SPLASH_KBAR(q_free, qk.seg & 1));
             qk.advance();
             issued = true;
           }
@@ -206,9 +207,9 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           if (!cached_make_tree(a, b, cur.g.before, trees++, bars_u32, parents_u32, lane, ctx)) break;
         }
         auto store = [&](int t, int r, uint32_t byte, uint32_t codes) {
-          sts_bytes<D / 32>(q_u32 + cached_swz<L::kBoxBytes>(t * R + r, byte >> 4) + (byte & 15u), codes);
+          sts_bytes<D / 32>(q_u32 + (seg & 1) * L::kQBytes + cached_swz<L::kBoxBytes>(t * R + r, byte >> 4) + (byte & 15u), codes);
         };
-        if (!cached_split_q<D, BF16, L::kTerms, R>(a, seg, b, rt, cur.seg_head, bars_u32, qscale_u32, lane, ctx, store)) break;
+        if (!cached_split_q<D, BF16, L::kTerms, R, 2, L::kQScaleSlots>(a, seg, b, rt, cur.seg_head, bars_u32, qscale_u32, lane, ctx, store)) break;
       }
     }
   } else {
@@ -221,6 +222,11 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     const uint32_t o_tmem = tmem_lane + L::kOCol;
     const uint32_t p_row = p_u32 + grp * L::kPBytes + key_lane * 16;
     const uint32_t my_info = info_u32 + warp * (R * 16);
+    const uint32_t my_state = state_u32 + warp * (R * 8);
+    auto load4 = [&](uint32_t at, float* x) {
+      const uint4 w = lds128(at);
+      x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
+    };
     const int piece_shift = min(a.page_shift, 7);
     const bool tree = a.parents != nullptr;
     const bool capped = a.soft_cap > 0.f;
@@ -316,13 +322,13 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if (key < g.hi) asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(id) : "l"(table + (key >> a.page_shift)));
         return id;
       };
-      float m[R], l[R], mul[R];  // maxima of s + ev (powers of 2; the same in every thread), this key's sums, factor of a row
+      float l[R];  // this key's sums
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        m[r] = -INFINITY;
-        l[r] = 0.f;
-        mul[r] = 0.f;
-      }
+      for (int r = 0; r < R; ++r) l[r] = 0.f;
+      // Maxima of s + ev (powers of 2; the same in every warp of the warpgroup) and the factors of the rows' scores: in shared
+      // memory and not in registers between the tiles.  Rows that are none have factor 0 and never call for new maxima.
+      if (lane < R) sts32(my_state + lane * 4, __float_as_uint(-INFINITY));
+      __syncwarp();
       const int i0 = (grp ^ step0) & 1;  // the CTA's tiles alternate between the warpgroups, whatever segment they are of
       int page = page_of(i0);
 
@@ -339,14 +345,15 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if (!warp_wait(SPLASH_KBAR(s_ready, buf), (step >> 2) & 1, ctx, kCSiteSmxS, step)) { ok = false; break; }
         tc_fence_after();
         uint32_t raw[L::kSCols];
-        tmem_ld16(tmem_lane + buf * L::kSCols, raw);
-        if constexpr (L::kSCols == 32) tmem_ld16(tmem_lane + buf * L::kSCols + 16, raw + 16);
+#pragma unroll
+        for (int c = 0; c < L::kSCols; c += 16) tmem_ld16(tmem_lane + buf * L::kSCols + c, raw + c);
         float k_scale = 1.f, v_exp = 0.f, v_scale = kPScale;
         // The key's own scales, and once the rows'.  (The exponents came with the keys, for which the scores waited.)
         if (i == i0) {
-#pragma unroll
-          for (int r = 0; r < R; ++r)  // rows that are none have factor 0 and never call for new maxima
-            if ((live >> r) & 1u) mul[r] = pre * __uint_as_float(lds32(qscale_u32 + ((seg & 1) * R + r) * 4));
+          if (lane < R)
+            sts32(my_state + (R + lane) * 4,
+                  (live >> lane) & 1u ? __float_as_uint(pre * __uint_as_float(lds32(qscale_u32 + (seg % L::kQScaleSlots * R + lane) * 4))) : 0u);
+          __syncwarp();
         }
         if (there) {
           const uint32_t at = aux_u32 + (step % kCachedAuxSlots) * (2 * kCachedTile) + key_lane;
@@ -360,11 +367,17 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         arrive(SPLASH_KBAR(s_free, buf));  // the scores of tile step + 4 may come
         float x[R];  // scores in powers of 2
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          x[r] = __uint_as_float(raw[r]);
+        for (int r4 = 0; r4 < R; r4 += 4) {
+          float mul[4];
+          load4(my_state + (R + r4) * 4, mul);
 #pragma unroll
-          for (int t = 1; t < L::kTerms; ++t) x[r] += __uint_as_float(raw[t * R + r]);
-          x[r] *= k_scale * mul[r];
+          for (int k = 0; k < 4; ++k) {
+            const int r = r4 + k;
+            x[r] = __uint_as_float(raw[r]);
+#pragma unroll
+            for (int t = 1; t < L::kTerms; ++t) x[r] += __uint_as_float(raw[t * R + r]);
+            x[r] *= k_scale * mul[k];
+          }
         }
         if (__builtin_expect(capped, 0)) {
 #pragma unroll
@@ -398,6 +411,9 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           }
         }
         // ---- does a score stand above the maxima by more than they may lag? ----
+        float m[R];
+#pragma unroll
+        for (int r = 0; r < R; r += 4) load4(my_state + r * 4, m + r);
         bool above = false;
 #pragma unroll
         for (int r = 0; r < R; ++r) above = above || x[r] + v_exp > m[r] + kThreshold;  // (-inf + lag is -inf)
@@ -433,15 +449,23 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               l[r] *= alpha[r];
             }
           }
+          __syncwarp();  // (all have read the old ones)
+          if (lane == 0) {
+#pragma unroll
+            for (int r = 0; r < R; r += 4)
+              sts128(my_state + r * 4, make_uint4(__float_as_uint(m[r]), __float_as_uint(m[r + 1]), __float_as_uint(m[r + 2]), __float_as_uint(m[r + 3])));
+          }
+          __syncwarp();
           if (i >= 2) {
-            uint32_t o[L::kOCols];
 #pragma unroll
-            for (int c = 0; c < L::kOCols; c += 16) tmem_ld16(o_tmem + grp * L::kOCols + c, o + c);
-            tmem_wait_ld();
+            for (int c = 0; c < L::kOCols; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(o_tmem + grp * L::kOCols + c, o);
+              tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < L::kOCols; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha[c % R]);
-#pragma unroll
-            for (int c = 0; c < L::kOCols; c += 16) tmem_st16(o_tmem + grp * L::kOCols + c, o + c);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha[(c + k) % R]);
+              tmem_st16(o_tmem + grp * L::kOCols + c, o);
+            }
             tmem_wait_st();
           }
         }
@@ -500,10 +524,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         for (int d = 16 / R; d > 0; d /= 2) l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
         if ((lane & (32 / R - 1)) == 0) sts32(sums + (warp * R + lane / (32 / R)) * 4, __float_as_uint(l[0]));
       }
-      if (quarter == 0 && lane == 0) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) sts32(maxima + (grp * R + r) * 4, __float_as_uint(m[r]));
-      }
+      if (quarter == 0 && lane < R) sts32(maxima + (grp * R + lane) * 4, lds32(my_state + lane * 4));
       if (!group_sync()) { ok = false; break; }
       // (Both warpgroups are past their tiles, so the barrier's phase before the last tile's is over.)
       const int last = step0 + n - 1;
@@ -511,11 +532,13 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       tc_fence_after();
       const bool whole = cur.whole;
       const bool has[2] = {n > 1 || !(step0 & 1), n > 1 || (step0 & 1)};  // which warpgroups had a tile
-      uint32_t o0[L::kOCols], o1[L::kOCols];
+      // Warpgroup g writes its half of the rows, a thread one number of each: of 8 rows' columns of every term, from row `r0` on.
+      const int r0 = R > 8 ? grp * 8 : 0;
+      uint32_t o0[L::kPTerms * 8], o1[L::kPTerms * 8];
 #pragma unroll
-      for (int c = 0; c < L::kOCols; c += 16) {
-        if (has[0]) tmem_ld16(o_tmem + c, o0 + c);
-        if (has[1]) tmem_ld16(o_tmem + L::kOCols + c, o1 + c);
+      for (int t = 0; t < L::kPTerms; ++t) {
+        if (has[0]) tmem_ld8(o_tmem + t * R + r0, o0 + t * 8);
+        if (has[1]) tmem_ld8(o_tmem + L::kOCols + t * R + r0, o1 + t * 8);
       }
       tmem_wait_ld();
       tc_fence_before();
@@ -544,17 +567,17 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         w1 *= scale;
         if (l_tot != l_tot) w0 = w1 = l_tot;
       }
-      // Warpgroup g writes its half of the rows, a thread one number of each.
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
+      for (int k = 0; k < 8; ++k) {
+        const int r = r0 + k;
         const float w0_r = __shfl_sync(0xffffffffu, w0, r), w1_r = __shfl_sync(0xffffffffu, w1, r);
-        if ((r >= R / 2) != (grp == 1) || rt * R + r >= a.rows) continue;
+        if ((R == 8 && (k >= 4) != (grp == 1)) || rt * R + r >= a.rows) continue;
         float value = 0.f;
         if ((live >> r) & 1u) {
           auto all_terms = [&](const uint32_t* o) {
-            float x = __uint_as_float(o[(L::kPTerms - 1) * R + r]);
+            float x = __uint_as_float(o[(L::kPTerms - 1) * 8 + k]);
 #pragma unroll
-            for (int t = L::kPTerms - 2; t >= 0; --t) x = fmaf(x, 1.f / 16, __uint_as_float(o[t * R + r]));
+            for (int t = L::kPTerms - 2; t >= 0; --t) x = fmaf(x, 1.f / 16, __uint_as_float(o[t * 8 + k]));
             return x;
           };
           if (has[0]) value = all_terms(o0) * w0_r;

@@ -28,7 +28,7 @@
 //   * P = p1 + p2 with p1, p2 e4m3: 8 bits as a bf16 P has, down to 2^-7 of the row's largest scaled probability; below
 //     that the steps stay at 2^-14 of it or less.  f16 takes a third term (two lose it 3 bits: 6e-4 of a result's size
 //     against 2e-4), for which tensor memory has no columns left: it lies where the tile's scores did, and the scores of tile
-//     t + 2 wait for P V of tile t (16 rows, 32 sequences of 8192 keys, 8 kv heads, head_dim 128: 169 us, bf16 124).
+//     t + 2 wait for P V of tile t (64 rows, 32 sequences of 8192 keys, 8 kv heads, head_dim 128: 236 us, bf16 156).
 #pragma once
 
 #include "cached_common.cuh"
@@ -56,7 +56,8 @@ struct CachedLayout {
   static constexpr int kBarBytes = 512;
   static constexpr int kAuxBytes = QUANT ? kCachedAuxSlots * 2 * kCachedTile : 0;
   static constexpr int kScaleBytes = QUANT ? 8 * kKeys * 12 : 0;  // per warp: three numbers for each of its keys
-  static constexpr int kQScaleBytes = QUANT ? 2 * 128 * 4 : 0;
+  static constexpr int kQScaleSlots = 4;                   // (two buffers of scores: see cached_split_q)
+  static constexpr int kQScaleBytes = QUANT ? kQScaleSlots * kRows * 4 : 0;
   static constexpr int kTreeBytes = kCachedMaxTree * 8 + 2 * kCachedMaxTree * 8 * 4;  // parents, pointers | two trees
   static constexpr int kFixed = 1024 + kQBytes + kStageBytes + kMlBytes + kBarBytes + kAuxBytes + kScaleBytes + kQScaleBytes + kTreeBytes;
   static constexpr int kSlotsFit = (227 * 1024 - kFixed) / (2 * kSlotBytes);
@@ -239,7 +240,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             for (int copy = 0; copy < KG; ++copy)
               sts_bytes<D / 32>(q_u32 + t * L::kQTerm + cached_swz<L::kBoxBytes>(copy * L::kRows + r, byte >> 4) + (byte & 15u), codes);
           };
-          if (!cached_split_q<D, BF16, L::kTerms, L::kRows>(a, seg, b, rt, cur.seg_head, bars_u32, qscale_u32, lane, ctx, store)) break;
+          if (!cached_split_q<D, BF16, L::kTerms, L::kRows, 1, L::kQScaleSlots>(a, seg, b, rt, cur.seg_head, bars_u32, qscale_u32, lane, ctx, store)) break;
         }
       }
     }
@@ -393,7 +394,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           // Scales of this warp's keys in shared memory of its own: 2^ek | ev | 2^ev * 32, while the scores arrive.
           // (The exponents came with the keys, for which the scores waited.)
           if (i == i0) {
-            const float q_scale = __uint_as_float(lds32(qscale_u32 + ((seg & 1) * L::kRows + r) * 4));
+            const float q_scale = __uint_as_float(lds32(qscale_u32 + (seg % L::kQScaleSlots * L::kRows + r) * 4));
             q_mul = q_scale * inv_cap;
             mul = a.soft_cap > 0.f ? unit2 : unit2 * q_scale;
           }

@@ -34,10 +34,10 @@ int launch_cached_form(const SplashCachedParams& p, const CachedPlan& plan, cons
   return SPLASH_OK;
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, int R>
 int launch_cached_few(const SplashCachedParams& p, const CachedPlan& plan, const CachedArgs& a, cudaStream_t stream) {
-  using L = CachedFewLayout<D, BF16>;
-  auto kernel = cached_few_kernel<D, BF16>;
+  using L = CachedFewLayout<D, BF16, R>;
+  auto kernel = cached_few_kernel<D, BF16, R>;
   CUtensorMap tm_k, tm_v;
   if (int rc = cached_maps<L, D>(kernel, p, tm_k, tm_v)) return rc;
   kernel<<<plan.ctas, kCachedThreads, L::kSmem, stream>>>(tm_k, tm_v, a);
@@ -48,7 +48,8 @@ int launch_cached_few(const SplashCachedParams& p, const CachedPlan& plan, const
 template <int D, bool BF16>
 int launch_cached(const SplashCachedParams& p, const CachedPlan& plan, const CachedArgs& a, cudaStream_t stream) {
   if (p.quantized) {
-    if (plan.row_cap == kCachedFewRows) return launch_cached_few<D, BF16>(p, plan, a, stream);
+    if (plan.row_cap == 8) return launch_cached_few<D, BF16, 8>(p, plan, a, stream);
+    if (plan.row_cap == 16) return launch_cached_few<D, BF16, 16>(p, plan, a, stream);
     if (plan.row_cap == 32) return launch_cached_form<D, BF16, true, 4>(p, plan, a, stream);
     if (plan.row_cap == 64) return launch_cached_form<D, BF16, true, 2>(p, plan, a, stream);
     return launch_cached_form<D, BF16, true, 1>(p, plan, a, stream);

@@ -74,7 +74,7 @@ def _want(q, k, v, codes, exps, seen, cap):
 
 
 def _check(b, h, kvh, n, d, dtype, quantized, page, lengths, *, counts=None, parents=None, window=None, sinks=0, cap=None, seed=0,
-           spread=1.0, capacity=0):
+           spread=1.0, capacity=0, fade=0):
   g = torch.Generator(device=DEV).manual_seed(seed)
   width = -(-max(max(lengths), capacity, 1) // page) + 1
   cache = sa.make_kv_cache(b * width + 2, kvh, d, page_size=page, dtype=dtype, quantized=quantized, device=DEV)
@@ -91,6 +91,8 @@ def _check(b, h, kvh, n, d, dtype, quantized, page, lengths, *, counts=None, par
   lens = torch.tensor(lengths, dtype=torch.int32, device=DEV)
   cache.write(k, v, table, torch.zeros_like(lens), counts=lens)
   q = (torch.randn(b, h, n, d, generator=g, device=DEV) * d ** -0.5 * spread).to(dtype)
+  if fade:  # other sizes from one sequence, and one row, to the next
+    q = q * torch.exp2(-((torch.arange(b * h, device=DEV) * 5).view(b, h, 1, 1) % fade).float()).to(dtype)
   news = [n] * b if counts is None else counts
   trees = None
   if parents is not None:
@@ -170,6 +172,25 @@ FORMS = [(64, torch.float16, False), (128, torch.bfloat16, False), (64, torch.bf
 ], ids=lambda c: f"b{c['b']}h{c['h']}kv{c['kvh']}len{max(c['lengths'])}")
 def test_gpu_one_token(d, dtype, quantized, case):
   _check(d=d, dtype=dtype, quantized=quantized, **case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    dict(h=16, n=1, lengths=[9000, 130, 1]), dict(h=3, n=4, lengths=[9000, 500, 3], counts=[4, 2, 4]),
+    dict(h=2, n=7, lengths=[8500, 300, 7], parents=[-1, 0, 0, 1, 1, 2, -1]),
+    dict(h=4, n=4, lengths=[9500, 300, 2], window=8200, sinks=5, cap=6.0),
+], ids=lambda c: f"h{c['h']}n{c['n']}")
+@pytest.mark.parametrize("page", [16, 256])
+def test_gpu_up_to_16_rows_against_long_contexts(case, page):
+  _check(b=3, kvh=1, d=128, dtype=torch.bfloat16, quantized=True, page=page, fade=5, **case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,dtype,quantized", [(128, torch.bfloat16, True), (64, torch.float16, True), (128, torch.bfloat16, False)], ids=str)
+@pytest.mark.parametrize("h,n", [(8, 1), (4, 4), (8, 3), (6, 9), (12, 10)])
+def test_gpu_many_short_sequences(d, dtype, quantized, h, n):
+  """A CTA goes through many units of one or two tiles: what it keeps of a unit is not the next one's."""
+  _check(b=700, h=h, kvh=1, n=n, d=d, dtype=dtype, quantized=quantized, page=64, lengths=[(i * 53) % 200 for i in range(700)], fade=11)
 
 
 @pytest.mark.gpu
