@@ -65,9 +65,12 @@ struct CachedLayout {
   static_assert(kSlots >= 2, "two tiles have to fit");
   static constexpr int kSmem = kFixed + 2 * kSlots * kSlotBytes;
   static constexpr int kPCol = 256, kOCol = 384;  // S of the two warpgroups | P of the two | O
-  // Registers of the warpgroups: 384 * 168 at launch = 256 * 208 + 128 * 88 = 256 * 184 + 128 * 136.
-  static constexpr int kSoftmaxRegs = kKeys == 128 ? 208 : 184;
-  static constexpr int kLoadRegs = kKeys == 128 ? 88 : 136;
+  // Scores that a thread has in registers at a time.  With all 128 of a row without copies it has registers for little else, and
+  // what is spilled comes back from L2, as shared memory leaves the L1 cache next to nothing: halves are read from tensor memory
+  // for the maximum, and the second once more for the exponentials (64 sequences of 100 to 3000 keys, 8 kv heads, 192 rows: 191 ->
+  // 172 us; 8 bit, where a half is also scaled twice, 343 -> 326).
+  static constexpr int kPart = kKeys < 64 ? kKeys : 64, kParts = kKeys / kPart;
+  static constexpr int kSoftmaxRegs = 184, kLoadRegs = 136;  // 384 * 168 at launch = 256 * 184 + 128 * 136
 };
 
 template <int D, bool BF16, bool QUANT, int KG>
@@ -384,12 +387,19 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         };
         if (!warp_wait(SPLASH_KBAR(s_ready, buf), par, ctx, kCSiteSmxS, step)) { ok = false; break; }
         tc_fence_after();
-        float sv[L::kKeys];
-        {
+        float sv[L::kPart];  // scores of part h of this thread's keys
+        auto fetch = [&](int h) {
           uint32_t* raw = reinterpret_cast<uint32_t*>(sv);
 #pragma unroll
-          for (int c = 0; c < L::kKeys / 32; ++c) tmem_ld32(s_tmem + col0 + c * 32, raw + c * 32);
-        }
+          for (int c = 0; c < L::kPart / 32; ++c) tmem_ld32(s_tmem + col0 + h * L::kPart + c * 32, raw + c * 32);
+        };
+        auto fetched = [&](bool last) {
+          tmem_wait_ld();
+          if (!last) return;
+          tc_fence_before();
+          arrive(SPLASH_KBAR(s_free, buf));  // the scores of tile step + 2 may come
+        };
+        fetch(L::kParts - 1);
         if constexpr (QUANT) {
           // Scales of this warp's keys in shared memory of its own: 2^ek | ev | 2^ev * 32, while the scores arrive.
           // (The exponents came with the keys, for which the scores waited.)
@@ -414,43 +424,65 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           }
           __syncwarp();
         }
-        tmem_wait_ld();
-        tc_fence_before();
-        arrive(SPLASH_KBAR(s_free, buf));  // the scores of tile step + 2 may come
-        if constexpr (QUANT) {
+        if (__builtin_expect(!plain, 0) && tree && !see_tree(seg)) { ok = false; break; }
+        auto prepare = [&](int h) {
+          if constexpr (QUANT) {
 #pragma unroll
-          for (int j = 0; j < L::kKeys; j += 4) {
-            const uint4 k4 = lds128(my_scales + j * 4);
-            const float2 x = mul2(make_float2(sv[j], sv[j + 1]), make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)));
-            const float2 y = mul2(make_float2(sv[j + 2], sv[j + 3]), make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)));
-            sv[j] = x.x; sv[j + 1] = x.y; sv[j + 2] = y.x; sv[j + 3] = y.y;
+            for (int j = 0; j < L::kPart; j += 4) {
+              const uint4 k4 = lds128(my_scales + (h * L::kPart + j) * 4);
+              const float2 x = mul2(make_float2(sv[j], sv[j + 1]), make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)));
+              const float2 y = mul2(make_float2(sv[j + 2], sv[j + 3]), make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)));
+              sv[j] = x.x; sv[j + 1] = x.y; sv[j + 2] = y.x; sv[j + 3] = y.y;
+            }
           }
-        }
-        if (__builtin_expect(a.soft_cap > 0.f, 0)) {
+          if (__builtin_expect(a.soft_cap > 0.f, 0)) {
 #pragma unroll
-          for (int j = 0; j < L::kKeys; ++j) sv[j] = tanh_approx(sv[j] * q_mul);
+            for (int j = 0; j < L::kPart; ++j) sv[j] = tanh_approx(sv[j] * q_mul);
+          }
+          if (__builtin_expect(!plain, 0)) {
+#pragma unroll
+            for (int c = 0; c < L::kPart / 32; ++c) {
+              const int at = col0 + h * L::kPart + c * 32, kb = key0 + at;
+              uint32_t vis = bit_run(v_lo - kb, v_hi - kb) | bit_run(-kb, v_sink - kb);
+              const int d0 = kb - g.before;
+              if (tree && d0 > -32 && d0 < kCachedMaxTree) {
+                const uint32_t w = above + (1 + (d0 >> 5)) * 4;
+                if (live) vis |= __funnelshift_r(lds32(w), lds32(w + 4), d0 & 31);
+              }
+              if (piece_shift >= 5) {
+                if (!((good >> (at >> piece_shift)) & 1u)) vis = 0;
+              } else {
+                if (!((good >> (at / 16)) & 1u)) vis &= 0xffff0000u;
+                if (!((good >> (at / 16 + 1)) & 1u)) vis &= 0x0000ffffu;
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!((vis >> j) & 1u)) sv[c * 32 + j] = -INFINITY;
+            }
+          }
+        };
+        const float2 mul_2 = make_float2(mul, mul);
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+        for (int h = L::kParts - 1; h >= 0; --h) {
+          if (h < L::kParts - 1) fetch(h);
+          fetched(L::kParts == 1);
+          prepare(h);
+#pragma unroll
+          for (int j = 0; j < L::kPart; j += 4) {
+            if constexpr (QUANT) {
+              const uint4 e4 = lds128(my_scales + (L::kKeys + h * L::kPart + j) * 4);
+              const float2 x = fma2(make_float2(sv[j], sv[j + 1]), mul_2, make_float2(__uint_as_float(e4.x), __uint_as_float(e4.y)));
+              const float2 y = fma2(make_float2(sv[j + 2], sv[j + 3]), mul_2, make_float2(__uint_as_float(e4.z), __uint_as_float(e4.w)));
+              mx0 = max3(mx0, x.x, x.y);
+              mx1 = max3(mx1, y.x, y.y);
+            } else {
+              mx0 = max3(mx0, sv[j], sv[j + 1]);
+              mx1 = max3(mx1, sv[j + 2], sv[j + 3]);
+            }
+          }
         }
         if (__builtin_expect(!plain, 0)) {
-          if (tree && !see_tree(seg)) { ok = false; break; }
-#pragma unroll
-          for (int c = 0; c < L::kKeys / 32; ++c) {
-            const int at = col0 + c * 32, kb = key0 + at;
-            uint32_t vis = bit_run(v_lo - kb, v_hi - kb) | bit_run(-kb, v_sink - kb);
-            const int d0 = kb - g.before;
-            if (tree && d0 > -32 && d0 < kCachedMaxTree) {
-              const uint32_t w = above + (1 + (d0 >> 5)) * 4;
-              if (live) vis |= __funnelshift_r(lds32(w), lds32(w + 4), d0 & 31);
-            }
-            if (piece_shift >= 5) {
-              if (!((good >> (at >> piece_shift)) & 1u)) vis = 0;
-            } else {
-              if (!((good >> (at / 16)) & 1u)) vis &= 0xffff0000u;
-              if (!((good >> (at / 16 + 1)) & 1u)) vis &= 0x0000ffffu;
-            }
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (!((vis >> j) & 1u)) sv[c * 32 + j] = -INFINITY;
-          }
           // Values that no row sees are cleared: their probability is 0, and 0 times what lies there may be NaN.
           const uint32_t clear = __ballot_sync(0xffffffffu, !there(row_lane));
           if (clear) {
@@ -472,21 +504,6 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         }
 
         // ---- online softmax with a maximum that may lag behind ----
-        const float2 mul_2 = make_float2(mul, mul);
-        float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < L::kKeys; j += 4) {
-          if constexpr (QUANT) {
-            const uint4 e4 = lds128(my_scales + (L::kKeys + j) * 4);
-            const float2 x = fma2(make_float2(sv[j], sv[j + 1]), mul_2, make_float2(__uint_as_float(e4.x), __uint_as_float(e4.y)));
-            const float2 y = fma2(make_float2(sv[j + 2], sv[j + 3]), mul_2, make_float2(__uint_as_float(e4.z), __uint_as_float(e4.w)));
-            mx0 = max3(mx0, x.x, x.y);
-            mx1 = max3(mx1, y.x, y.y);
-          } else {
-            mx0 = max3(mx0, sv[j], sv[j + 1]);
-            mx1 = max3(mx1, sv[j + 2], sv[j + 3]);
-          }
-        }
         float top = fmaxf(mx0, mx1);
         if constexpr (!QUANT) top *= mul;
         if (i > 0) {
@@ -516,14 +533,22 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         // columns behind the first.
 #pragma unroll
         for (int c = 0; c < L::kKeys / 32; ++c) {
+          constexpr int kChunks = L::kPart / 32;
+          const int in_part = c % kChunks * 32;  // (the loop is unrolled)
+          if (c >= kChunks && c % kChunks == 0) {
+            fetch(c / kChunks);
+            fetched(c / kChunks == L::kParts - 1);
+            prepare(c / kChunks);
+          }
           if constexpr (QUANT) {
             uint32_t p1[8], p2[8], p3[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const int at = c * 32 + j * 4;
               const uint4 v4 = lds128(my_scales + (2 * L::kKeys + at) * 4);
-              const float2 x = fma2(make_float2(sv[at], sv[at + 1]), mul_2, shift_2);
-              const float2 y = fma2(make_float2(sv[at + 2], sv[at + 3]), mul_2, shift_2);
+              const int in = in_part + j * 4;
+              const float2 x = fma2(make_float2(sv[in], sv[in + 1]), mul_2, shift_2);
+              const float2 y = fma2(make_float2(sv[in + 2], sv[in + 3]), mul_2, shift_2);
               const float2 ex = make_float2(ex2_approx(x.x), ex2_approx(x.y)), ey = make_float2(ex2_approx(y.x), ex2_approx(y.y));
               sum_a = add2(sum_a, ex);
               sum_b = add2(sum_b, ey);
@@ -558,7 +583,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             uint32_t pk[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              const float2 x = fma2(make_float2(sv[c * 32 + 2 * j], sv[c * 32 + 2 * j + 1]), mul_2, shift_2);
+              const float2 x = fma2(make_float2(sv[in_part + 2 * j], sv[in_part + 2 * j + 1]), mul_2, shift_2);
               const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
               if (j & 1) sum_b = add2(sum_b, e); else sum_a = add2(sum_a, e);
               pk[j] = pack2<BF16>(e.x, e.y);
