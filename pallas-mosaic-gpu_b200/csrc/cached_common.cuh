@@ -195,6 +195,30 @@ __device__ __forceinline__ void umma8_ts2_w(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
+// Probabilities as operands of 8 bits.  A number of f16 is a sum of numbers of e5m2: its upper byte is one (sign, exponent, the
+// first 2 of 10 bits, subnormals alike), what that leaves is a number of f16 again and needs no rounding, and so on, 3 bits each.
+// Four hold all of it, three round it to 9 bits; every one is a float of its own, so what is small loses nothing beside what is
+// large, down to e5m2's lowest step, 2^-16.  Two pairs of f16 to TERMS words of four codes.
+template <int TERMS>
+__device__ __forceinline__ void e5m2_terms(uint32_t a, uint32_t b, uint32_t* codes) {
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    if (t == TERMS - 1) {  // to nearest (numbers that are left over are far from the carry into the sign, but for NaN)
+      a += 0x00800080u;
+      b += 0x00800080u;
+    }
+    codes[t] = __byte_perm(a, b, 0x7531);
+    if (t < TERMS - 1) {
+      asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(a) : "r"(a & 0xff00ff00u));
+      asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(b) : "r"(b & 0xff00ff00u));
+    }
+  }
+}
+// Probabilities are scaled so that a row's largest 2^ev p stands at 2^12, or up to 2^kCachedLag8 above while the maximum lags behind
+// (f16 and e5m2 end below 2^16): what is lost of a small one is half of 2^-16, 2^-29 of the row's largest or less.
+constexpr float kCachedLag8 = 3.f;
+constexpr float kCachedPScale8 = 4096.f;
+
 // Upper half of a shared-memory descriptor of tiles with 128- or 64-byte rows, swizzled over their rows.
 template <int BOX_BYTES>
 __host__ __device__ constexpr uint32_t cached_desc_hi() {

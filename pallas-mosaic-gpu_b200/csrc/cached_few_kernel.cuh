@@ -13,8 +13,8 @@
 // four warps reduce, agree on new maxima and rescale their warpgroup's O.  The two warpgroups take the tiles in turn, each
 // with maxima, sums and O of its own, joined at the end of a segment.
 //
-// Q is 2 (bf16) or 3 (f16) e4m3 terms side by side in B, whose columns of S are added; P is as many, p1 + p2 / 16 + p3 / 256,
-// side by side as well, whose columns of O are added with those factors.
+// Q is 2 (bf16) or 3 (f16) e4m3 terms side by side in B, whose columns of S are added; P is 3 (bf16) or 4 (f16) terms of e5m2 (see
+// e5m2_terms), side by side as well, whose columns of O are added.
 //
 // Maxima and factors of the rows are in shared memory between the tiles: with them in registers 16 rows need more than a thread
 // has, and what is spilled comes back from L2, as shared memory leaves the L1 cache next to nothing (173 us instead of 105).
@@ -31,7 +31,7 @@ template <int D, bool BF16, int R>
 struct CachedFewLayout {
   static constexpr int kTerms = BF16 ? 2 : 3;
   static constexpr int kSCols = (kTerms * R + 15) / 16 * 16;  // N of the scores: a multiple of 16
-  static constexpr int kPTerms = BF16 ? 2 : 3;
+  static constexpr int kPTerms = BF16 ? 3 : 4;
   static constexpr int kOCols = (kPTerms * R + 15) / 16 * 16;  // N of P V
   static constexpr int kItem = 1, kRowBytes = D, kBoxBytes = D, kBoxes = 1, kBoxElems = D;  // a key: one box of 64 or 128 bytes
   static constexpr int kSlotBytes = kCachedTile * kRowBytes;
@@ -134,7 +134,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       constexpr uint32_t kHi = cached_desc_hi<L::kBoxBytes>();
       constexpr uint32_t kPHi = desc_hi_plain(L::kPBlock);  // N-major without swizzle
       constexpr uint32_t kIdescS = make_idesc(false, 128, L::kSCols, false, false);
-      constexpr uint32_t kIdescO = make_idesc(false, 128, L::kOCols, true, true);
+      constexpr uint32_t kIdescO = make_idesc(false, 128, L::kOCols, true, true) | (1u << 10);  // B is e5m2
       // An MMA takes 32 of a key's numbers, or 32 keys.  V^T has 128 rows; at head_dim 64 they are the 64 of its box twice, whose
       // second half is not read (distance 0 from one box to the next).
       const int tiles = cached_share_tiles(a, cur);
@@ -232,8 +232,8 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     const bool capped = a.soft_cap > 0.f;
     // What takes a score to powers of 2, or to the argument of the soft-cap and from there to powers of 2.
     const float pre = capped ? 1.f / a.soft_cap : kCachedLog2e, post = a.soft_cap * kCachedLog2e;
-    constexpr float kThreshold = 3.f;  // powers of 2 by which the maxima may lag behind
-    constexpr float kPScale = 32.f;    // P up to 2^3 * 32 of e4m3's 448
+    constexpr float kThreshold = kCachedLag8;  // powers of 2 by which the maxima may lag behind
+    constexpr float kPScale = kCachedPScale8;
     uint32_t sync_par = 0;
     int step0 = 0;           // tiles of the CTA in front of the segment
     int trees = 0, last_b = -1;
@@ -411,12 +411,14 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           }
         }
         // ---- does a score stand above the maxima by more than they may lag? ----
-        float m[R];
-#pragma unroll
-        for (int r = 0; r < R; r += 4) load4(my_state + r * 4, m + r);
         bool above = false;
 #pragma unroll
-        for (int r = 0; r < R; ++r) above = above || x[r] + v_exp > m[r] + kThreshold;  // (-inf + lag is -inf)
+        for (int r = 0; r < R; r += 4) {
+          float m[4];
+          load4(my_state + r * 4, m);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) above = above || x[r + k] + v_exp > m[k] + kThreshold;  // (-inf + lag is -inf)
+        }
         bool move;
         if (!vote(__any_sync(0xffffffffu, above), move)) { ok = false; break; }
         if (__builtin_expect(move, 0)) {
@@ -436,7 +438,9 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           // O may be touched once P V of this warpgroup's previous tile is done.
           if (i >= 2 && !warp_wait(SPLASH_KBAR(pv_done, grp), ((step - 2) >> 1) & 1, ctx, kCSiteSmxO, step)) { ok = false; break; }
           tc_fence_after();
-          float alpha[R];
+          float alpha[R], m[R];
+#pragma unroll
+          for (int r = 0; r < R; r += 4) load4(my_state + r * 4, m + r);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             float t = -INFINITY;
@@ -473,28 +477,19 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         uint32_t pk[L::kOCols / 4] = {};
 #pragma unroll
         for (int r = 0; r < R; r += 4) {
-          float p[4];
+          float p[4], m[4];
+          load4(my_state + r * 4, m);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float shift = m[r + k] == -INFINITY ? 0.f : -m[r + k];
+            const float shift = m[k] == -INFINITY ? 0.f : -m[k];
             const float e = ex2_approx(x[r + k] + shift);
             l[r + k] += e;
             p[k] = e * v_scale;
           }
-          // The first term is P rounded to four bits, in integer arithmetic: its code need not be read back.  The next is what
-          // is left, times 16, and f16's third what that leaves, times 16 once more.
-          const float2 a0 = make_float2(p[0], p[1]), a1 = make_float2(p[2], p[3]);
-          const float2 h0 = four_bits(a0), h1 = four_bits(a1);
-          const float2 r0 = mul2(sub2(a0, h0), make_float2(16.f, 16.f)), r1 = mul2(sub2(a1, h1), make_float2(16.f, 16.f));
-          pk[r / 4] = e4m3x2(h0.x, h0.y) | (e4m3x2(h1.x, h1.y) << 16);
-          if constexpr (L::kPTerms == 2) {
-            pk[R / 4 + r / 4] = e4m3x2(r0.x, r0.y) | (e4m3x2(r1.x, r1.y) << 16);
-          } else {
-            const float2 g0 = e4m3_steps(four_bits(r0)), g1 = e4m3_steps(four_bits(r1));
-            const float2 t0 = mul2(sub2(r0, g0), make_float2(16.f, 16.f)), t1 = mul2(sub2(r1, g1), make_float2(16.f, 16.f));
-            pk[R / 4 + r / 4] = e4m3x2(g0.x, g0.y) | (e4m3x2(g1.x, g1.y) << 16);
-            pk[R / 2 + r / 4] = e4m3x2(t0.x, t0.y) | (e4m3x2(t1.x, t1.y) << 16);
-          }
+          uint32_t codes[L::kPTerms];
+          e5m2_terms<L::kPTerms>(pack2<false>(p[0], p[1]), pack2<false>(p[2], p[3]), codes);
+#pragma unroll
+          for (int t = 0; t < L::kPTerms; ++t) pk[t * (R / 4) + r / 4] = codes[t];
         }
         // P's room is free once P V of this warpgroup's previous tile is done.
         if (step >= 2 && !warp_wait(SPLASH_KBAR(pv_done, grp), ((step - 2) >> 1) & 1, ctx, kCSiteSmxP, step)) { ok = false; break; }
@@ -577,7 +572,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           auto all_terms = [&](const uint32_t* o) {
             float x = __uint_as_float(o[(L::kPTerms - 1) * 8 + k]);
 #pragma unroll
-            for (int t = L::kPTerms - 2; t >= 0; --t) x = fmaf(x, 1.f / 16, __uint_as_float(o[t * 8 + k]));
+            for (int t = L::kPTerms - 2; t >= 0; --t) x += __uint_as_float(o[t * 8 + k]);
             return x;
           };
           if (has[0]) value = all_terms(o0) * w0_r;
