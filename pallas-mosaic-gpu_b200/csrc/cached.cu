@@ -104,16 +104,14 @@ static int check_cached(const SplashCachedParams* p) {
 }
 
 // Rows per tile: as few as hold the call's.  8-bit caches take the kernel whose MMA rows are keys (cached_few_kernel.cuh) with up
-// to 8 rows, and with up to 16 where the products of the copies would bound the other (cached_kernel.cuh): in f16, whose P has
-// three terms, and at head_dim 128 where a unit may see 8192 keys or more.  us with 16 rows, few | copies, for 32 sequences of
-// 8192 keys and for 64 of 100 to 3000, 8 kv heads: f16 120 | 169, 89 | 95 (head_dim 64: 116 | 145, 78 | 79); bf16 105 | 127,
-// 78 | 69 (head_dim 64: 102 | 102, 71 | 58); windows of 4096 121 | 118.
+// to 16 rows, above which the other (cached_kernel.cuh) has at most 4 copies.  us with 16 rows in bf16, few | copies, from L2
+// flushed: 32 sequences of 8192 keys, 8 kv heads 129 | 170 (head_dim 64: 115 | 141), 64 of 100 to 3000 keys 86 | 98 (78 | 82),
+// 64 windows of 4096 keys with a soft-cap 160 | 186.
 static CachedPlan cached_plan(const SplashCachedParams& p) {
   CachedPlan plan;
   const int64_t rows = static_cast<int64_t>(p.heads / p.kv_heads) * p.n;
   const int64_t capacity = static_cast<int64_t>(p.table_width) * p.page_size;
-  const bool sees_many = capacity >= 8192 && (p.window_left < 0 || p.window_left >= 8192);
-  const bool few = p.quantized && (rows <= 8 || (rows <= 16 && (p.dtype == SPLASH_DTYPE_F16 || (p.head_dim == 128 && sees_many))));
+  const bool few = p.quantized && rows <= 16;
   plan.row_cap = few ? (rows <= 8 ? 8 : 16) : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   // A unit stands in the line by as many tiles more as its start and the sum of its parts take.  us for 64 sequences of 100 to
   // 3000 keys, 8 kv heads, head_dim 128, with a cost of 2 | 4 | 8 | 12: 4 rows 80 | 80 | 82 | 86, 128 rows 138 | 124 | 113 |

@@ -158,12 +158,6 @@ __device__ __forceinline__ float exponent_scale(int e) {  // -128 marks a row th
   return e == -128 ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
-// Rounded to four significant bits.
-__device__ __forceinline__ float2 four_bits(float2 x) {
-  return make_float2(__uint_as_float((__float_as_uint(x.x) + 0x80000u) & 0xfff00000u),
-                     __uint_as_float((__float_as_uint(x.y) + 0x80000u) & 0xfff00000u));
-}
-
 // Warp-collective forms as in ptx.cuh, for 8-bit operands (kind::f8f6f4, e4m3 by e4m3).
 __device__ __forceinline__ void umma8_ss2_w(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
                                             uint32_t idesc, uint32_t accumulate) {
@@ -263,11 +257,6 @@ template <int N>
 __device__ __forceinline__ void sts_bytes(uint32_t addr, uint32_t v) {
   if constexpr (N == 4) sts32(addr, v);
   else asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(static_cast<uint16_t>(v)) : "memory");
-}
-// Numbers of four bits and below 2^13, to the steps of e4m3's subnormals where they are among those: what e4m3 holds of them.
-__device__ __forceinline__ float2 e4m3_steps(float2 x) {
-  const float2 c = make_float2(0x1.8p14f, 0x1.8p14f);  // its last bit is 2^-9
-  return sub2(add2(x, c), c);
 }
 __device__ __forceinline__ int lds_s8(uint32_t addr) {
   int v;

@@ -1,15 +1,15 @@
-// Attention over an 8-bit paged cache for few rows: up to 8 or 16 new tokens x heads of a kv head, as in token-by-token decoding.
+// Attention over an 8-bit paged cache for few rows: up to 16 new tokens x heads of a kv head, as in token-by-token decoding.
 //
 // cached_kernel.cuh spends an MMA's 128 rows on copies of the few rows there are, and its products then take about as long as
 // an 8-bit tile's transfer (32 sequences of 2000 to 32768 keys, 64 / 8 heads: 278 us; here 196).  Here the keys are the 128
 // rows instead:
 //   S^T = K Q^T       [128 keys x rows]        A = K as it lies in the cache, B = Q, 16 to 48 columns
-//   O^T += V^T P^T    [head_dim x rows]        A = V^T (V read M-major), B = P^T, which a key's thread writes as 16 to 48 bytes
-// An MMA costs its 4 KB of A, 32 cycles: 256 a tile, where the copies cost 1024.  A thread has one key and all rows: the
+//   O^T += V^T P^T    [head_dim x rows]        A = V^T (V read M-major), B = P^T, which a key's thread writes as 32 to 64 bytes
+// An MMA costs its 4 KB of A, 32 cycles: 256 a tile, where the copies cost 1280.  A thread has one key and all rows: the
 // scales of the key and its value are two numbers of its own, and no exponential is computed twice.
 //
 // The rows' maxima lie across the threads now.  They are not looked for: a thread compares its scores with the lagging maxima
-// (registers, the same in every thread of a warpgroup), and only if one of the warpgroup's threads is above by 2^lag do the
+// (the same in every warp of a warpgroup), and only if one of the warpgroup's threads is above by 2^lag do the
 // four warps reduce, agree on new maxima and rescale their warpgroup's O.  The two warpgroups take the tiles in turn, each
 // with maxima, sums and O of its own, joined at the end of a segment.
 //

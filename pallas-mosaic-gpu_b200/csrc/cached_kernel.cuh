@@ -4,8 +4,9 @@
 // the kv head -- against the keys its rows can see, in tiles of 128 keys:  S = Q K^T, online softmax, O += P V.
 //
 // What bounds it: HBM with up to 64 rows over a 16-bit cache (16 sequences of 4000 to 32768 keys, 32 / 8 heads: 188 us, 98 % of
-// the copy bandwidth); the products over an 8-bit one, whose tiles take 1390 cycles to arrive and 1024 or more to multiply (16
-// rows, windows of 4096: 117 us, 54 %); with more rows the start and end of a unit, and the exponentials.  2 * 128 * head_dim
+// the copy bandwidth); the products over an 8-bit one, whose tiles take 1390 cycles to arrive and 1280 (f16: 1792) or more to
+// multiply (64 rows, 32 sequences of 8192 keys, 8 kv heads: 211 us, f16 246; the bytes are 83); with more rows the start and end of
+// a unit, and the exponentials.  2 * 128 * head_dim
 // numbers a tile are read once for all rows, so everything is arranged to keep a ring of loads full:
 //   * The tiles of all units stand in one line that is cut into equal shares, one per CTA (one CTA per SM), whatever the
 //     lengths of the sequences are.  A unit that several CTAs share leaves partial results (unnormalised O, maximum and
@@ -26,11 +27,13 @@
 //   * q * 2^-eq = q1 + q2 (+ q3 for f16), each term what the ones before leave; S sums their products.  bf16 has 8 bits,
 //     a term 4: nothing is lost but below 2^-18 of the row's largest number.
 //   * 2^ek of a key scales its column of S; 2^ev of a value scales its column of P, and the running maximum is one of
-//     s + ev and lags behind by a factor of 8 at most, so that the scaled probabilities end between 32 and 256.
-//   * P = p1 + p2 with p1, p2 e4m3: 8 bits as a bf16 P has, down to 2^-7 of the row's largest scaled probability; below
-//     that the steps stay at 2^-14 of it or less.  f16 takes a third term (two lose it 3 bits: 6e-4 of a result's size
-//     against 2e-4), for which tensor memory has no columns left: it lies where the tile's scores did, and the scores of tile
-//     t + 2 wait for P V of tile t (64 rows, 32 sequences of 8192 keys, 8 kv heads, head_dim 128: 236 us, bf16 156).
+//     s + ev and lags behind by a factor of 8 at most, so that a row's largest scaled probability stands at 2^12 to 2^15.
+//   * P is rounded to f16 and cut into e5m2 terms (e5m2_terms), three for bf16 (9 bits, where a bf16 P has 8) and four for f16 (all
+//     of it).  Every probability down to 2^-18 of the row's largest keeps these bits and every one down to 2^-29 some: many
+//     small ones beside a large one add up to what they should.  Two terms of e4m3 would be one product less, but their steps
+//     end at 2^-14 of the largest, and with the tail of a softmax goes its mass (one key of 32768 with weight 0.4: results off by a
+//     third).  Tensor memory has columns for two terms; the others lie where the tile's scores did, and the scores of tile t + 2
+//     wait for P V of tile t.
 #pragma once
 
 #include "cached_common.cuh"
@@ -47,8 +50,8 @@ struct CachedLayout {
   static constexpr int kBoxes = kRowBytes / kBoxBytes;
   static constexpr int kBoxElems = kBoxBytes / kItem;
   static constexpr int kSlotBytes = kCachedTile * kRowBytes;
-  static constexpr int kTerms = QUANT ? (BF16 ? 2 : 3) : 1;  // of Q, and of P
-  static constexpr bool kThird = kTerms == 3;
+  static constexpr int kTerms = QUANT ? (BF16 ? 2 : 3) : 1;   // of Q
+  static constexpr int kPTerms = QUANT ? (BF16 ? 3 : 4) : 1;  // of P
   static constexpr int kQTerm = 128 * kRowBytes;
   static constexpr int kQBytes = kTerms * kQTerm;
   static constexpr int kStageStride = 36;                  // words per row of the staging area (32 used)
@@ -70,7 +73,7 @@ struct CachedLayout {
   // Scores that a thread has in registers at a time.  With all 128 of a row without copies it has registers for little else, and
   // what is spilled comes back from L2, as shared memory leaves the L1 cache next to nothing: halves are read from tensor memory
   // for the maximum, and the second once more for the exponentials (64 sequences of 100 to 3000 keys, 8 kv heads, 192 rows: 191 ->
-  // 172 us; 8 bit, where a half is also scaled twice, 343 -> 326).
+  // 172 us; 8 bit, where a half is also scaled twice, 343 -> 326 with a P of two terms).
   static constexpr int kPart = kKeys < 64 ? kKeys : 64, kParts = kKeys / kPart;
   static constexpr int kSoftmaxRegs = 184, kLoadRegs = 136;  // 384 * 168 at launch = 256 * 184 + 128 * 136
 };
@@ -154,7 +157,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       // ------------------------------------------ products -----------------------------------------------------------
       constexpr uint32_t kHi = cached_desc_hi<L::kBoxBytes>();
       constexpr uint32_t kIdescQK = make_idesc(BF16 && !QUANT, 128, kCachedTile, false, false);
-      constexpr uint32_t kIdescPV = make_idesc(BF16 && !QUANT, 128, D, false, true);
+      constexpr uint32_t kIdescPV = make_idesc(BF16 && !QUANT, 128, D, false, true) | (QUANT ? 1u << 7 : 0u);  // P: e5m2
       constexpr int kStepsPerBox = L::kBoxBytes / 32;  // an MMA takes 32 bytes of K per row
       const int tiles = cached_share_tiles(a, cur);
       CachedWalk qk, pv;
@@ -166,7 +169,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           const int buf = qk.step & 1, slot = qk.step % L::kSlots;
           const bool ready = mbar_probe(SPLASH_KBAR(k_full, slot), (qk.step / L::kSlots) & 1) &&
                              (qk.step < 2 || mbar_probe(SPLASH_KBAR(s_free, buf), ((qk.step - 2) >> 1) & 1)) &&
-                             (!L::kThird || qk.step < 2 || mbar_probe(SPLASH_KBAR(pv_done, buf), ((qk.step - 2) >> 1) & 1)) &&
+                             (!QUANT || qk.step < 2 || mbar_probe(SPLASH_KBAR(pv_done, buf), ((qk.step - 2) >> 1) & 1)) &&
                              (qk.i > 0 || mbar_probe(SPLASH_KBAR(q_full, 0), qk.seg & 1));
           if (__all_sync(0xffffffffu, ready)) {
             tc_fence_after();
@@ -201,10 +204,10 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             const uint32_t b_lo = desc_lo(v_u32 + slot * L::kSlotBytes, kCachedTile * L::kBoxBytes);
             const uint32_t p_tmem = tmem + L::kPCol + buf * 64;
             constexpr int kKeysPerMma = QUANT ? 32 : 16;
-            // P is 8 columns an MMA; 8 bit: its second term follows in columns 32 .. 63, the third where the scores were, on the
+            // P is 8 columns an MMA; 8 bit: its second term follows in columns 32 .. 63, the others where the scores were, on the
             // same values.
 #pragma unroll
-            for (int kk = 0; kk < L::kTerms * kCachedTile / kKeysPerMma; ++kk) {
+            for (int kk = 0; kk < L::kPTerms * kCachedTile / kKeysPerMma; ++kk) {
               const uint32_t off = ((kk * kKeysPerMma) % kCachedTile * L::kBoxBytes) >> 4;
               const uint32_t p_at = kk < 8 ? p_tmem + kk * 8 : tmem + buf * 128 + (kk - 8) * 8;
               if constexpr (QUANT) umma8_ts2_w(tmem + L::kOCol, p_at, b_lo + off, kHi, kIdescPV, pv.i > 0 || kk > 0);
@@ -291,8 +294,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     const float inv_cap = a.soft_cap > 0.f ? 1.f / a.soft_cap : 1.f;
     // Powers of 2 by which the maximum may lag behind before O is rescaled, which takes about a tile's time.  8 bit: with a
     // lag of 2^1 every third tile rescales (32 x 64 heads, 2000 to 32768 keys: 272 us), with 2^3 hardly one.
-    constexpr float kThreshold = QUANT ? 3.f : 8.f;
-    constexpr float kPScale = QUANT ? 32.f : 1.f;            // 8 bit: P up to 2^3 * 32 of e4m3's 448
+    constexpr float kThreshold = QUANT ? kCachedLag8 : 8.f;
+    constexpr float kPScale = QUANT ? kCachedPScale8 : 1.f;
     uint32_t sync_par = 0;
     int step0 = 0;   // tiles of the CTA in front of the segment
     bool ok = true;
@@ -531,8 +534,8 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         const float shift = m_run == -INFINITY ? 0.f : -m_run;
         const float2 shift_2 = make_float2(shift, shift);
         float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
-        // P is written 32 keys at a time: 16 columns of 16-bit numbers, or 8 columns of either e4m3 term, the second term 32
-        // columns behind the first.
+        // P is written 32 keys at a time: 16 columns of 16-bit numbers, or 8 columns of every e5m2 term, each 32 columns behind
+        // the one before.
 #pragma unroll
         for (int c = 0; c < L::kKeys / 32; ++c) {
           constexpr int kChunks = L::kPart / 32;
@@ -543,7 +546,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             prepare(c / kChunks);
           }
           if constexpr (QUANT) {
-            uint32_t p1[8], p2[8], p3[8];
+            uint32_t codes[8][L::kPTerms];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const int at = c * 32 + j * 4;
@@ -556,29 +559,24 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
               sum_b = add2(sum_b, ey);
               const float2 px = mul2(ex, make_float2(__uint_as_float(v4.x), __uint_as_float(v4.y)));
               const float2 py = mul2(ey, make_float2(__uint_as_float(v4.z), __uint_as_float(v4.w)));
-              // The first term is P rounded to four bits, in integer arithmetic: its code need not be read back.
-              const float2 hx = four_bits(px), hy = four_bits(py);
-              const float2 rx = sub2(px, hx), ry = sub2(py, hy);
-              p1[j] = e4m3x2(hx.x, hx.y) | (e4m3x2(hy.x, hy.y) << 16);
-              if constexpr (!L::kThird) {
-                p2[j] = e4m3x2(rx.x, rx.y) | (e4m3x2(ry.x, ry.y) << 16);
-              } else {
-                const float2 gx = e4m3_steps(four_bits(rx)), gy = e4m3_steps(four_bits(ry));
-                const float2 tx = sub2(rx, gx), ty = sub2(ry, gy);
-                p2[j] = e4m3x2(gx.x, gx.y) | (e4m3x2(gy.x, gy.y) << 16);
-                p3[j] = e4m3x2(tx.x, tx.y) | (e4m3x2(ty.x, ty.y) << 16);
-              }
+              e5m2_terms<L::kPTerms>(pack2<false>(px.x, px.y), pack2<false>(py.x, py.y), codes[j]);
             }
-            tmem_st8(p_tmem + col0 / 4 + c * 8, p1);
-            tmem_st8(p_tmem + 32 + col0 / 4 + c * 8, p2);
-            if constexpr (L::kThird) {
-              // (The other copies' keys are scores here, and not zeros from the start.)
+#pragma unroll
+            for (int t = 0; t < L::kPTerms; ++t) {
+              uint32_t x[8];
+              if (t < 2) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = codes[j][t];
+                tmem_st8(p_tmem + t * 32 + col0 / 4 + c * 8, x);
+                continue;
+              }
+              // (The other copies' keys are scores here, and not zeros from the start.  Rows without copies have read the scores of
+              // columns 0 .. 63 when they write the first of these; the others they read from behind them.)
 #pragma unroll
               for (int other = 0; other < KG; ++other) {
-                uint32_t x[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = other == part ? p3[j] : 0u;
-                tmem_st8(s_tmem + other * (L::kKeys / 4) + c * 8, x);
+                for (int j = 0; j < 8; ++j) x[j] = other == part ? codes[j][t] : 0u;
+                tmem_st8(s_tmem + (t - 2) * 32 + other * (L::kKeys / 4) + c * 8, x);
               }
             }
           } else {

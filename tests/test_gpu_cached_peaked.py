@@ -74,7 +74,7 @@ def _check(*args):
 CASES = [(8192, 8.0, 0.0, 0), (32768, 11.0, 0.5, 5), (32768, 10.4, 0.0, -20000), (20000, 9.0, 1.0, -2)]
 
 
-# Rows = h / kvh * n.  Up to 8 (and for some 16) are served by the kernel whose MMA rows are keys.
+# Rows = h / kvh * n.  Up to 16 are served by the kernel whose MMA rows are keys.
 @pytest.mark.gpu
 @pytest.mark.parametrize("d,dtype", FORMS, ids=str)
 @pytest.mark.parametrize("h,kvh,n,batch", [(1, 1, 1, 150), (8, 2, 2, 75), (8, 1, 1, 5)])
@@ -84,6 +84,15 @@ def test_gpu_few_rows(d, dtype, h, kvh, n, batch, keys):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("d,dtype", [(128, torch.bfloat16), (128, torch.float16), (64, torch.float16)], ids=str)
-def test_gpu_16_rows_against_long_contexts(d, dtype):
+@pytest.mark.parametrize("d,dtype", FORMS, ids=str)
+def test_gpu_16_rows(d, dtype):
   _check(d, dtype, 16, 1, 1, 150, *CASES[1])
+
+
+# Rows as the MMA's rows, with 4, 2 and 1 copies of them, and two tiles of rows.
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,dtype", FORMS, ids=str)
+@pytest.mark.parametrize("h,kvh,n,batch", [(20, 1, 1, 150), (16, 2, 7, 75), (100, 1, 1, 150), (48, 2, 8, 40)])
+@pytest.mark.parametrize("keys", CASES, ids=str)
+def test_gpu_many_rows(d, dtype, h, kvh, n, batch, keys):
+  _check(d, dtype, h, kvh, n, batch, *keys)
