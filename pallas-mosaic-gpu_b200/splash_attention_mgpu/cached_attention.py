@@ -39,6 +39,9 @@ class CachedAttentionKernel:
     self.mask_value = mask_value
     self._calls: dict = {}
 
+  def __getstate__(self):
+    return {**self.__dict__, "_calls": {}}  # (what is kept of calls lies on their devices)
+
   def __repr__(self):
     return (f"CachedAttentionKernel(window_left={self.window_left}, num_sinks={self.num_sinks},"
             f" attn_logits_soft_cap={self.attn_logits_soft_cap})")

@@ -118,7 +118,8 @@ class KVCache:
   def head_dim(self) -> int:
     return self.k.shape[3]
 
-  def _params(self, page_table, lengths, batch, length, dtype) -> _ffi.SplashCacheParams:
+  def _params(self, page_table, batch, length, dtype) -> _ffi.SplashCacheParams:
+    """The parameter block of a call of this class, without its pointers."""
     if not self.k.is_cuda:
       raise RuntimeError("the cache works only on a CUDA (sm_100a) device; there is no CPU path.")
     if dtype not in _TORCH_DTYPES:
@@ -126,16 +127,19 @@ class KVCache:
     if not self.quantized and dtype != self.k.dtype:
       raise ValueError(f"the cache holds {self.k.dtype}, got {dtype}")
     p = _ffi.SplashCacheParams()
-    p.k_cache, p.v_cache = self.k.data_ptr(), self.v.data_ptr()
-    if self.quantized:
-      p.k_exponent, p.v_exponent = self.k_exponent.data_ptr(), self.v_exponent.data_ptr()
-      p.quantized = 1
-    p.page_table, p.lengths = page_table.data_ptr(), lengths.data_ptr()
+    p.quantized = self.quantized
     p.table_stride, p.table_width = page_table.stride(0), page_table.shape[1]
     p.batch, p.len = batch, length
     p.num_pages, p.kv_heads, p.page_size, p.head_dim = self.k.shape
     p.dtype = _TORCH_DTYPES[dtype]
     return p
+
+  def _point(self, p, page_table, lengths) -> None:
+    """Addresses of a call: never kept, so that a copy of a cache works on its own buffers."""
+    p.k_cache, p.v_cache = self.k.data_ptr(), self.v.data_ptr()
+    if p.quantized:
+      p.k_exponent, p.v_exponent = self.k_exponent.data_ptr(), self.v_exponent.data_ptr()
+    p.page_table, p.lengths = page_table.data_ptr(), lengths.data_ptr()
 
   def write(self, k, v, page_table, start, *, counts=None) -> None:
     """Stores new tokens: token j of sequence b becomes token start[b] + j of that sequence.
@@ -166,7 +170,7 @@ class KVCache:
       start = _index_tensor(start, "start", device, (batch,))
       if counts is not None:
         counts = _index_tensor(counts, "counts", device, (batch,))
-      p = self._params(page_table, start, batch, n, k.dtype)
+      p = self._params(page_table, batch, n, k.dtype)
       in_place = lambda x: x.stride(-1) == 1 and not any(s % 8 for s in x.stride()[:-1])
       if not (in_place(k) and in_place(v)) or any(x is not y for x, y in zip(as_given, (page_table, start, counts))):
         k, v = (x if in_place(x) else x.clone(memory_format=torch.contiguous_format) for x in (k, v))
@@ -176,7 +180,8 @@ class KVCache:
     if k.data_ptr() % 16 or v.data_ptr() % 16:
       return self.write(*(x.clone(memory_format=torch.contiguous_format) for x in (k, v)), page_table, start, counts=counts)
     p = _ffi.SplashCacheParams.from_buffer_copy(template)
-    p.k, p.v, p.page_table, p.lengths = k.data_ptr(), v.data_ptr(), page_table.data_ptr(), start.data_ptr()
+    self._point(p, page_table, start)
+    p.k, p.v = k.data_ptr(), v.data_ptr()
     if counts is not None:
       p.counts = counts.data_ptr()
     rc = _launch(self.k.device, _ffi.load().splash_cache_write, ctypes.byref(p))
@@ -197,7 +202,8 @@ class KVCache:
     max_len = int(max_len)
     if max_len < 0:
       raise ValueError(f"max_len must not be negative, got {max_len}")
-    p = self._params(page_table, lengths, batch, max_len, dtype)
+    p = self._params(page_table, batch, max_len, dtype)
+    self._point(p, page_table, lengths)
     shape = (batch, self.num_kv_heads, max_len, self.head_dim)
     k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
     p.k_out, p.v_out = k.data_ptr(), v.data_ptr()

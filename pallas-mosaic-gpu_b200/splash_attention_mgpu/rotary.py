@@ -61,6 +61,10 @@ class RotaryEmbedding:
                                   torch.tensor(self.axes, dtype=torch.int32, device=device))
     return self._device_tables[key]
 
+  def __getstate__(self):
+    # (a copy makes tables of its own, on whatever devices it is called)
+    return {**self.__dict__, "_device_tables": {}, "_calls": {}}
+
   # -- call --------------------------------------------------------------------
   def __call__(self, q, k, positions):
     """Rotated q (times q_scale) and k; `k` may be None, then the rotated q alone."""
@@ -113,8 +117,6 @@ class RotaryEmbedding:
     p.pairs, p.dtype = len(self.axes), _TORCH_DTYPES[q.dtype]
     p.adjacent, p.inverse, p.pos_is_64 = self.pairing == "adjacent", inverse, positions.dtype == torch.int64
     p.q_scale = self.q_scale
-    turns, axis = self._tables(q.device)
-    p.turns, p.axis = turns.data_ptr(), axis.data_ptr()
     return p
 
   def _run(self, q, k, positions, *, inverse):
@@ -134,6 +136,8 @@ class RotaryEmbedding:
     p = _ffi.SplashRotaryParams.from_buffer_copy(template)
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     p.q, p.q_out, p.positions = q.data_ptr(), q_out.data_ptr(), positions.data_ptr()
+    turns, axis = self._tables(q.device)
+    p.turns, p.axis = turns.data_ptr(), axis.data_ptr()
     k_out = None
     if k is not None:
       k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
