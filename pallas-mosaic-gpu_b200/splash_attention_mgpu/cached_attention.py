@@ -20,6 +20,7 @@ import math
 import os
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _ffi
 from .config import DEFAULT_MASK_VALUE
@@ -64,6 +65,8 @@ class CachedAttentionKernel:
       raise TypeError(f"cache must be a KVCache, got {type(cache).__name__}")
     if q.requires_grad and torch.is_grad_enabled():
       raise NotImplementedError("attention over the cache has no backward pass; call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(q).tangent is not None:
+      raise NotImplementedError("attention over the cache has no forward-mode derivative")
     if q.ndim == 3:
       out = self(q[None], cache, page_table, lengths, counts=counts, parents=parents, save_residuals=save_residuals)
       return (out[0][0], (out[1][0][0],)) if save_residuals else out[0]

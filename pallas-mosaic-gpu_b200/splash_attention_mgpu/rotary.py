@@ -7,7 +7,7 @@
 
 The attention kernels expect a pre-scaled q; `q_scale` is that factor, applied before the one rounding of the result.
 q and k may be views (a fused projection's output, transposed): only the last dimension has to be contiguous.  The
-results are contiguous [(B,) heads, S, head_dim], as the kernels want them.  Differentiable in q and k.
+results are contiguous [(B,) heads, S, head_dim], as the kernels want them.  Differentiable in q and k, backward and forward.
 
 No counterpart in the reference, whose callers rotate with JAX operations.
 """
@@ -20,6 +20,7 @@ from typing import Sequence
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _ffi
 from .splash_attention import _TORCH_DTYPES, _launch
@@ -71,11 +72,13 @@ class RotaryEmbedding:
     for x in (q, positions) if k is None else (q, k, positions):
       if not isinstance(x, torch.Tensor):
         raise TypeError("q, k and positions must be torch tensors")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-      out = _RotaryFn.apply(q, k, positions, self)
-    else:
-      out = self._run(q, k, positions, inverse=False)
+    out = self._rotate(q, k, positions, inverse=False)
     return out[0] if k is None else out
+
+  def _rotate(self, q, k, positions, *, inverse):
+    if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) or forward_ad._current_level >= 0:
+      return _RotaryFn.apply(q, k, positions, self, inverse)
+    return self._run(q, k, positions, inverse=inverse)
 
   def _params(self, q, k, positions, inverse):
     """The parameter block of a call with these shapes and strides, without its pointers."""
@@ -150,21 +153,30 @@ class RotaryEmbedding:
 
 
 class _RotaryFn(torch.autograd.Function):
-  """The gradient of a rotation is the rotation back: the positions are all that is kept."""
+  """Linear: the derivative along a direction is the rotation of that, the gradient the rotation back.  The positions are all that
+  is kept."""
 
   @staticmethod
-  def forward(ctx, q, k, positions, plan):
-    ctx.plan = plan
+  def forward(q, k, positions, plan, inverse):
+    return plan._run(q, k, positions, inverse=inverse)
+
+  @staticmethod
+  def setup_context(ctx, inputs, output):
+    _, _, positions, ctx.plan, ctx.inverse = inputs
     ctx.save_for_backward(positions)
+    ctx.save_for_forward(positions)
     ctx.set_materialize_grads(True)
-    return plan._run(q, k, positions, inverse=False)
 
   @staticmethod
-  @torch.autograd.function.once_differentiable
   def backward(ctx, dq, dk):
     (positions,) = ctx.saved_tensors
-    dq, dk = ctx.plan._run(dq, dk, positions, inverse=True)
-    return dq, dk, None, None
+    dq, dk = ctx.plan._rotate(dq, dk, positions, inverse=not ctx.inverse)
+    return dq, dk, None, None, None
+
+  @staticmethod
+  def jvp(ctx, dq, dk, *_):
+    (positions,) = ctx.saved_tensors
+    return ctx.plan._rotate(dq, dk, positions, inverse=ctx.inverse)
 
 
 def make_rotary(head_dim: int, sections: Sequence[int] | None = None, *, base: float = 10000.0,
