@@ -436,8 +436,8 @@ splash_bwd_col_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         const bool partial = a.block_kind[off] == SPLASH_BLOCK_PARTIAL;
         if (a.mask_desc && it.mask_head(it.g) != cur_mh) {
           cur_mh = it.mask_head(it.g);
-          band_lo = a.mask_desc[cur_mh * 4 + 0];
-          band_hi = a.mask_desc[cur_mh * 4 + 1];
+          band_lo = band_bound(a.mask_desc[cur_mh * 4 + 0]);
+          band_hi = band_bound(a.mask_desc[cur_mh * 4 + 1]);
           const int chunk = a.mask_desc[cur_mh * 4 + 2];
           if (chunk > 0) {
             // q must share the kv row's chunk: start <= q_pos <= start + chunk - 1.

@@ -277,8 +277,8 @@ splash_bwd_row_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       int sinks = 0;  // keys below this position are seen from behind the window too
       if (a.mask_desc) {
         sinks = a.mask_desc[mh * 4 + 3];
-        band_lo = a.mask_desc[mh * 4 + 0];
-        band_hi = a.mask_desc[mh * 4 + 1];
+        band_lo = band_bound(a.mask_desc[mh * 4 + 0]);
+        band_hi = band_bound(a.mask_desc[mh * 4 + 1]);
         const int chunk = a.mask_desc[mh * 4 + 2];
         if (chunk > 0) {
           const int start = (q_pos / chunk) * chunk;

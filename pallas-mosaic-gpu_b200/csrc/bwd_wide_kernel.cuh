@@ -680,8 +680,8 @@ splash_bwd_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
         if (a.mask_desc && mh != cur_mh) {
           cur_mh = mh;
-          band_lo = a.mask_desc[cur_mh * 4 + 0];
-          band_hi = a.mask_desc[cur_mh * 4 + 1];
+          band_lo = band_bound(a.mask_desc[cur_mh * 4 + 0]);
+          band_hi = band_bound(a.mask_desc[cur_mh * 4 + 1]);
           const int chunk = a.mask_desc[cur_mh * 4 + 2];
           if (chunk > 0) {
             // q must share the kv row's chunk: start <= q_pos <= start + chunk - 1.

@@ -562,6 +562,9 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
+// A bound of a band, of which no more is looked at than any sequence is long: sums with two positions do not wrap.
+__device__ __forceinline__ int band_bound(int x) { return min(max(x, -(1 << 30)), 1 << 30); }
+
 // Bits [from, to) of a word, as far as there are any.
 __device__ __forceinline__ uint32_t bit_run(int from, int to) {
   from = max(from, 0);

@@ -149,7 +149,7 @@ class CausalMask(_ComputableMask):
     self.offset = int(offset)
 
   def band(self):
-    return (BAND_NEG_INF, self.offset, 0)
+    return (BAND_NEG_INF, min(max(self.offset, BAND_NEG_INF), BAND_POS_INF), 0)
 
 
 class LocalMask(_ComputableMask):
@@ -173,7 +173,8 @@ class LocalMask(_ComputableMask):
     left, right = self.window_size
     lo = BAND_NEG_INF if left is None else self.offset - int(left)
     hi = BAND_POS_INF if right is None else self.offset + int(right)
-    return (lo, hi, 0)
+    # (No sequence is that long, and the kernels' sums of a bound and two positions stay within 31 bits.)
+    return (min(max(lo, BAND_NEG_INF), BAND_POS_INF), min(max(hi, BAND_NEG_INF), BAND_POS_INF), 0)
 
 
 class ChunkedCausalMask(_ComputableMask):
