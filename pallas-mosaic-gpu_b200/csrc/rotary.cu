@@ -3,8 +3,8 @@
 // Pair i of a row of x turns by theta_i = pos[axis(i)] * f_i:
 //   (a, b) -> scale * (a cos - b sin, b cos + a sin),        backward: the same with -sin.
 // The angle is kept in turns as a 64-bit fixed-point fraction: f_i / 2 pi rounded to 2^-64, times the whole position,
-// modulo 2^64.  The wrap of the product is the range reduction, so an angle is off by at most |pos| 2^-64 turns (and
-// 2^-25 half turns from the conversion to f32) whatever the position; sin and cos are then CUDA's sincospif.
+// modulo 2^64.  The wrap of the product is the range reduction, so an angle is off by at most |pos| 2^-65 turns (and
+// 2^-25 half turns from the conversion to f32, which is more up to positions of 2^39); sin and cos are then CUDA's sincospif.
 //
 // Bound: HBM, each number read and written once.  A thread holds the sines of VEC pairs of one position and takes
 // `chunk` heads of q and k with them, so that the ~40 instructions of a sine are shared by up to 8 heads; eight lanes

@@ -15,6 +15,7 @@ No counterpart in the reference, whose callers rotate with JAX operations.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Sequence
 
@@ -35,6 +36,29 @@ def _in_place(x):
   return x.stride(-1) == 1 and not any(s % 4 for s in x.stride()[:-1])
 
 
+@functools.lru_cache(maxsize=16)
+def _pi(bits: int) -> int:
+  """Pi in units of 2^-bits, within 2 of them: Machin's formula, pi = 16 atan(1/5) - 4 atan(1/239)."""
+  def atan_of_inverse(n):
+    power = (1 << (bits + 16)) // n
+    total, k = 0, 1
+    while power:
+      total += power // k if k % 4 == 1 else -(power // k)
+      power //= n * n
+      k += 2
+    return total
+
+  return (16 * atan_of_inverse(5) - 4 * atan_of_inverse(239)) >> 16
+
+
+def _turns(f: float) -> int:
+  """f / 2 pi modulo one turn in units of 2^-64, to nearest (in whole numbers: a double has 53 bits)."""
+  n, d = f.as_integer_ratio()
+  bits = 128 + max(0, 64 + n.bit_length() - d.bit_length())
+  den = d * _pi(bits)
+  return ((n << (64 + bits)) + den) // (2 * den) % (1 << 64)
+
+
 class RotaryEmbedding:
   """Rotation plan: which axis each pair of a row turns with, and how fast.  Made by `make_rotary`."""
 
@@ -45,9 +69,8 @@ class RotaryEmbedding:
     self.pairing = pairing
     self.q_scale = float(q_scale)
     self.num_axes = max(self.axes) + 1
-    # f / 2 pi modulo one turn, in units of 2^-64: the kernel's product with a position wraps where turns do.
-    turns = [int(math.fmod(f / (2 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64) for f in self.inv_freq]
-    self._turns = np.array(turns, np.uint64).view(np.int64)
+    # The kernel's product of these with a position wraps where turns do.
+    self._turns = np.array([_turns(f) for f in self.inv_freq], np.uint64).view(np.int64)
     self._device_tables: dict = {}
     self._calls: dict = {}
 
