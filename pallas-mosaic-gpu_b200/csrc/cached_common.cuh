@@ -210,8 +210,10 @@ __device__ __forceinline__ void e5m2_terms(uint32_t a, uint32_t b, uint32_t* cod
 }
 // Probabilities are scaled so that a row's largest 2^ev p stands at 2^12, or up to 2^kCachedLag8 above while the maximum lags behind
 // (f16 and e5m2 end below 2^16): what is lost of a small one is half of 2^-16, 2^-29 of the row's largest or less.
+// The exponentials, and with them the sums, carry 2^5 of that and the values' scales the rest: 2^ev goes up to 2^120.
 constexpr float kCachedLag8 = 3.f;
-constexpr float kCachedPScale8 = 4096.f;
+constexpr float kCachedExpBits8 = 5.f;
+constexpr float kCachedVScale8 = 128.f;
 
 // Upper half of a shared-memory descriptor of tiles with 128- or 64-byte rows, swizzled over their rows.
 template <int BOX_BYTES>

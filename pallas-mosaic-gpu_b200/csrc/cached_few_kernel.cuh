@@ -233,7 +233,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     // What takes a score to powers of 2, or to the argument of the soft-cap and from there to powers of 2.
     const float pre = capped ? 1.f / a.soft_cap : kCachedLog2e, post = a.soft_cap * kCachedLog2e;
     constexpr float kThreshold = kCachedLag8;  // powers of 2 by which the maxima may lag behind
-    constexpr float kPScale = kCachedPScale8;
+    constexpr float kVScale = kCachedVScale8, kExpBits = kCachedExpBits8;
     uint32_t sync_par = 0;
     int step0 = 0;           // tiles of the CTA in front of the segment
     int trees = 0, last_b = -1;
@@ -347,7 +347,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         uint32_t raw[L::kSCols];
 #pragma unroll
         for (int c = 0; c < L::kSCols; c += 16) tmem_ld16(tmem_lane + buf * L::kSCols + c, raw + c);
-        float k_scale = 1.f, v_exp = 0.f, v_scale = kPScale;
+        float k_scale = 1.f, v_exp = 0.f, v_scale = kVScale;
         // The key's own scales, and once the rows'.  (The exponents came with the keys, for which the scores waited.)
         if (i == i0) {
           if (lane < R)
@@ -360,7 +360,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           const int ek = lds_s8(at), ev = lds_s8(at + kCachedTile);
           k_scale = exponent_scale(ek);
           v_exp = static_cast<float>(ev);
-          v_scale = exponent_scale(ev) * kPScale;
+          v_scale = exponent_scale(ev) * kVScale;
         }
         tmem_wait_ld();
         tc_fence_before();
@@ -481,7 +481,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           load4(my_state + r * 4, m);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float shift = m[k] == -INFINITY ? 0.f : -m[k];
+            const float shift = m[k] == -INFINITY ? 0.f : kExpBits - m[k];
             const float e = ex2_approx(x[r + k] + shift);
             l[r + k] += e;
             p[k] = e * v_scale;
@@ -557,7 +557,7 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         w0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - m_tot);
         w1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - m_tot);
         l_tot = (l0 != 0.f ? (m0 == -INFINITY ? l0 : l0 * w0) : 0.f) + (l1 != 0.f ? (m1 == -INFINITY ? l1 : l1 * w1) : 0.f);
-        const float scale = l_tot != l_tot ? l_tot : (whole ? (l_tot > 0.f ? 1.f / l_tot : 0.f) : 1.f) / kPScale;
+        const float scale = l_tot != l_tot ? l_tot : (whole ? (l_tot > 0.f ? 1.f / l_tot : 0.f) : 1.f) / kVScale;
         w0 *= scale;
         w1 *= scale;
         if (l_tot != l_tot) w0 = w1 = l_tot;
@@ -583,9 +583,9 @@ cached_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         else static_cast<uint16_t*>(a.out)[(out_row0 + r) * D + key_lane] = static_cast<uint16_t>(pack2<BF16>(value, 0.f));
       }
       if (warp == 0 && lane < R && rt * R + lane < a.rows) {
-        if (!whole) a.part_ml[part0 + lane] = make_float2(m_tot, l_tot);
+        if (!whole) a.part_ml[part0 + lane] = make_float2(m_tot - kExpBits, l_tot);
         else if (a.lse_out)
-          a.lse_out[out_row0 + lane] = ((live >> lane) & 1u) && l_tot != 0.f ? (m_tot + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
+          a.lse_out[out_row0 + lane] = ((live >> lane) & 1u) && l_tot != 0.f ? (m_tot - kExpBits + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
       }
       step0 += n;
     }

@@ -295,7 +295,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     // Powers of 2 by which the maximum may lag behind before O is rescaled, which takes about a tile's time.  8 bit: with a
     // lag of 2^1 every third tile rescales (32 x 64 heads, 2000 to 32768 keys: 272 us), with 2^3 hardly one.
     constexpr float kThreshold = QUANT ? kCachedLag8 : 8.f;
-    constexpr float kPScale = QUANT ? kCachedPScale8 : 1.f;
+    constexpr float kVScale = QUANT ? kCachedVScale8 : 1.f, kExpBits = QUANT ? kCachedExpBits8 : 0.f;  // (see kCachedLag8)
     uint32_t sync_par = 0;
     int step0 = 0;   // tiles of the CTA in front of the segment
     bool ok = true;
@@ -425,7 +425,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
             }
             sts32(my_scales + at * 4, __float_as_uint(exponent_scale(ek)));
             sts32(my_scales + (L::kKeys + at) * 4, __float_as_uint(static_cast<float>(ev)));
-            sts32(my_scales + (2 * L::kKeys + at) * 4, __float_as_uint(exponent_scale(ev) * kPScale));
+            sts32(my_scales + (2 * L::kKeys + at) * 4, __float_as_uint(exponent_scale(ev) * kVScale));
           }
           __syncwarp();
         }
@@ -531,7 +531,7 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         sts64(m_sh, static_cast<uint64_t>(__float_as_uint(m_run)) << 32 | static_cast<uint32_t>(step));
         // P's columns are free once P.V of this warpgroup's previous tile is done.
         if (step >= 2 && !warp_wait(SPLASH_KBAR(pv_done, buf), ((step - 2) >> 1) & 1, ctx, kCSiteSmxP, step)) { ok = false; break; }
-        const float shift = m_run == -INFINITY ? 0.f : -m_run;
+        const float shift = m_run == -INFINITY ? 0.f : kExpBits - m_run;
         const float2 shift_2 = make_float2(shift, shift);
         float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
         // P is written 32 keys at a time: 16 columns of 16-bit numbers, or 8 columns of every e5m2 term, each 32 columns behind
@@ -645,16 +645,16 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       tc_fence_after();
       const bool whole = cur.whole;
       float w = m_run == -INFINITY ? 0.f : ex2_approx(m_run - m_tot);
-      w *= 1.f / kPScale;
+      w *= 1.f / kVScale;
       if (l_mine != l_mine) w = l_mine;  // NaN: no maximum may have been met
       if (whole) w *= l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
       const long long out_row0 = static_cast<long long>(b * a.kv_heads + cur.seg_head) * a.rows + rt * L::kRows;
       const long long part0 = static_cast<long long>(2 * blockIdx.x + (seg > 0)) * L::kRows;
       if (seg == 0 && threadIdx.x == 0) a.cuts[blockIdx.x] = make_int4(cur.seg_entry, cur.seg_head, cur.seg_tile, g.tiles);
       if (grp == 0 && part == 0) {
-        if (!whole) a.part_ml[part0 + r] = make_float2(m_tot, l_tot);
+        if (!whole) a.part_ml[part0 + r] = make_float2(m_tot - kExpBits, l_tot);
         else if (a.lse_out && row_all < a.rows)
-          a.lse_out[out_row0 + r] = live && l_tot != 0.f ? (m_tot + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
+          a.lse_out[out_row0 + r] = live && l_tot != 0.f ? (m_tot - kExpBits + lg2_approx(l_tot)) * kCachedLn2 : a.mask_value;
       }
       // Each warpgroup has one half of O's columns, 32 at a time: every copy's lanes leave theirs, eight threads add up the 128
       // bytes of a row.  Rows without copies stay within their warp, which waits for no other.
