@@ -4,7 +4,8 @@
 //   e = the smallest whole number in [-64, 120] with max|x| <= 448 * 2^e,   code = e4m3(x * 2^-e),   x' = code * 2^e
 // The scale is a power of two because a floating-point code loses nothing by that (its relative step is the same
 // everywhere) and everything after the one rounding of 2^-4 is exact: the product with the scale, and the 16-bit number
-// it gives.  A row with an infinity or NaN has exponent -128 and reads back as NaN throughout.
+// it gives, but at the ends of the types: f16's subnormals are rounded once more, and what was rounded up to 2^16 (f16) or 2^128
+// (bf16) reads as infinity.  A row with an infinity or NaN has exponent -128 and reads back as NaN throughout.
 //
 // Bound: HBM for long writes and reads, launch latency for single tokens.  head_dim / 8 lanes take a row, 16 bytes of
 // 16-bit numbers a lane; a row's largest magnitude is an integer maximum over the lanes (bits of |x| order like |x|,

@@ -10,7 +10,10 @@ that one write fills have to differ (a page shared by two sequences is written b
 
 An 8-bit cache holds e4m3 codes and one exponent e per (token, head): x = code * 2^e, with e the smallest whole number in
 [-64, 120] for which max|x| <= 448 * 2^e.  Storing rounds once, by at most 2^-4 of the number (or 2^-10 * 2^e);
-reading back adds nothing.  A row that holds an infinity or NaN reads back as NaN throughout.
+reading back adds nothing where the 16-bit type has that number: f16 rounds what lies among its subnormals once more, and
+what was rounded to 2^16 (f16, from 63488 on) or 2^128 (bf16, from 0.96875 * 2^128 on) reads as infinity, while attention
+over the cache has it as the finite number it is.  A row that holds an infinity or NaN reads back as NaN throughout.
+Gradients and forward-mode derivatives do not pass through a cache.
 
 No counterpart in the reference, which attends to contiguous keys.
 """
