@@ -431,7 +431,9 @@ class SplashAttentionKernel:
     heavy = -(-sinks // cfg.TILE_ROWS)
     if not 0 < heavy < len(steps):
       return 0, 1
-    parts = min(256, int(steps[0]) // max(1, int(steps[heavy])))
+    # No more shares than there are KV blocks: they take twice the memory of dK and dV in f32 (8192 sinks of 65536 keys beside a
+    # window of 128 would have 16384 shares, 2 GB for every kv head; there are other CTAs enough then).
+    parts = min(256, int(steps[0]) // max(1, int(steps[heavy])), len(steps) // heavy)
     return (heavy, parts) if parts > 1 else (0, 1)
 
   # -- device schedules ------------------------------------------------------
