@@ -137,12 +137,13 @@ def check_device_status(device=None) -> None:
 
 def _poll_status(device) -> None:
   """Start of a call: raises if the copy queued by an earlier call has landed and shows a failure.
-  Never waits for the device."""
+  Waits for the device only then."""
   mirror = _status_mirrors.get((device.type, device.index))
   if mirror is None or mirror.code.value == 0 or torch.cuda.is_current_stream_capturing():
     return
   if mirror.copied.query():
     record = mirror.host.tolist()
+    torch.cuda.synchronize(device)  # kernels queued behind the failure still find the word set, and some write the record themselves
     mirror.reset()
     _raise_device_status(_status_word(device), record)
 
