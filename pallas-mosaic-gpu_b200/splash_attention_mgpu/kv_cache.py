@@ -26,7 +26,7 @@ import dataclasses
 import torch
 
 from . import _ffi
-from .splash_attention import _TORCH_DTYPES, _launch
+from .splash_attention import _TORCH_DTYPES, _launch, _set_up_status
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
@@ -100,6 +100,8 @@ class KVCache:
       raise NotImplementedError(f"caches are bf16, f16 or float8_e4m3fn, got {self.k.dtype}")
     elif self.k_exponent is not None or self.v_exponent is not None:
       raise ValueError("exponents belong to 8-bit caches")
+    if self.k.is_cuda:
+      _set_up_status(self.k.device)
 
   @property
   def quantized(self) -> bool:

@@ -75,8 +75,17 @@ def _status_word(device: torch.device) -> torch.Tensor:
   """The 4-int status word the kernels report into (one per device)."""
   key = (device.type, device.index)
   if key not in _status_words:
+    if torch.cuda.is_current_stream_capturing():  # (it would be the graph's memory, and cleared at every replay)
+      raise RuntimeError("the first call on a device sets up its status word, which cannot be done during a stream capture")
     _status_words[key] = torch.zeros(4, dtype=torch.int32, device=device)
   return _status_words[key]
+
+
+def _set_up_status(device: torch.device) -> None:
+  """What calls on a device report through, made ahead of a first call that may be captured."""
+  if not torch.cuda.is_current_stream_capturing():
+    _status_word(device)
+    _status_host(device)
 
 
 def _on_device(device: torch.device):

@@ -1,7 +1,11 @@
-"""The status word and attention over the cache: one report for one failure.
+"""The status word and attention over the cache: one report for one failure, and no word made inside a graph.
 
 As in test_gpu_status.py no kernel is made to time out: the word is set from the host."""
 
+import os
+import subprocess
+import sys
+import textwrap
 import time
 
 import pytest
@@ -10,6 +14,8 @@ import torch
 import splash_attention_mgpu as sa
 from splash_attention_mgpu import _ffi
 from splash_attention_mgpu import splash_attention as api
+
+from conftest import ROOT
 
 DEV = "cuda:0"
 
@@ -48,3 +54,38 @@ def test_gpu_calls_still_queued_do_not_report_again(monkeypatch):
   torch.cuda.synchronize()
   sa.check_device_status()
   assert torch.equal(again, good)
+
+
+@pytest.mark.gpu
+def test_gpu_first_call_of_a_process_in_a_capture():
+  code = """
+    import torch
+    import test_gpu_status_of_cached as t
+    import splash_attention_mgpu as sa
+    from splash_attention_mgpu import splash_attention as api
+    q, cache, table, lens = t._serving()
+    words, mirrors = dict(api._status_words), dict(api._status_mirrors)
+    assert words and mirrors  # there before the capture
+    attend, graph = sa.make_splash_cached(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+      captured = attend(q, cache, table, lens)
+    assert words == api._status_words
+    eager = attend(q, cache, table, lens)  # before the graph has ever run
+    sa.check_device_status()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert eager.any() and torch.equal(eager, captured)
+    print("fine")
+  """
+  path = f"import sys; sys.path[:0] = [{ROOT + '/tests'!r}, {ROOT + '/pallas-mosaic-gpu_b200'!r}, {ROOT!r}]\n"
+  done = subprocess.run([sys.executable, "-c", path + textwrap.dedent(code)], capture_output=True, text=True, timeout=300,
+                        env={**os.environ, "SPLASH_CHECK_STATUS": "async"})
+  assert done.returncode == 0 and "fine" in done.stdout, done.stderr[-2000:]
+
+
+def test_no_word_is_made_in_a_capture(monkeypatch):
+  monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+  monkeypatch.setattr(api, "_status_words", {})
+  with pytest.raises(RuntimeError, match="capture"):
+    api._status_word(torch.device("cpu"))
+  assert not api._status_words
