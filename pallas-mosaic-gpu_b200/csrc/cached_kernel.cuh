@@ -295,7 +295,10 @@ cached_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     // Powers of 2 by which the maximum may lag behind before O is rescaled, which takes about a tile's time.  8 bit: with a
     // lag of 2^1 every third tile rescales (32 x 64 heads, 2000 to 32768 keys: 272 us), with 2^3 hardly one.
     constexpr float kThreshold = QUANT ? kCachedLag8 : 8.f;
-    constexpr float kVScale = QUANT ? kCachedVScale8 : 1.f, kExpBits = QUANT ? kCachedExpBits8 : 0.f;  // (see kCachedLag8)
+    // Powers of 2 that the exponentials, and with them the sums and O, are scaled by.  8 bit: see kCachedLag8.  An f16 P has steps of
+    // 2^-24 at the least: with a row's largest at 2^7 or above, and below 2^16, that is 2^-31 of it (131072 keys of weight 2^-20
+    // beside a large one: results off by 3 % without).
+    constexpr float kVScale = QUANT ? kCachedVScale8 : 1.f, kExpBits = QUANT ? kCachedExpBits8 : BF16 ? 0.f : 7.f;
     uint32_t sync_par = 0;
     int step0 = 0;   // tiles of the CTA in front of the segment
     bool ok = true;
