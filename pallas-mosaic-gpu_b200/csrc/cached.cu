@@ -115,8 +115,8 @@ static CachedPlan cached_plan(const SplashCachedParams& p) {
   plan.row_cap = few ? (rows <= 8 ? 8 : 16) : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   // A unit stands in the line by as many tiles more as its start and the sum of its parts take.  us for 64 sequences of 100 to
   // 3000 keys, 8 kv heads, head_dim 128, with a cost of 2 | 4 | 8 | 12: 4 rows 80 | 80 | 82 | 86, 128 rows 138 | 124 | 113 |
-  // 113; 8 bit: 4 rows 68 | 63 | 57 | 61, 16 rows 81 | 72 | 75 | 81, 64 rows 153 | 126 | 106 | 105.  Contexts of 30000 keys and
-  // more move by 1 % at most.
+  // 113; 8 bit, with L2 flushed: 4 rows 78 | 68 | 67 | 70 (6: 66), 16 rows 100 | 90 | 82 | 84 (6: 84), 32 rows 109 | 98 | 100 | 109,
+  // 64 rows 162 | 139 | 135 | 141, 128 rows 277 | 238 | 229 | 238.  Contexts of 8192 keys and more move by 3 % at most.
   plan.unit_cost = plan.row_cap == 128 || (p.quantized && plan.row_cap == 64) ? 8 : few ? 6 : 4;
   plan.row_tiles = static_cast<int>((rows + plan.row_cap - 1) / plan.row_cap);
   const int64_t entries = static_cast<int64_t>(p.batch) * plan.row_tiles;

@@ -7,7 +7,8 @@
     out, (lse,) = attend(q, cache, page_table, lengths, save_residuals=True)
 
 The serving counterpart of `make_splash_mha` with `CausalMask` / `LocalMask`: the same window (`LocalMask`'s left side), the
-same sinks, soft-cap and treatment of rows that see no key (zeros and lse = mask_value).  Forward only.  Lengths, page
+same sinks, soft-cap and treatment of rows that see no key (zeros and lse = mask_value).  Forward only.  What no row of a call
+sees may be anything; a value that one of them sees and that is infinite or NaN reaches the others too (0 times it is NaN).  Lengths, page
 tables and trees stay on the device; a call synchronises nothing and can be captured into a graph.
 
 No counterpart in the reference, which attends to contiguous keys in multiples of a block.
