@@ -70,6 +70,7 @@ typedef struct SplashParams {
   /* [mask_heads, 4] int32 {lo, hi, chunk, sinks}: a key is visible iff
    * (lo <= kv_pos - q_pos or kv_pos < sinks) and kv_pos - q_pos <= hi and
    * (chunk == 0 or q_pos/chunk == kv_pos/chunk).  With a chunk, sinks is 0.
+   * Bounds beyond -2^30 and 2^30 count as those.
    * NULL when partial blocks are dense or when there are no partial blocks. */
   const int32_t* mask_desc;
   /* ---- results ------------------------------------------------------------ */
